@@ -149,6 +149,11 @@ SYMBOLS = [
     ("ab_blockpool_grow", C.c_int, [_P, _P, C.c_int, C.c_int]),
     ("ab_blockpool_free", C.c_int, [_P, _P, C.c_int]),
     ("ab_blockpool_positions", C.c_int, [_P, C.c_int]),
+    ("ab_blockpool_share", C.c_int, [_P, _P, C.c_int]),
+    ("ab_blockpool_refs", C.c_int, [_P, C.c_uint32]),
+    ("ab_blockpool_own", C.c_int, [_P, _P, C.c_int, _P, _P]),
+    ("ab_blockpool_compact", C.c_int, [_P, _P, _P]),
+    ("ab_cache_copy_pages", C.c_int, [_P, _P, C.c_int, C.c_size_t, C.c_uint32, _P, _P, C.c_int]),
     ("ab_int4_prepack_bytes", C.c_size_t, [C.c_uint32, C.c_uint32]),
     ("ab_int4_prepack", C.c_int, [_P, _P, _P, _P, C.c_uint32, C.c_uint32, _P]),
     ("ab_int4_stream_error", C.c_int, []),

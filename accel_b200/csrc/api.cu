@@ -122,6 +122,16 @@ static const KernelEntry kKernels[] = {
     {"AttentionPrefillF16", 5, 32, launch_attention_prefill_f16},
     {"AttentionPrefillPaged", 6, 32, launch_attention_prefill_paged},
     {"AttentionPrefillPagedF16", 6, 32, launch_attention_prefill_paged_f16},
+    {"AttentionWindow", 5, 48, launch_attention_window},
+    {"AttentionWindowF16", 5, 48, launch_attention_window_f16},
+    {"AttentionWindowBatched", 6, 48, launch_attention_window_batched},
+    {"AttentionWindowBatchedF16", 6, 48, launch_attention_window_batched_f16},
+    {"AttentionWindowRagged", 7, 48, launch_attention_window_ragged},
+    {"AttentionWindowRaggedF16", 7, 48, launch_attention_window_ragged_f16},
+    {"AttentionWindowPrefill", 5, 48, launch_attention_window_prefill},
+    {"AttentionWindowPrefillF16", 5, 48, launch_attention_window_prefill_f16},
+    {"AttentionWindowPrefillPaged", 6, 48, launch_attention_window_prefill_paged},
+    {"AttentionWindowPrefillPagedF16", 6, 48, launch_attention_window_prefill_paged_f16},
     {"GroupedMatVec", 4, 16, launch_grouped_matvec},
     {"GroupedMatMul", 4, 16, launch_grouped_matmul},
     {"GroupedMatMulInt4", 6, 16, launch_grouped_matmul_int4},
@@ -138,6 +148,8 @@ static const KernelEntry kKernels[] = {
     {"SampleArgmax", 2, 16, launch_sample_argmax},
     {"ArgmaxShard", 2, 32, launch_argmax_shard},
     {"ArgmaxMerge", 2, 16, launch_argmax_merge},
+    {"TokenLogprobs", 6, 16, launch_token_logprobs},
+    {"TokenLogprobsF16", 6, 16, launch_token_logprobs_f16},
     {"Softmax", 2, 16, launch_softmax},
     {"ScaleRows", 3, 16, launch_scale_rows},
     {"LogitBias", 4, 16, launch_logit_bias},
@@ -305,6 +317,10 @@ static size_t elem_bytes_of(const char *k, int i)
     if (is("AttentionDecodeF16") || is("AttentionDecodePagedF16") || is("AttentionDecodeBatchedF16") ||
         is("AttentionDecodeBatchedF16Max") || is("AttentionRaggedF16"))
         return (i == 1 || i == 2) ? 2 : 4;
+    if (is("AttentionWindowF16") || is("AttentionWindowBatchedF16") || is("AttentionWindowRaggedF16") ||
+        is("AttentionWindowPrefillF16") || is("AttentionWindowPrefillPagedF16"))
+        return (i == 1 || i == 2) ? 2 : 4;
+    if (is("TokenLogprobsF16")) return i == 0 ? 2 : 4;
     if (is("ScatterRowsF16")) return (i == 0 || i == 2) ? 2 : 4;
     if (is("GatherRowsF16")) return i == 0 ? 2 : 4;
     if (is("CastF32ToF16")) return i == 1 ? 2 : 4;
@@ -1033,6 +1049,7 @@ struct ab_blockpool {
     int total;
     std::mutex mu;
     std::vector<uint32_t> free_list;
+    std::vector<uint32_t> refs;      // how many page rows hold each block; 0 = free
 };
 
 extern "C" {
@@ -1045,6 +1062,7 @@ int ab_blockpool_new(int blocks, int per, ab_blockpool **out)
     if (!p) return fail(AB_ERR_OOM, "ab_blockpool_new: host allocation failed");
     p->block = per; p->total = blocks;
     p->free_list.resize((size_t)blocks);
+    p->refs.assign((size_t)blocks, 0);
     for (int i = 0; i < blocks; i++) p->free_list[(size_t)i] = (uint32_t)(blocks - 1 - i);
     *out = p;
     return AB_OK;
@@ -1074,6 +1092,7 @@ int ab_blockpool_grow(ab_blockpool *p, uint32_t *pages, int n_pages, int n)
                     "make for you", n, need, p->free_list.size());
     // the new pages are the tail of the free list, in list order; earlier pages never move
     std::copy(p->free_list.end() - need, p->free_list.end(), pages + n_pages);
+    for (int i = n_pages; i < want; i++) p->refs[pages[i]] = 1;
     p->free_list.resize(p->free_list.size() - (size_t)need);
     return want;
 }
@@ -1082,18 +1101,83 @@ int ab_blockpool_free(ab_blockpool *p, const uint32_t *pages, int n_pages)
 {
     if (!p || n_pages < 0 || (n_pages && !pages)) return fail(AB_ERR_INVALID, "ab_blockpool_free: bad argument");
     std::lock_guard<std::mutex> lk(p->mu);
-    std::vector<bool> held((size_t)p->total, false);
-    for (uint32_t f : p->free_list) held[f] = true;
     int bad = 0;
     uint32_t first_bad = 0;
     for (int i = 0; i < n_pages; i++) {
         const uint32_t pg = pages[i];
-        if (pg >= (uint32_t)p->total || held[pg]) { if (!bad) first_bad = pg; bad++; continue; }
-        held[pg] = true;
-        p->free_list.push_back(pg);
+        if (pg == AB_PAGE_NONE) continue;
+        if (pg >= (uint32_t)p->total || p->refs[pg] == 0) { if (!bad) first_bad = pg; bad++; continue; }
+        if (--p->refs[pg] == 0) p->free_list.push_back(pg);
     }
     if (bad) return fail(AB_ERR_INVALID, "block %u is already free (%d such block(s))", first_bad, bad);
     return AB_OK;
+}
+
+int ab_blockpool_share(ab_blockpool *p, const uint32_t *pages, int n_pages)
+{
+    if (!p || n_pages < 0 || (n_pages && !pages)) return fail(AB_ERR_INVALID, "ab_blockpool_share: bad argument");
+    std::lock_guard<std::mutex> lk(p->mu);
+    for (int i = 0; i < n_pages; i++)
+        if (pages[i] != AB_PAGE_NONE && (pages[i] >= (uint32_t)p->total || p->refs[pages[i]] == 0))
+            return fail(AB_ERR_INVALID, "block %u is free; only a held block can be shared", pages[i]);
+    for (int i = 0; i < n_pages; i++)
+        if (pages[i] != AB_PAGE_NONE) p->refs[pages[i]]++;
+    return AB_OK;
+}
+
+int ab_blockpool_refs(ab_blockpool *p, uint32_t page)
+{
+    if (!p || page >= (uint32_t)p->total) return fail(AB_ERR_INVALID, "block %u of a pool of %d", page, p ? p->total : 0);
+    std::lock_guard<std::mutex> lk(p->mu);
+    return (int)p->refs[page];
+}
+
+int ab_blockpool_own(ab_blockpool *p, uint32_t *pages, int n_pages, uint32_t *src, uint32_t *dst)
+{
+    if (!p || n_pages < 0 || (n_pages && (!pages || !src || !dst))) return fail(AB_ERR_INVALID, "ab_blockpool_own: bad argument");
+    std::lock_guard<std::mutex> lk(p->mu);
+    size_t need = 0;
+    for (int i = 0; i < n_pages; i++) {
+        if (pages[i] == AB_PAGE_NONE) continue;
+        if (pages[i] >= (uint32_t)p->total || p->refs[pages[i]] == 0)
+            return fail(AB_ERR_INVALID, "block %u is free; only a held block can be written", pages[i]);
+        need += p->refs[pages[i]] > 1;
+    }
+    if (need > p->free_list.size())
+        return fail(AB_ERR_OOM, "%zu shared block(s) to copy and %zu are free; the pool does not evict", need, p->free_list.size());
+    int n = 0;
+    for (int i = 0; i < n_pages; i++) {
+        const uint32_t pg = pages[i];
+        if (pg == AB_PAGE_NONE || p->refs[pg] < 2) continue;
+        const uint32_t to = p->free_list.back();
+        p->free_list.pop_back();
+        p->refs[pg]--;
+        p->refs[to] = 1;
+        src[n] = pg; dst[n] = to;
+        n++;
+        pages[i] = to;
+    }
+    return n;
+}
+
+int ab_blockpool_compact(ab_blockpool *p, uint32_t *src, uint32_t *dst)
+{
+    if (!p || !src || !dst) return fail(AB_ERR_INVALID, "ab_blockpool_compact: bad argument");
+    std::lock_guard<std::mutex> lk(p->mu);
+    const uint32_t live = (uint32_t)p->total - (uint32_t)p->free_list.size();
+    int n = 0;
+    uint32_t to = 0;
+    for (uint32_t pg = live; pg < (uint32_t)p->total; pg++) {
+        if (p->refs[pg] == 0) continue;
+        while (p->refs[to]) to++;             // as many free blocks below `live` as held ones above it
+        src[n] = pg; dst[n] = to;
+        n++;
+        p->refs[to] = p->refs[pg];
+        p->refs[pg] = 0;
+    }
+    // the free blocks are now [live, total), handed out from the lowest as a new pool does
+    for (size_t i = 0; i < p->free_list.size(); i++) p->free_list[i] = (uint32_t)p->total - 1 - (uint32_t)i;
+    return n;
 }
 
 int ab_blockpool_positions(ab_blockpool *p, int n_pages) { return p ? n_pages * p->block : 0; }

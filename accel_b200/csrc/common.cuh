@@ -162,6 +162,18 @@ int launch_attention_prefill(Launch &);
 int launch_attention_prefill_f16(Launch &);
 int launch_attention_prefill_paged(Launch &);
 int launch_attention_prefill_paged_f16(Launch &);
+int launch_attention_window(Launch &);
+int launch_attention_window_f16(Launch &);
+int launch_attention_window_batched(Launch &);
+int launch_attention_window_batched_f16(Launch &);
+int launch_attention_window_ragged(Launch &);
+int launch_attention_window_ragged_f16(Launch &);
+int launch_attention_window_prefill(Launch &);
+int launch_attention_window_prefill_f16(Launch &);
+int launch_attention_window_prefill_paged(Launch &);
+int launch_attention_window_prefill_paged_f16(Launch &);
+int launch_token_logprobs(Launch &);
+int launch_token_logprobs_f16(Launch &);
 int launch_grouped_matvec(Launch &);
 int launch_grouped_matmul(Launch &);
 int launch_grouped_matmul_int4(Launch &);

@@ -44,6 +44,8 @@ class ModelConfig:
     rope_base: float = 10000.0
     block: int = 16               # positions per KV page
     cache_dtype: torch.dtype = torch.float32
+    window: int = 0               # attention sees the last `window` positions and the first `sinks`; 0: all of them
+    sinks: int = 0
 
     def int4_weights(self) -> int:
         d, f = self.d_model, self.ffn
@@ -356,10 +358,54 @@ class DecodeEngine:
         self.page_rows[seq] = self.pool.grow(self.page_rows[seq], n_positions)
 
     def upload_pages(self):
-        host = np.zeros((self.batch, self.max_pages), np.int32)
+        host = np.zeros((self.batch, self.max_pages), np.uint32)
         for s, row in enumerate(self.page_rows):
             host[s, :len(row)] = row
-        self.pages.copy_(torch.from_numpy(host))
+        self.pages.copy_(torch.from_numpy(host.view(np.int32)))
+
+    def trim(self):
+        """Gives the pages behind the attention window back to the pool (BlockPool.trim), for every
+        sequence at its current length; the sinks' pages stay."""
+        if not self.cfg.window:
+            raise ValueError("the model has no attention window: every position stays visible")
+        self.page_rows = [self.pool.trim(row, int(n), self.cfg.window, self.cfg.sinks)
+                          for row, n in zip(self.page_rows, self.lengths_host)]
+        self.upload_pages()
+
+    def _copy_pages(self, src: List[int], dst: List[int]):
+        if src:
+            from .tensor import copy_pages
+            copy_pages([*self.k_cache, *self.v_cache], src, dst, self.cfg.block)
+
+    def fork(self, src: int, dst: int):
+        """Makes sequence `dst` a copy of sequence `src` as it stands (a beam, another sample of one
+        prompt): what dst held is freed, the filled pages are shared, and only a partly filled last
+        page is copied, since both go on writing there.  dst gets as many reserved positions as src.
+        The next step's inputs are the caller's to set for both (step, or set_inputs)."""
+        if src == dst or not 0 <= src < self.batch or not 0 <= dst < self.batch:
+            raise ValueError(f"fork of sequence {src} to {dst} in a batch of {self.batch}")
+        n, blk = int(self.lengths_host[src]), self.cfg.block
+        reserved = len(self.page_rows[src]) * blk
+        self.pool.free(self.page_rows[dst])
+        self.page_rows[dst], self.lengths_host[dst] = [], 0
+        row = self.pool.share(self.page_rows[src][:(n + blk - 1) // blk])
+        try:
+            row, s, d = self.pool.own(row, n, n + 1)
+            row = self.pool.grow(row, reserved)
+        except Exception:
+            self.pool.free(row)
+            raise
+        self._copy_pages(s, d)
+        self.page_rows[dst], self.lengths_host[dst] = row, n
+        self.upload_pages()
+
+    def compact(self) -> int:
+        """Moves the pages in use to the pool's lowest numbers and returns how many moved; afterwards the
+        caches hold nothing beyond the first (pages in use) * block positions."""
+        self.page_rows, s, d = self.pool.compact(self.page_rows)
+        self._copy_pages(s, d)
+        self.upload_pages()
+        return len(s)
 
     def fill_context(self, context: int, seed: int = 7):
         """Stands in for a prefill: reserves pages for `context` positions per sequence and fills
@@ -445,6 +491,11 @@ class DecodeEngine:
                        _u("<IIIIIIfI", m, self.hq, self.hk, D, D, self.capacity, cfg.rope_base, 0))
                 for sq in range(B):
                     rows = slice(sq * s_now, (sq + 1) * s_now)
+                    if cfg.window:
+                        launch("AttentionWindowPrefillPagedF16" if f16 else "AttentionWindowPrefillPaged",
+                               [q[rows], self.k_cache[li], self.v_cache[li], pages_of[sq], kv_len, attn[rows]],
+                               self._window_dims(1, s_now, p0))
+                        continue
                     launch("AttentionPrefillPagedF16" if f16 else "AttentionPrefillPaged",
                            [q[rows], self.k_cache[li], self.v_cache[li], pages_of[sq], kv_len, attn[rows]],
                            _u("<IIIIIIfI", self.hq, self.hk, D, s_now, p0, blk, scale, 0))
@@ -459,6 +510,12 @@ class DecodeEngine:
         t1.synchronize()
         self.lengths_host += T
         return t0.elapsed_time(t1) / 1e3
+
+    def _window_dims(self, batch: int, q_seq: int, base: int) -> bytes:
+        cfg = self.cfg
+        return rt.window_dims(batch, self.hq, self.hk, cfg.head_dim, cfg.block, self.max_pages,
+                              float(np.float32(1.0) / np.float32(np.sqrt(cfg.head_dim))), cfg.window, cfg.sinks,
+                              self.capacity, q_seq, base)
 
     def step_inputs_host(self, token_ids: np.ndarray) -> np.ndarray:
         """The per-step host buffers for the CURRENT lengths, laid out as `self.inputs` is:
@@ -633,7 +690,10 @@ class DecodeEngine:
                   _u("<IIIIIIfI", B, self.hq, self.hk, D, D, self.capacity, cfg.rope_base, 0))
             attn_u = _u("<IIIIIIfI", B, self.hq, self.hk, D, cfg.block, self.max_pages, scale, 0)
             attn_b = [self.q, self.k_cache[li], self.v_cache[li], self.pages, self.lengths, self.attn]
-            if maxima:
+            if cfg.window:
+                L("AttentionWindowBatchedF16" if f16 else "AttentionWindowBatched", attn_b, self._window_dims(B, 1, 0))
+                self._linear(self.attn, lay.wo_p if self.use_packed else lay.wo, self._proj[0])
+            elif maxima:
                 # the kernel that writes a product's input also leaves its rows' largest magnitudes
                 L("AttentionDecodeBatchedF16Max" if f16 else "AttentionDecodeBatchedMax", attn_b + [self.attn_max], attn_u)
                 w = lay.wo_p
@@ -706,6 +766,13 @@ class DecodeEngine:
         dist.all_gather(parts, mine, group=self.group)
         return torch.cat([parts[r][:, :widths[r]] for r in range(self.shard.tp)], dim=1)
 
+    def score(self, targets: Optional[torch.Tensor] = None, top: int = 0):
+        """Log probabilities of `targets` (u32 [batch], or [batch, n]) under the last step's logits, each
+        sequence's entropy and its `top` most probable tokens (tensor.token_logprobs).  With the
+        vocabulary split over ranks this is a collective, as full_logits is."""
+        from .tensor import token_logprobs
+        return token_logprobs(self.full_logits(), targets, top)
+
     def prepare(self):
         if self.cfg.cache_dtype == torch.float16 and not hasattr(self, "_k16"):
             self._k16 = torch.zeros_like(self.k, dtype=torch.float16)
@@ -770,10 +837,13 @@ class DecodeEngine:
         return 4 * self.batch
 
     def kv_bytes_read_per_step(self) -> int:
-        """Algorithmic K/V bytes one step reads on this rank: every cached position of every
+        """Algorithmic K/V bytes one step reads on this rank: every visible position of every
         sequence, K and V, once per KV head, in every layer."""
         e = 2 if self.cfg.cache_dtype == torch.float16 else 4
-        return int(self.cfg.layers * 2 * self.hk * self.cfg.head_dim * e * (self.lengths_host + 1).sum())
+        seen = self.lengths_host + 1
+        if self.cfg.window:
+            seen = np.minimum(seen, self.cfg.window + np.minimum(self.cfg.sinks, np.maximum(seen - self.cfg.window, 0)))
+        return int(self.cfg.layers * 2 * self.hk * self.cfg.head_dim * e * seen.sum())
 
 
 class SeamStep:

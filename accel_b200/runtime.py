@@ -42,6 +42,16 @@ def paged_prefill_dims(q_heads, kv_heads, head_dim, q_seq, base, block, scale) -
     return struct.pack("<IIIIIIfI", q_heads, kv_heads, head_dim, q_seq, base, block, scale, 0)
 
 
+def window_dims(batch, q_heads, kv_heads, head_dim, block, max_pages, scale, window, sinks, capacity, q_seq, base) -> bytes:
+    # WindowDims: the window forms' own block
+    return struct.pack("<IIIIIIfIIIII", batch, q_heads, kv_heads, head_dim, block, max_pages, scale, window, sinks,
+                       capacity, q_seq, base)
+
+
+def logprob_dims(vocab, rows, targets, top) -> bytes:
+    return struct.pack("<IIII", vocab, rows, targets, top)
+
+
 def grouped_dims(experts, K, N) -> bytes:                       # GroupedDims, grouped.go:10
     return struct.pack("<IIII", experts, K, N, 0)
 
@@ -139,6 +149,41 @@ def launch(name: str, bindings: Sequence[torch.Tensor], uniform: Optional[bytes]
                          C.c_void_p(workspace.data_ptr()) if workspace is not None else None,
                          workspace.numel() if workspace is not None else 0)
     _lib.check(rc)
+
+
+def launch_own(name: str, bindings: Sequence[torch.Tensor], uniform: bytes):
+    """`launch` for the operators whose scratch memory is the call's own: it comes from torch's
+    allocator, so a call captured into a CUDA graph keeps it in that graph's pool and two graphs, or
+    two streams, never share it.  A binding of more elements than 32 bits count is passed as
+    0xffffffff, which those kernels read as that many or more."""
+    dev = bindings[0].device
+    lens = [min(t.numel(), 0xffffffff) for t in bindings]
+    ws = None
+    if dev.type == "cuda":
+        need = workspace_bytes(name, lens, uniform)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    launch(name, bindings, uniform, lens, ws)
+
+
+def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], block: int):
+    """ab_cache_copy_pages on the current stream of the caches' device."""
+    L = _lib.lib()
+    dev, n = caches[0].device, len(src)
+    if dev.type != "cuda":
+        raise _lib.AccelError(_lib.AB_ERR_NO_DEVICE, f"copy_pages: the caches live on {dev}; this backend runs on a CUDA "
+                              "device and has no CPU path")
+    if any(not 0 <= p < 0xffffffff for p in (*src, *dst)):
+        raise _lib.AccelError(_lib.AB_ERR_INVALID, "copy_pages: a page id is u32")
+    t = caches[0]
+    page_bytes = t.stride(0) * t.element_size() * block if t.numel() else 0
+    if page_bytes == 0:
+        if n:
+            raise _lib.AccelError(_lib.AB_ERR_INVALID, "copy_pages: the caches are empty")
+        return
+    ptrs = (C.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
+    with torch.cuda.device(dev):
+        _lib.check(L.ab_cache_copy_pages(C.c_void_p(torch.cuda.current_stream(dev).cuda_stream), ptrs, len(caches), page_bytes,
+                                         t.shape[0] // block, (C.c_uint32 * n)(*src), (C.c_uint32 * n)(*dst), n))
 
 
 def last_selection() -> str:

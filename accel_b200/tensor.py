@@ -8,7 +8,7 @@ poisons the result rather than running."""
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -17,7 +17,8 @@ from .quant import INT4_GROUP
 
 __all__ = ["Refused", "Int4", "int4_matvec", "int4_matmul", "AttentionOptions", "attention",
            "grouped_matvec", "grouped_matmul", "grouped_matmul_int4", "segment_offsets",
-           "scatter_rows", "gather_rows", "rms_norm", "rope", "swiglu", "add", "argmax", "cast"]
+           "scatter_rows", "gather_rows", "rms_norm", "rope", "swiglu", "add", "argmax", "cast",
+           "copy_pages", "TokenLogprobs", "token_logprobs"]
 
 U32 = torch.int32       # torch has no general uint32 arithmetic; the bits are what the kernels read
 
@@ -32,6 +33,13 @@ class Refused(ValueError):
 
 def _is_u32(t: torch.Tensor) -> bool:
     return t.dtype in (torch.int32, torch.uint32)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor on a 16-byte boundary, which every binding is: a row of a larger tensor may
+    start anywhere."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 # ------------------------------------------------------------------------------- int4 linear
@@ -178,6 +186,10 @@ class AttentionOptions:
     scale: float = 1.0
     query_extents: Optional[torch.Tensor] = None
     base: Optional[int] = None     # stands for BaseName: the cache position of a prefill's first query token
+    # a sliding window (no reference counterpart): a query sees the last `window` positions, its own among
+    # them, and the first `sinks` positions of the sequence; 0 is no window
+    window: int = 0
+    sinks: int = 0
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: AttentionOptions) -> torch.Tensor:
@@ -185,7 +197,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
     token; [batch, 1, qHeads, D] with Pages the batched decode (f32 cache; an f16 cache runs the
     batched-f16 extension); [tokens, qHeads, D] with QueryExtents the ragged step; [qSeq, qHeads, D]
     without it a causal prefill of one sequence (Base required; paged when Pages is set).
-    k and v are the caches, [capacity, kvHeads, D], f32 or f16."""
+    k and v are the caches, [capacity, kvHeads, D], f32 or f16.  With opts.window every form masks the
+    positions further back than the window, but for the first opts.sinks of the sequence; page-table
+    entries of pages that no query sees are not read (BlockPool.trim frees such pages)."""
     op = "Attention"
     if q.dtype != torch.float32:
         raise Refused(op, f"q is {q.dtype} and the registered kernels read an f32 query")
@@ -245,20 +259,41 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
     if opts.lengths.numel() != batch:
         raise Refused(op, f"Lengths holds {opts.lengths.numel()} entries and this step has {batch} "
                       "sequence(s); it is one length per sequence")
+    for name, n in (("Window", opts.window), ("Sinks", opts.sinks)):
+        if not isinstance(n, int) or isinstance(n, bool) or not 0 <= n < 1 << 32:
+            raise Refused(op, f"{name} is {n!r}; it is a number of positions")
+    if opts.sinks and not opts.window:
+        raise Refused(op, f"Sinks is {opts.sinks} and Window is 0; without a window every position is visible")
     k, v = k.contiguous(), v.contiguous()
     scale = float(opts.scale)
+
+    def windowed(form, rows, max_pages=0, base=0, pages=None, offsets=None):
+        """The windowed kernel of a form whose arguments have been checked."""
+        out = torch.empty((rows, q_heads, head_dim), dtype=torch.float32, device=q.device)
+        if rows and q_heads and head_dim:
+            b = [q, k, v] + [_aligned(t) for t in (pages, opts.lengths, offsets) if t is not None] + [out]
+            rt.launch_own("AttentionWindow" + form + ("F16" if f16 else ""), b,
+                          rt.window_dims(batch, q_heads, kv_heads, head_dim, opts.block, max_pages, scale, opts.window,
+                                         opts.sinks, k.shape[0], rows, base))
+        return out
 
     if prefill:
         if opts.base is None:
             raise Refused(op, "a prefill needs BaseName: the position of its first query token within "
                           "the cache, which is what the causal mask is measured from")
+        if opts.pages is not None and opts.pages.dim() != 1 and (q_seq or opts.window):
+            raise Refused(op, f"Pages is {tuple(opts.pages.shape)}; a prefill is one sequence, whose "
+                          "page table is one row of block ids")
+        if opts.window:
+            if not 0 <= int(opts.base) <= 0xffffffff - q_seq:
+                raise Refused(op, f"Base is {opts.base} and q holds {q_seq} rows; positions are u32")
+            if opts.pages is None:
+                return windowed("Prefill", q_seq, base=int(opts.base))
+            return windowed("PrefillPaged", q_seq, opts.pages.numel(), int(opts.base), opts.pages)
         out = torch.empty((q_seq, q_heads, head_dim), dtype=torch.float32, device=q.device)
         if q_seq == 0:
             return out
         if opts.pages is not None:
-            if opts.pages.dim() != 1:
-                raise Refused(op, f"Pages is {tuple(opts.pages.shape)}; a prefill is one sequence, whose "
-                              "page table is one row of block ids")
             rt.launch("AttentionPrefillPagedF16" if f16 else "AttentionPrefillPaged",
                       [q, k, v, opts.pages.contiguous(), opts.lengths, out],
                       rt.paged_prefill_dims(q_heads, kv_heads, head_dim, q_seq, int(opts.base), opts.block, scale))
@@ -276,6 +311,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
                           "sequences; a page table is [batch, maxPages]")
         tokens = q.shape[0]
         offsets = segment_offsets(opts.query_extents)
+        if opts.window:
+            return windowed("Ragged", tokens, opts.pages.shape[1], pages=opts.pages, offsets=offsets)
         out = torch.empty((tokens, q_heads, head_dim), dtype=torch.float32, device=q.device)
         if tokens:
             rt.launch("AttentionRaggedF16" if f16 else "AttentionRagged",
@@ -294,6 +331,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
             raise Refused(op, f"Pages is {tuple(opts.pages.shape)} and the batch is {batch}; a "
                           "batched page table is [batch, maxPages], one row of block ids per "
                           "sequence")
+        if opts.window:
+            return windowed("Batched", batch, opts.pages.shape[1], pages=opts.pages)
         out = torch.empty((batch, q_heads, head_dim), dtype=torch.float32, device=q.device)
         if batch:
             rt.launch("AttentionDecodeBatchedF16" if f16 else "AttentionDecodeBatched",
@@ -301,6 +340,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
                       rt.batched_dims(batch, q_heads, kv_heads, head_dim, opts.block,
                                       opts.pages.shape[1], scale))
         return out
+    if opts.window:
+        if opts.pages is not None and opts.pages.dim() != 1:
+            raise Refused(op, f"Pages is {tuple(opts.pages.shape)}; one token's page table is one row of block ids")
+        if opts.pages is None:
+            return windowed("", 1)[0]
+        return windowed("Batched", 1, opts.pages.numel(), pages=opts.pages)[0]
     out = torch.empty((q_heads, head_dim), dtype=torch.float32, device=q.device)
     if opts.pages is not None:
         rt.launch("AttentionDecodePagedF16" if f16 else "AttentionDecodePaged",
@@ -519,6 +564,78 @@ def cast(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
         raise Refused("Cast", f"{x.dtype} to {dtype}; f32 and f16 are built")
     if x.numel():
         rt.launch(name, [x.contiguous(), out])
+    return out
+
+
+# ------------------------------------------------------------------------------- cache pages
+def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], block: int) -> None:
+    """Copies whole pages inside every one of `caches` (the key and value caches of all layers,
+    [capacity, ...] each, of one shape and dtype): positions [dst[i] * block, (dst[i] + 1) * block)
+    become those of src[i], as BlockPool.own and BlockPool.compact ask for.  src and dst are host
+    numbers; a page that is written twice, or both written and read, is refused.  No reference
+    counterpart."""
+    op = "CopyPages"
+    caches = list(caches)
+    if len(src) != len(dst):
+        raise Refused(op, f"{len(src)} source pages and {len(dst)} destination pages")
+    if not isinstance(block, int) or block <= 0:
+        raise Refused(op, f"Block is {block!r}; it is how many positions a page holds")
+    if not caches:
+        return
+    first = caches[0]
+    seen = set()
+    for c in caches:
+        if c.dim() < 1 or c.shape != first.shape or c.dtype != first.dtype or c.device != first.device:
+            raise Refused(op, f"the caches are {tuple(first.shape)} {first.dtype} on {first.device} and {tuple(c.shape)} "
+                          f"{c.dtype} on {c.device}; one call copies in caches of one form")
+        if not c.is_contiguous():
+            raise Refused(op, "a cache is a strided view; pages are copied in place, so it is contiguous")
+        seen.add(c.data_ptr())
+    if len(seen) != len(caches) and first.numel():
+        raise Refused(op, "a cache is named twice")
+    rt.copy_pages(caches, src, dst, block)
+
+
+# ------------------------------------------------------------------------------- log probabilities
+@dataclass
+class TokenLogprobs:
+    """What token_logprobs found in each row of logits, natural logarithms: `logprobs` in the shape of
+    the targets (None without targets), `entropy` [rows], and the most probable tokens, largest first:
+    `top_ids` u32 [rows, top] and `top_logprobs` [rows, top]."""
+    logprobs: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of given tokens under logits [rows, vocab] (f32 or f16): targets u32 [rows], or
+    [rows, n] for several tokens of each row; the entropy of every row; and the `top` (at most 32) most
+    probable tokens, ties to the lowest index.  A target at or past the vocabulary gives NaN, and a
+    row that holds a NaN or +inf, or nothing above -inf, gives NaN throughout.  No reference
+    counterpart."""
+    op = "TokenLogprobs"
+    if logits.dtype not in (torch.float32, torch.float16) or logits.dim() != 2 or logits.shape[1] == 0:
+        raise Refused(op, f"logits are {logits.dtype} {tuple(logits.shape)}; they are f32 or f16 [rows, vocab]")
+    rows, vocab = logits.shape
+    if not isinstance(top, int) or isinstance(top, bool) or not 0 <= top <= min(32, vocab):
+        raise Refused(op, f"{top!r} alternatives of a vocabulary of {vocab}; at most 32")
+    dev = logits.device
+    n = 0
+    if targets is not None:
+        if not _is_u32(targets):
+            raise Refused(op, f"targets are {targets.dtype} and a token id is u32")
+        if targets.dim() not in (1, 2) or targets.shape[0] != rows:
+            raise Refused(op, f"targets are {tuple(targets.shape)} and the logits hold {rows} rows; they are [rows] or [rows, n]")
+        n = 1 if targets.dim() == 1 else targets.shape[1]
+    new = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)
+    lp = None if targets is None else torch.empty(targets.shape, dtype=torch.float32, device=dev)
+    out = TokenLogprobs(lp, new(rows), torch.empty((rows, top), dtype=U32, device=dev), new(rows, top))
+    if rows:
+        none = out.top_ids.new_empty(0)
+        rt.launch_own("TokenLogprobsF16" if logits.dtype == torch.float16 else "TokenLogprobs",
+                      [_aligned(logits), none if targets is None else _aligned(targets), none if lp is None else lp,
+                       out.entropy, out.top_ids, out.top_logprobs], rt.logprob_dims(vocab, rows, n, top))
     return out
 
 

@@ -238,6 +238,25 @@ AB_API uint64_t ab_launch_count(void);
  *  AttentionPrefillPaged, AttentionPrefillPagedF16   q, k, v, pages u32[P], lengths u32[1], out
  *                    PagedPrefillDims{QHeads,KVHeads,HeadDim,QSeq,Base,Block,Scale f32}@0..24 (32 B)
  *                    internal/kernels/prefill.go:409, pagedprefillf16.go:31.  Query row s sees positions <= Base + s.
+ *  AttentionWindow, AttentionWindowF16   q f32[qH*D], k, v, lengths u32[1], out
+ *  AttentionWindowBatched, AttentionWindowBatchedF16   q f32[B*qH*D], k, v, pages u32[B*MaxPages], lengths u32[B], out
+ *  AttentionWindowRagged, AttentionWindowRaggedF16   q, k, v, pages, lengths u32[B], offsets u32[B+1], out
+ *  AttentionWindowPrefill, AttentionWindowPrefillF16   q f32[QSeq*qH*D], k, v, lengths u32[1], out
+ *  AttentionWindowPrefillPaged, AttentionWindowPrefillPagedF16   q, k, v, pages u32[MaxPages], lengths u32[1], out
+ *                    WindowDims{Batch,QHeads,KVHeads,HeadDim,Block,MaxPages,Scale f32,Window,Sinks,Capacity,QSeq,Base}
+ *                    @0..44 (48 B).  No reference kernels: the forms above with a sliding window.  A query at position p
+ *                    sees the positions j <= p that are within its cache length and have p - j < Window or j < Sinks.
+ *                    Window is at least 1 (1: its own position and the sinks).  Table entries of pages that no row of the call sees are not
+ *                    read, and a visible position whose page is outside the cache counts as masked.  Capacity is the
+ *                    cache's positions: its element count may pass 32 bits, and a length of 0xffffffff in the lengths
+ *                    block says that many or more.  A row that sees nothing is NaN, ragged padding is zeros.
+ *                    A row that sees a key or a value that is not finite comes out NaN or infinite; other rows do not.
+ *  TokenLogprobs, TokenLogprobsF16   logits f32 | f16 [Rows*Vocab], targets u32[Rows*Targets], logprobs f32[Rows*Targets],
+ *                    entropy f32[Rows], top_ids u32[Rows*Top], top_logprobs f32[Rows*Top]   {Vocab,Rows,Targets,Top}@0..12
+ *                    (16 B).  No reference kernels: log softmax of the targets, the distribution's entropy in nats, and
+ *                    the Top <= 32 largest logits (value descending, index ascending; -0 equals 0, a NaN is the largest)
+ *                    with their log probabilities.  A target at or past Vocab gives NaN, and so does every entry of a
+ *                    row that holds a NaN or +inf or nothing above -inf.
  *  Softmax           x f32[rows*width], out                                 RowDims   internal/kernels/norm.go:95
  *  ScaleRows         x, factors f32[rows], out                              RowSampleDims{Vocab,Rows,History,Slots}@0..12 (16 B)
  *                    internal/kernels/rowsample.go:226
@@ -325,9 +344,31 @@ AB_API int ab_blockpool_available(ab_blockpool *p);
 /* Grow: `pages` holds n_pages entries and has room for ceil(n/block); returns the new count
  * (>= n_pages) or a negative status; the pool never evicts (AB_ERR_OOM). */
 AB_API int ab_blockpool_grow(ab_blockpool *p, uint32_t *pages, int n_pages, int n_positions);
-/* Free: returns AB_OK, or AB_ERR_INVALID when any page was already free (the others are freed). */
+/* Free: returns AB_OK, or AB_ERR_INVALID when any page was already free (the others are freed).  A
+ * shared page returns to the pool when its last holder frees it; AB_PAGE_NONE entries are skipped. */
 AB_API int ab_blockpool_free(ab_blockpool *p, const uint32_t *pages, int n_pages);
 AB_API int ab_blockpool_positions(ab_blockpool *p, int n_pages);
+/* Sharing, copy on write and compaction (no reference counterpart).  The entry of a page row whose
+ * page was freed ahead of the others (behind an attention window) is AB_PAGE_NONE. */
+#define AB_PAGE_NONE 0xffffffffu
+/* One more holder of each page (a forked sequence's row): AB_ERR_INVALID, and nothing shared, if any
+ * is free. */
+AB_API int ab_blockpool_share(ab_blockpool *p, const uint32_t *pages, int n_pages);
+AB_API int ab_blockpool_refs(ab_blockpool *p, uint32_t page);    /* holders of a page, 0 = free */
+/* Makes the caller the only holder of each of `pages`: a shared page is replaced in the row by a new
+ * one, and (src, dst) get the copy that has to be made before the row is written (or read) through
+ * it.  Room for n_pages pairs; returns how many, or a negative status with nothing changed. */
+AB_API int ab_blockpool_own(ab_blockpool *p, uint32_t *pages, int n_pages, uint32_t *src, uint32_t *dst);
+/* Moves the held pages to the lowest numbers: (src, dst) get the moves, room for all of the pool's
+ * pages in each; returns how many.  No page is both a source and a destination.  The caller rewrites
+ * its page rows (src -> dst) and copies the pages before anything reads through the new rows. */
+AB_API int ab_blockpool_compact(ab_blockpool *p, uint32_t *src, uint32_t *dst);
+/* caches[c][dst[i]] = caches[c][src[i]] for every cache (a HOST array of device pointers) and pair (HOST
+ * numbers), on `stream`: a page is page_bytes contiguous bytes and a cache `pages` of them.  Refused,
+ * with nothing launched, when a page is out of range, written twice, or both written and read.  A
+ * stream capture records the pairs and pointers of the call. */
+AB_API int ab_cache_copy_pages(void *stream, void *const *caches, int n_caches, size_t page_bytes, uint32_t pages,
+                               const uint32_t *src, const uint32_t *dst, int n_pairs);
 
 /* Group-aligned column split of an int4 [K,N] matrix for tensor-parallel sharding: shard r of
  * `parts` owns columns [begin, end), both multiples of 128, so each shard's codes, scales and

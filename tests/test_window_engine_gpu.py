@@ -1,0 +1,195 @@
+"""The decode engine over an attention window: prefill, steps, pages freed behind the window, forks, compaction and
+scored tokens together, as a serving loop uses them.  On a B200."""
+import numpy as np
+import pytest
+import torch
+
+from accel_b200 import decode as dec
+from accel_b200 import runtime as rt
+from accel_b200.blockpool import BlockPool
+from util import assert_close
+from window_ref import visible
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+WINDOW, SINKS, BLOCK = 20, 3, 4
+
+
+def config(dtype=torch.float32, window=WINDOW):
+    return dec.ModelConfig(layers=2, d_model=256, n_heads=4, n_kv_heads=2, head_dim=64, ffn=512, vocab=1024, block=BLOCK,
+                           cache_dtype=dtype, window=window, sinks=SINKS if window else 0)
+
+
+def model(cfg):
+    return dec.DecodeModel(cfg, dec.Shard.plan(cfg, 1, 0), DEV, seed=3, std=0.08)
+
+
+class PlainAttention:
+    """The library's dispatch with the windowed attention kernels replaced by their definition in 64 bits."""
+    calls = 0
+
+    @staticmethod
+    def launch_count():
+        return 0
+
+    @classmethod
+    def launch(cls, name, bindings, uniform=None):
+        if not name.startswith("AttentionWindow"):
+            return rt.launch(name, bindings, uniform)
+        cls.calls += 1
+        q, k, v, pages, lengths, out = bindings
+        d = np.frombuffer(uniform, np.uint32)
+        batch, heads, kv, D, block, window, sinks, q_seq, base = (int(d[i]) for i in (0, 1, 2, 3, 4, 7, 8, 10, 11))
+        scale = float(np.frombuffer(uniform, np.float32)[6])
+        prefill = "Prefill" in name
+        table = pages.view(1 if prefill else batch, -1).long()
+        rows = [(0, base + i, int(lengths[0])) for i in range(q_seq)] if prefill else [(b, int(n) - 1, int(n)) for b, n in enumerate(lengths)]
+        qs, o = q.view(len(rows), heads, D).double(), out.view(len(rows), heads, D)
+        for r, (b, p, n) in enumerate(rows):
+            j = torch.tensor(visible(p, n, window, sinks), device=DEV)
+            at = table[b][j // block] * block + j % block
+            kk, vv = (x[at].double().repeat_interleave(heads // kv, 1) for x in (k, v))
+            w = torch.softmax(torch.einsum("hd,nhd->hn", qs[r], kk) * scale, 1)
+            o[r] = torch.einsum("hn,nhd->hd", w, vv).float()
+
+
+def engine(m, batch, context=96):
+    e = dec.DecodeEngine(m, batch, max_context=context)
+    e.prepare()
+    return e
+
+
+def steps(e, tok, n, trim=False):
+    logits = []
+    for _ in range(n):
+        for s in range(e.batch):
+            e.reserve(s, int(e.lengths_host[s]) + 1)
+        e.upload_pages()
+        tok = e.step(tok)
+        logits.append(e.full_logits().clone())
+        if trim:
+            e.trim()
+    return tok, torch.stack(logits)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_prefill_and_steps_against_plain_attention(dtype):
+    m = model(config(dtype))
+    rng = np.random.default_rng(1)
+    prompts = rng.integers(0, 1024, (3, 41))
+    a, b = engine(m, 3), engine(m, 3)
+    b.ops = PlainAttention
+    PlainAttention.calls = 0
+    for e in (a, b):
+        e.prefill(prompts, chunk=16)
+    tok = prompts[:, -1]
+    for t in range(30):
+        for e in (a, b):
+            for s in range(3):
+                e.reserve(s, 41 + t + 1)
+            e.upload_pages()
+            e.set_inputs(tok)
+            e.run_step()
+            e.lengths_host += 1
+        assert_close(a.full_logits().cpu().numpy(), b.full_logits().cpu().numpy(), 5e-3, f"logits at step {t}")
+        tok = rng.integers(0, 1024, 3)
+        if t % 4 == 0:
+            a.trim(), b.trim()
+    assert PlainAttention.calls == 3 * 3 * 2 + 30 * 2
+    assert any(x == BlockPool.NONE for x in a.page_rows[0])
+
+
+def test_freeing_forking_and_compaction_change_no_bit():
+    m = model(config())
+    rng = np.random.default_rng(2)
+    prompts = rng.integers(0, 1024, (4, 33))
+    a, b = engine(m, 4), engine(m, 4)
+    for e in (a, b):
+        e.prefill(prompts, chunk=16)
+    free0 = a.pool.available()
+    tok = prompts[:, -1]
+    ta, la = steps(a, tok, 12, trim=True)
+    tb, lb = steps(b, tok, 12)
+    assert np.array_equal(ta, tb) and torch.equal(la, lb)                # freed pages are never read
+    assert a.pool.available() > b.pool.available() and free0 >= 0
+    # sequence 2 becomes a copy of 0; both go on with the same token: the same bits, and 0's are untouched
+    a.fork(0, 2)
+    assert a.lengths_host[2] == a.lengths_host[0] and a.lengths_host[0] % BLOCK
+    last = int(a.lengths_host[0]) // BLOCK
+    assert a.page_rows[2][last] != a.page_rows[0][last]                  # the partly filled page is its own
+    assert all(x == y for x, y in zip(a.page_rows[2][:last], a.page_rows[0][:last]))
+    tok = np.array([7, 8, 7, 9])
+    ta, la = steps(a, tok, 3, trim=True)
+    tb, lb = steps(b, np.array([7, 8, 1, 9]), 3)
+    assert torch.equal(la[:, 0], la[:, 2]) and torch.equal(la[:, 0], lb[:, 0]) and torch.equal(la[:, 1], lb[:, 1])
+    # then they part: what one writes the other does not see
+    ta, la = steps(a, np.array([5, 6, 900, 6]), 4)
+    tb, lb = steps(b, np.array([5, 6, 1, 6]), 4)
+    assert torch.equal(la[:, 0], lb[:, 0]) and torch.equal(la[:, 3], lb[:, 3]) and not torch.equal(la[:, 0], la[:, 2])
+    # the pages in use move to the front of the pool
+    a.trim()
+    held = {x for r in a.page_rows for x in r if x != BlockPool.NONE}
+    moved = a.compact()
+    assert moved == len([x for x in held if x >= len(held)]) and moved > 0
+    assert {x for r in a.page_rows for x in r if x != BlockPool.NONE} == set(range(len(held)))
+    for c in (*a.k_cache, *a.v_cache):
+        c[len(held) * BLOCK:] = float("nan")                             # nothing lives there any more
+    ta, la = steps(a, np.array([5, 6, 900, 6]), 2)
+    tb, lb = steps(b, np.array([5, 6, 1, 6]), 2)
+    assert torch.equal(la[:, 0], lb[:, 0]) and torch.equal(la[:, 1], lb[:, 1]) and torch.isfinite(la).all()
+    for s in range(4):
+        a.pool.free(a.page_rows[s])
+    assert a.pool.available() == a.batch * a.max_pages
+
+
+def test_fork_refuses_and_survives_a_full_pool():
+    e = engine(model(config()), 2, context=16)
+    for bad in ((0, 0), (0, 2), (-1, 0)):
+        with pytest.raises(ValueError, match="fork of sequence"):
+            e.fork(*bad)
+    with pytest.raises(ValueError, match="no attention window"):
+        engine(model(config(window=0)), 1).trim()
+    e.reserve(0, 6)
+    e.lengths_host[0] = 6
+    extra = e.pool.grow(None, e.pool.available() * BLOCK)                 # somebody holds the rest
+    with pytest.raises(Exception, match="does not evict"):
+        e.fork(0, 1)
+    assert e.page_rows[1] == [] and e.lengths_host[1] == 0 and all(e.pool.refs(p) == 1 for p in e.page_rows[0])
+    e.pool.free(extra)
+    e.fork(0, 1)
+    assert e.lengths_host[1] == 6 and len(e.page_rows[1]) == len(e.page_rows[0])
+
+
+def test_captured_steps_and_the_plan_seam_run_the_windowed_kernels():
+    m = model(config())
+    a, b, c = (engine(m, 2) for _ in range(3))
+    for e in (a, b, c):
+        e.fill_context(30, seed=2)
+        for s in range(2):
+            e.reserve(s, 60)
+        e.upload_pages()
+    tok = np.array([3, 4])
+    b.set_inputs(tok)
+    b.capture(warmup=1)
+    seam = dec.SeamStep(c)
+    t1 = t2 = t3 = tok
+    for _ in range(10):
+        t1, t2, t3 = a.step(t1), b.step(t2), seam.step(t3)
+        assert np.array_equal(t1, t2) and np.array_equal(t1, t3)
+        assert torch.equal(a.full_logits(), b.full_logits()) and torch.equal(a.full_logits(), c.full_logits())
+    seam.close()
+
+
+def test_scored_tokens_are_those_of_the_logits():
+    e = engine(model(config()), 3)
+    e.fill_context(25, seed=4)
+    nxt, logits = steps(e, np.array([1, 2, 3]), 1)
+    r = e.score(e.next_tokens, top=4)
+    x = logits[0].double()
+    lp = torch.log_softmax(x, 1)
+    want = lp.gather(1, e.next_tokens.long()[:, None])[:, 0]
+    # (the sum over 1024 tokens and the difference x - m: 1024 + |lp| ulp at most)
+    assert (r.logprobs.double() - want).abs().max() <= 2.0**-24 * (1024 + 4 * want.abs().max())
+    assert torch.equal(r.top_ids[:, 0], e.next_tokens) and torch.equal(r.top_logprobs[:, 0], r.logprobs)
+    assert torch.equal(r.top_ids, torch.sort(logits[0], dim=1, descending=True, stable=True).indices[:, :4].int())
+    assert ((r.entropy.double() + (lp.exp() * lp).sum(1)).abs() <= 2.0**-24 * 1024 * 20).all()
