@@ -20,6 +20,8 @@
 #include <algorithm>
 #include <math_constants.h>
 
+#include <mutex>
+
 #include "common.cuh"
 
 namespace ab {
@@ -99,50 +101,467 @@ __device__ __forceinline__ uint32_t win_row(const WinParams &p, const WinView &w
     return r < p.capacity ? (uint32_t)r : 0xffffffffu;
 }
 
-template <typename T> __device__ __forceinline__ float to_f32(T x);
-template <> __device__ __forceinline__ float to_f32<float>(float x) { return x; }
-template <> __device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+// ------------------------------------------------------------------------------------------------
+// The row kernel: a few query heads against one list of positions.
+//
+// A cluster of CTAs takes one (row, KV head, up to eight of its query heads); every warp takes tiles of 16
+// positions of the list in turn, with the heads as the 8-wide dimension of mma.sync:
+//     S^T[16 positions x 8 heads] = K Q^T,      O^T[dims x 8 heads] += V^T P^T
+// and a running maximum and sum per warp; the warps are joined through shared memory and the CTAs of the
+// cluster through distributed shared memory, in a fixed order, so one launch does it all without a
+// workspace and repeats its bits.  HBM bounds it: the list is read once for all heads of the group.
+//
+// The products keep f32 accuracy.  An operand is held as a high and a low part of 11 bits each (tf32 for
+// an f32 cache, f16 for an f16 cache, whose K and V are exact in one part); the product of the two low
+// parts, 2^-22, is dropped.  Every tile's products start from zero and the smaller ones come first; the
+// sums over tiles are f32 additions outside the tensor core.
+// ------------------------------------------------------------------------------------------------
+constexpr int kRowWarps = 4;
+constexpr int kTile = 16;
+// an f16 cache's weights are carried times 2^14: the low part of a small one would otherwise meet f16's
+// smallest step; they are at most 1, and the quotient by their sum does not change
+constexpr float kWeightBias = 14.f;
 
-// One warp per (row, query head), a lane holds the dimensions lane, lane + 32, ...
-template <typename T>
-__global__ void __launch_bounds__(128) win_simple_kernel(const WinParams p)
+// Row strides of the tiles in shared memory, in bytes: f32 K is read as 16 bytes of two neighbouring rows by a quarter
+// warp (stride = 64 mod 128), f32 V as 32 bytes of four (32 mod 128), f16 by ldmatrix as 16 bytes of eight (16 mod 128).
+template <typename T, int DP> struct RowTile {
+    static constexpr int kRow = DP * (int)sizeof(T);
+    static constexpr int kStrideK = sizeof(T) == 4 ? kRow + 64 : kRow + 16;
+    static constexpr int kStrideV = sizeof(T) == 4 ? kRow + 32 : kRow + 16;
+    static constexpr int kBytesK = kTile * kStrideK, kBytesV = kTile * kStrideV;
+    static constexpr int kWarpBytes = kBytesK + kBytesV;
+    static constexpr int kMergeBytes = kRowWarps * 8 * (DP + 2) * 4 + 8 * (DP + 2) * 4;
+    static constexpr int kSmem = kRowWarps * kWarpBytes > kMergeBytes ? kRowWarps * kWarpBytes : kMergeBytes;
+};
+
+__device__ __forceinline__ void cp16(uint32_t smem, const void *gmem, bool on)
 {
-    const uint64_t item = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (item >= (uint64_t)p.rows * p.q_heads) return;
-    const uint32_t row = (uint32_t)(item / p.q_heads), h = (uint32_t)(item % p.q_heads);
-    const int lane = threadIdx.x & 31;
-    const uint32_t D = p.head_dim, kvh = h / (p.q_heads / p.kv_heads);
-    const WinView w = win_view(p, row);
-    const T *k = static_cast<const T *>(p.k), *v = static_cast<const T *>(p.v);
-    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, oc[4];
-    for (int e = 0; e < 4; e++) q[e] = (uint32_t)(lane + 32 * e) < D ? p.q[item * D + lane + 32 * e] * p.scale_log2 : 0.f;
-    // sums over runs of 64 positions are joined by the same recurrence: a run of thousands of additions
-    // into one accumulator would lose two more bits of it
-    float m = -CUDART_INF_F, l = 0.f;
-    for (uint32_t i0 = 0; i0 < w.n; i0 += 64) {
-        float mc = -CUDART_INF_F, lc = 0.f;
-        for (int e = 0; e < 4; e++) oc[e] = 0.f;
-        for (uint32_t i = i0; i < min(i0 + 64, w.n); i++) {
-            const uint32_t r = win_row(p, w, i);
-            if (r == 0xffffffffu) continue;
-            const size_t at = ((size_t)r * p.kv_heads + kvh) * D;
-            float s = 0.f;
-            for (int e = 0; e < 4; e++) if ((uint32_t)(lane + 32 * e) < D) s = fmaf(q[e], to_f32(k[at + lane + 32 * e]), s);
-            for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            const float m1 = fmaxf(mc, s), a = mc == m1 ? 1.f : exp2f(mc - m1), pr = exp2f(s - m1);
-            mc = m1;
-            lc = fmaf(lc, a, pr);
-            for (int e = 0; e < 4; e++)
-                if ((uint32_t)(lane + 32 * e) < D) oc[e] = fmaf(oc[e], a, pr * to_f32(v[at + lane + 32 * e]));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float4 lds128(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// x = hi + lo with hi of 11 bits.  Cut off (K and V, two instructions): the low part is exact and keeps the sign of x.
+// Rounded (q and the weights): the low part has either sign, so the dropped product of two low parts averages out.
+__device__ __forceinline__ void cut_tf32(float x, uint32_t &hi, uint32_t &lo)
+{
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void round_tf32(float x, uint32_t &hi, uint32_t &lo)
+{
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void round_f16x2(float x, float y, uint32_t &hi, uint32_t &lo)
+{
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// A group of query heads in the B fragments of S^T = K Q^T, with Scale * log2(e) applied; column g = lane / 4.
+template <typename T, int DP> struct QFrag;
+template <int DP> struct QFrag<float, DP> {
+    uint32_t hi[DP / 4], lo[DP / 4];
+    // of every 16 dimensions a thread holds four neighbouring ones of K and of q: the order of a sum's terms is free
+    __device__ __forceinline__ void load(const float *q, bool on, uint32_t D, int t, float scale, float (&undo)[2])
+    {
+#pragma unroll
+        for (int j = 0; j < DP / 16; j++) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (on && (uint32_t)(16 * j + 4 * t) < D) x = *reinterpret_cast<const float4 *>(q + 16 * j + 4 * t);
+            round_tf32(x.x * scale, hi[4 * j], lo[4 * j]);
+            round_tf32(x.y * scale, hi[4 * j + 1], lo[4 * j + 1]);
+            round_tf32(x.z * scale, hi[4 * j + 2], lo[4 * j + 2]);
+            round_tf32(x.w * scale, hi[4 * j + 3], lo[4 * j + 3]);
         }
-        if (mc == -CUDART_INF_F && lc == 0.f) continue;
-        const float m1 = fmaxf(m, mc), a = m == m1 ? 1.f : exp2f(m - m1), c = mc == m1 ? 1.f : exp2f(mc - m1);
-        m = m1;
-        l = fmaf(l, a, lc * c);
-        for (int e = 0; e < 4; e++) o[e] = fmaf(o[e], a, oc[e] * c);
+        undo[0] = undo[1] = 1.f;
     }
-    for (int e = 0; e < 4; e++)
-        if ((uint32_t)(lane + 32 * e) < D) p.out[item * D + lane + 32 * e] = w.zero ? 0.f : o[e] / l;
+};
+template <int DP> struct QFrag<__half, DP> {
+    uint32_t hi[DP / 8], lo[DP / 8];
+    // f16 has 5 bits of exponent: a head's q is scaled by a power of two that brings its largest element near one
+    __device__ __forceinline__ void load(const float *q, bool on, uint32_t D, int t, float scale, float (&undo)[2])
+    {
+        float2 x[DP / 8];
+        float amax = 0.f;
+#pragma unroll
+        for (int j = 0; j < DP / 8; j++) {
+            x[j] = make_float2(0.f, 0.f);
+            if (on && (uint32_t)(8 * j + 2 * t) < D) x[j] = *reinterpret_cast<const float2 *>(q + 8 * j + 2 * t);
+            x[j].x *= scale;
+            x[j].y *= scale;
+            amax = fmaxf(amax, fmaxf(fabsf(x[j].x), fabsf(x[j].y)));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -126), 126);
+#pragma unroll
+        for (int j = 0; j < DP / 8; j++) round_f16x2(x[j].x * ab_pow2(-e), x[j].y * ab_pow2(-e), hi[j], lo[j]);
+        const float back = ab_pow2(e);
+        undo[0] = __shfl_sync(0xffffffffu, back, 8 * t);            // columns 2t and 2t + 1 are held by lanes 8t and 8t + 4
+        undo[1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+    }
+};
+
+template <typename T, int DP> struct RowMath;
+template <int DP> struct RowMath<float, DP> {
+    static __device__ __forceinline__ void scores(const QFrag<float, DP> &q, uint32_t k, int g, int t, float (&s)[4])
+    {
+        float small[2][4] = {}, big[2][4] = {};
+        const uint32_t r0 = k + g * RowTile<float, DP>::kStrideK + t * 16, r1 = r0 + 8 * RowTile<float, DP>::kStrideK;
+#pragma unroll
+        for (int j = 0; j < DP / 16; j++) {
+            const float4 x = lds128(r0 + 64 * j), y = lds128(r1 + 64 * j);
+            uint32_t h[4], l[4];
+            cut_tf32(x.x, h[0], l[0]); cut_tf32(y.x, h[1], l[1]); cut_tf32(x.y, h[2], l[2]); cut_tf32(y.y, h[3], l[3]);
+            mma_tf32(small[0], l, q.hi[4 * j], q.hi[4 * j + 1]);
+            mma_tf32(small[1], h, q.lo[4 * j], q.lo[4 * j + 1]);
+            mma_tf32(big[0], h, q.hi[4 * j], q.hi[4 * j + 1]);
+            cut_tf32(x.z, h[0], l[0]); cut_tf32(y.z, h[1], l[1]); cut_tf32(x.w, h[2], l[2]); cut_tf32(y.w, h[3], l[3]);
+            mma_tf32(small[0], l, q.hi[4 * j + 2], q.hi[4 * j + 3]);
+            mma_tf32(small[1], h, q.lo[4 * j + 2], q.lo[4 * j + 3]);
+            mma_tf32(big[1], h, q.hi[4 * j + 2], q.hi[4 * j + 3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] = (small[0][i] + small[1][i]) + (big[0][i] + big[1][i]);
+    }
+    // o[dims] = o * alpha + V^T P^T; the 16 positions as 2 x 8 with a thread on t, t + 4 | t + 8, t + 12
+    static __device__ __forceinline__ void values(const float (&p)[4], uint32_t v, int g, int t, int lane, const float (&a)[2],
+                                                  float (&o)[DP / 16][4])
+    {
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {                               // weight of (position t + 4 i, column g)
+            const int from = ((t + 4 * i) & 7) * 4 + (g >> 1);
+            const float even = __shfl_sync(0xffffffffu, p[(i >> 1) * 2], from), odd = __shfl_sync(0xffffffffu, p[(i >> 1) * 2 + 1], from);
+            round_tf32((g & 1) ? odd : even, ph[i], pl[i]);
+        }
+        const uint32_t row = v + t * RowTile<float, DP>::kStrideV + g * 16;
+#pragma unroll
+        for (int jj = 0; jj < DP / 32; jj++) {
+            float x[4][4];                                          // [position t + 4 i][dimension 32 jj + 4 g + e]
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4 y = lds128(row + 4 * i * RowTile<float, DP>::kStrideV + 128 * jj);
+                x[i][0] = y.x; x[i][1] = y.y; x[i][2] = y.z; x[i][3] = y.w;
+            }
+#pragma unroll
+            for (int m = 0; m < 2; m++) {                           // rows g and g + 8 of an MMA are elements 2 m and 2 m + 1
+                float small[4] = {}, big[4] = {};
+                uint32_t h[2][4], l[2][4];
+#pragma unroll
+                for (int ks = 0; ks < 2; ks++) {
+                    cut_tf32(x[2 * ks][2 * m], h[ks][0], l[ks][0]);
+                    cut_tf32(x[2 * ks][2 * m + 1], h[ks][1], l[ks][1]);
+                    cut_tf32(x[2 * ks + 1][2 * m], h[ks][2], l[ks][2]);
+                    cut_tf32(x[2 * ks + 1][2 * m + 1], h[ks][3], l[ks][3]);
+                    mma_tf32(small, l[ks], ph[2 * ks], ph[2 * ks + 1]);
+                    mma_tf32(small, h[ks], pl[2 * ks], pl[2 * ks + 1]);
+                    mma_tf32(big, h[ks], ph[2 * ks], ph[2 * ks + 1]);
+                }
+                float (&d)[4] = o[2 * jj + m];
+#pragma unroll
+                for (int i = 0; i < 4; i++) d[i] = fmaf(d[i], a[i & 1], small[i] + big[i]);
+            }
+        }
+    }
+    // the dimension of o[m][i]
+    static __device__ __forceinline__ int dim(int m, int i, int g) { return 32 * (m >> 1) + 4 * g + 2 * (m & 1) + (i >> 1); }
+};
+template <int DP> struct RowMath<__half, DP> {
+    static __device__ __forceinline__ void scores(const QFrag<__half, DP> &q, uint32_t k, int, int, float (&s)[4])
+    {
+        const int lane = threadIdx.x & 31;
+        float small[4] = {}, big[2][4] = {};
+        const uint32_t at = k + (lane & 15) * RowTile<__half, DP>::kStrideK + (lane >> 4) * 16;
+#pragma unroll
+        for (int j = 0; j < DP / 16; j++) {
+            uint32_t a[4];
+            ldsm4(a, at + 32 * j);
+            mma_f16(small, a, q.lo[2 * j], q.lo[2 * j + 1]);
+            mma_f16(big[j & 1], a, q.hi[2 * j], q.hi[2 * j + 1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] = small[i] + (big[0][i] + big[1][i]);
+    }
+    static __device__ __forceinline__ void values(const float (&p)[4], uint32_t v, int, int, int lane, const float (&a)[2],
+                                                  float (&o)[DP / 16][4])
+    {
+        uint32_t h0, l0, h1, l1;
+        round_f16x2(p[0], p[1], h0, l0);
+        round_f16x2(p[2], p[3], h1, l1);
+        h0 = transpose8x8(h0); l0 = transpose8x8(l0); h1 = transpose8x8(h1); l1 = transpose8x8(l1);
+        const uint32_t at = v + ((lane & 7) + ((lane >> 4) & 1) * 8) * RowTile<__half, DP>::kStrideV + ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int m = 0; m < DP / 16; m++) {
+            uint32_t x[4];
+            float c[4] = {};
+            ldsm4_t(x, at + 32 * m);
+            mma_f16(c, x, l0, l1);
+            mma_f16(c, x, h0, h1);
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[m][i] = fmaf(o[m][i], a[i & 1], c[i]);
+        }
+    }
+    static __device__ __forceinline__ int dim(int m, int i, int g) { return 16 * m + g + 8 * (i >> 1); }
+};
+
+__device__ __forceinline__ float ld_cluster(uint32_t smem, uint32_t rank)
+{
+    float v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}"
+                 : "=f"(v) : "r"(smem), "r"(rank) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_rows_kernel(const WinParams p, const uint32_t parts)
+{
+    using Tile = RowTile<T, DP>;
+    using Math = RowMath<T, DP>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t row = blockIdx.x / parts, part = blockIdx.x % parts;
+    const uint32_t D = p.head_dim, group = p.q_heads / p.kv_heads, per_kv = (group + 7) / 8;
+    const uint32_t kvh = blockIdx.y / per_kv, h0 = kvh * group + (blockIdx.y % per_kv) * 8;
+    const uint32_t heads = min(8u, (kvh + 1) * group - h0);
+    const uint32_t tile_k = (uint32_t)__cvta_generic_to_shared(smem) + warp * Tile::kWarpBytes, tile_v = tile_k + Tile::kBytesK;
+
+    const WinView w = win_view(p, row);
+    const uint32_t n_tiles = (w.n + kTile - 1) / kTile, step = parts * kRowWarps;
+    uint32_t tile = part * kRowWarps + warp;
+
+    // lanes 0..15 know the cache rows of a tile's positions (lanes 16..31 the same again)
+    const auto rows_of = [&](uint32_t tl) -> uint32_t {
+        const uint32_t i = tl * kTile + (lane & 15);
+        return i < w.n ? win_row(p, w, i) : 0xffffffffu;
+    };
+    const uint32_t row_bytes = D * sizeof(T), chunks = row_bytes / 16;
+    const int span = chunks > 16 ? 32 : (chunks > 8 ? 16 : 8);      // lanes that copy one row
+    const uint32_t chunk = lane & (span - 1);
+    const uint64_t pitch = (uint64_t)p.kv_heads * row_bytes;
+    const char *kb = static_cast<const char *>(p.k) + (uint64_t)kvh * row_bytes + chunk * 16;
+    const char *vb = static_cast<const char *>(p.v) + (uint64_t)kvh * row_bytes + chunk * 16;
+    const auto copy = [&](const char *base, uint32_t dst, uint32_t stride, uint32_t rows) {
+        if (span == 32) {
+#pragma unroll
+            for (int r = 0; r < kTile; r++) {
+                const uint32_t x = __shfl_sync(0xffffffffu, rows, r);
+                if (chunk < chunks) cp16(dst + r * stride + chunk * 16, base + (x == 0xffffffffu ? 0 : x * pitch), x != 0xffffffffu);
+            }
+        } else {
+            const int per = 32 / span;
+            for (int r0 = 0; r0 < kTile; r0 += per) {
+                const int r = r0 + lane / span;
+                const uint32_t x = __shfl_sync(0xffffffffu, rows, r);
+                if (chunk < chunks) cp16(dst + r * stride + chunk * 16, base + (x == 0xffffffffu ? 0 : x * pitch), x != 0xffffffffu);
+            }
+        }
+        cp_commit();
+    };
+
+    if (D < DP) {                                                   // what a shorter head leaves unwritten of a tile is zero
+        for (uint32_t i = lane; i < Tile::kWarpBytes / 16; i += 32)
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(tile_k + i * 16), "r"(0) : "memory");
+        __syncwarp();
+    }
+    uint32_t rows = 0xffffffffu, next = 0xffffffffu;
+    if (tile < n_tiles) {
+        rows = rows_of(tile);
+        copy(kb, tile_k, Tile::kStrideK, rows);
+        copy(vb, tile_v, Tile::kStrideV, rows);
+        if (tile + step < n_tiles) next = rows_of(tile + step);
+    }
+    QFrag<T, DP> q;
+    float undo[2];
+    q.load(p.q + ((uint64_t)row * p.q_heads + h0 + min((uint32_t)g, heads - 1)) * D, (uint32_t)g < heads, D, t, p.scale_log2, undo);
+
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f}, o[DP / 16][4];
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (; tile < n_tiles; tile += step) {
+        const bool more = tile + step < n_tiles;
+        const uint32_t seen = __ballot_sync(0xffffffffu, rows != 0xffffffffu);
+        cp_wait<1>();
+        __syncwarp();
+        float s[4];
+        Math::scores(q, tile_k, g, t, s);
+        __syncwarp();
+        rows = next;
+        if (more) {
+            copy(kb, tile_k, Tile::kStrideK, rows);
+            next = tile + 2 * step < n_tiles ? rows_of(tile + 2 * step) : 0xffffffffu;
+        } else {
+            cp_commit();
+        }
+        if (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[i] *= undo[i & 1];
+        }
+        if (!((seen >> g) & 1)) s[0] = s[1] = -CUDART_INF_F;
+        if (!((seen >> (g + 8)) & 1)) s[2] = s[3] = -CUDART_INF_F;
+        float a[2], pr[4];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            float x = fmaxf(s[c], s[c + 2]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float m1 = fmaxf(m[c], x), ms = m1 == -CUDART_INF_F ? 0.f : m1;
+            const float bias = sizeof(T) == 2 ? kWeightBias : 0.f;
+            a[c] = m[c] == m1 ? 1.f : exp2f(m[c] - ms);
+            pr[c] = exp2f(s[c] - ms + bias);
+            pr[c + 2] = exp2f(s[c + 2] - ms + bias);
+            m[c] = m1;
+            l[c] = fmaf(l[c], a[c], pr[c] + pr[c + 2]);
+        }
+        cp_wait<1>();
+        __syncwarp();
+        Math::values(pr, tile_v, g, t, lane, a, o);
+        __syncwarp();
+        if (more) copy(vb, tile_v, Tile::kStrideV, rows);
+        else cp_commit();
+    }
+    cp_wait<0>();
+    __syncthreads();
+
+    // ---- the warps' parts, then the CTAs'
+    // per warp and column: maximum, sum, DP values; then the same of the CTA
+    float *part_ml = reinterpret_cast<float *>(smem), *part_o = part_ml + kRowWarps * 16;
+    float *cta_ml = part_o + kRowWarps * 8 * DP, *cta_o = cta_ml + 16;
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        l[c] += __shfl_xor_sync(0xffffffffu, l[c], 4);
+        l[c] += __shfl_xor_sync(0xffffffffu, l[c], 8);
+        l[c] += __shfl_xor_sync(0xffffffffu, l[c], 16);
+        if (g == 0) { part_ml[warp * 16 + 2 * t + c] = m[c]; part_ml[warp * 16 + 8 + 2 * t + c] = l[c]; }
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 16; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) part_o[(warp * 8 + 2 * t + (e & 1)) * DP + Math::dim(i, e, g)] = o[i][e];
+    __syncthreads();
+    for (uint32_t x = threadIdx.x; x < heads * DP; x += kRowWarps * 32) {
+        const uint32_t c = x / DP, d = x % DP;
+        float M = part_ml[c];
+        for (int i = 1; i < kRowWarps; i++) M = fmaxf(M, part_ml[i * 16 + c]);
+        float ls = 0.f, os = 0.f;
+        for (int i = 0; i < kRowWarps; i++) {
+            const float f = part_ml[i * 16 + c] == -CUDART_INF_F ? 0.f : exp2f(part_ml[i * 16 + c] - M);
+            ls = fmaf(part_ml[i * 16 + 8 + c], f, ls);
+            os = fmaf(part_o[(i * 8 + c) * DP + d], f, os);
+        }
+        if (parts == 1) {
+            if (d < D) p.out[((uint64_t)row * p.q_heads + h0 + c) * D + d] = w.zero ? 0.f : os / ls;
+        } else {
+            cta_o[c * DP + d] = os;
+            if (d == 0) { cta_ml[c] = M; cta_ml[8 + c] = ls; }
+        }
+    }
+    if (parts == 1) return;
+    cluster_sync();
+    const uint32_t ml_at = (uint32_t)__cvta_generic_to_shared(cta_ml), o_at = (uint32_t)__cvta_generic_to_shared(cta_o);
+    for (uint32_t x = part * (kRowWarps * 32) + threadIdx.x; x < heads * DP; x += parts * kRowWarps * 32) {
+        const uint32_t c = x / DP, d = x % DP;
+        if (d >= D) continue;
+        float M = -CUDART_INF_F;
+        for (uint32_t i = 0; i < parts; i++) M = fmaxf(M, ld_cluster(ml_at + c * 4, i));
+        float ls = 0.f, os = 0.f;
+        for (uint32_t i = 0; i < parts; i++) {
+            const float mi = ld_cluster(ml_at + c * 4, i), f = mi == -CUDART_INF_F ? 0.f : exp2f(mi - M);
+            ls = fmaf(ld_cluster(ml_at + (8 + c) * 4, i), f, ls);
+            os = fmaf(ld_cluster(o_at + (c * DP + d) * 4, i), f, os);
+        }
+        p.out[((uint64_t)row * p.q_heads + h0 + c) * D + d] = w.zero ? 0.f : os / ls;
+    }
+    cluster_sync();                                                 // nobody leaves while its parts are being read
+}
+
+// the kernel's dynamic shared memory and cluster sizes beyond what a kernel gets unasked: once per device
+template <typename T, int DP> int rows_prepare(const char *name)
+{
+    static std::mutex mu;
+    static uint64_t done[4];                                        // a bit per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= 0 && dev < 256 && (done[dev / 64] >> (dev % 64) & 1)) return AB_OK;
+    int rc = check_cuda(cudaFuncSetAttribute(win_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             RowTile<T, DP>::kSmem), name);
+    if (rc) return rc;
+    if (dev >= 0 && dev < 256) done[dev / 64] |= 1ull << (dev % 64);
+    return AB_OK;
+}
+
+template <typename T, int DP> int launch_rows(Launch &l, const WinParams &p, const char *name)
+{
+    const uint32_t group = p.q_heads / p.kv_heads, groups = p.kv_heads * ((group + 7) / 8);
+    // CTAs of a cluster that share a row's list: enough to give the SMs their three resident CTAs, as long as every warp
+    // still has a tile of its own
+    const uint64_t longest = std::min<uint64_t>((uint64_t)p.window + p.sinks, p.reach), want = 3ull * sm_count();
+    uint32_t parts = 1;
+    while (parts < 8 && (uint64_t)p.rows * groups * parts < want && longest > (uint64_t)parts * kRowWarps * kTile) parts *= 2;
+    if ((uint64_t)p.rows * parts > 0x7fffffffull || groups > 65535)
+        return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
+    const int rc = rows_prepare<T, DP>(name);
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.rows * parts, groups);
+    cfg.blockDim = dim3(kRowWarps * 32);
+    cfg.dynamicSmemBytes = RowTile<T, DP>::kSmem;
+    cfg.stream = l.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, win_rows_kernel<T, DP>, p, parts);
+    count_launch();
+    note_selection("%s: %u rows, %u group(s) of up to 8 query heads, a list split over %u CTA(s)", name, p.rows, groups, parts);
+    return check_cuda(e, name);
 }
 
 template <typename T> int run_window(Launch &l, WinParams &p, const char *name)
@@ -151,13 +570,8 @@ template <typename T> int run_window(Launch &l, WinParams &p, const char *name)
         return fail(AB_ERR_INVALID, "%s: Base=%u and %u rows pass 32 bits", name, p.base, p.rows);
     l.ws_need = 0;
     if (l.query_ws) return AB_OK;
-    const uint64_t items = (uint64_t)p.rows * p.q_heads;
-    if (items == 0) return AB_OK;
-    if ((items + 3) / 4 > 0x7fffffffull) return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
-    win_simple_kernel<T><<<(uint32_t)((items + 3) / 4), 128, 0, l.stream>>>(p);
-    count_launch();
-    note_selection("%s: a warp per row and head", name);
-    return check_cuda(cudaGetLastError(), name);
+    if (p.rows == 0) return AB_OK;
+    return p.head_dim <= 64 ? launch_rows<T, 64>(l, p, name) : launch_rows<T, 128>(l, p, name);
 }
 
 // WindowDims{Batch,QHeads,KVHeads,HeadDim,Block,MaxPages,Scale f32,Window,Sinks,Capacity,QSeq,Base}, 48 bytes.
