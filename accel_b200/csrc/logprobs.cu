@@ -2,14 +2,27 @@
 // of every row of logits.  No counterpart in the reference.
 //
 //     m = max x,  s = sum e^(x - m),  logprob(t) = (x_t - m) - log s,
-//     entropy = -sum p log p = log s - (sum (x - m) e^(x - m)) / s
+//     entropy = -sum p log p = log s - u / s,  u = sum (x - m) e^(x - m)
 //
 // and the Top largest logits in (value descending, index ascending) order with their log
 // probabilities; -0 equals +0 and a NaN is larger than every number.  A logit of -inf is a token of
 // probability 0 and adds nothing to the entropy.  A row that holds a NaN or a +inf, or nothing above
 // -inf, has no distribution: its log probabilities and entropy are NaN (its indices still stand).  A
 // target at or past Vocab has the log probability NaN.
+//
+// The row is read once: a thread carries (m, s, u) over its pieces, moving to a new maximum m' by
+//     s' = s e^(m - m'),  u' = (u + (m - m') s) e^(m - m'),
+// once per 16 elements, and threads, warps and CTAs are joined by the same rule in a fixed order.  One
+// exponential and seven instructions per element: HBM bounds it.
+//
+// The alternatives cost no second pass.  A warp's `each`-th largest thread maximum is reached by `each` of
+// its elements; with `each` = ceil(Top / warps) at least Top elements reach the smallest of these over
+// the warps, the floor.  Only threads whose maximum reaches it can hold an alternative (some tens); their
+// pieces are read again (L2), what reaches the floor is listed, and an element's place among the
+// alternatives is the number of listed ones before it.
 #include <math_constants.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 
@@ -17,12 +30,13 @@ namespace ab {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kMaxTop = 32;
+constexpr uint32_t kList = 1024;           // candidates a CTA can list; more (a shape made for it) takes the slow way
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.402823466e38f;
 
-template <typename T> __device__ __forceinline__ float lp_f32(T x);
-template <> __device__ __forceinline__ float lp_f32<float>(float x) { return x; }
-template <> __device__ __forceinline__ float lp_f32<__half>(__half x) { return __half2float(x); }
+typedef unsigned long long u64;
 
 // values in the order of their magnitude as unsigned numbers; 0 is below every value
 __device__ __forceinline__ uint32_t lp_key(float x)
@@ -36,6 +50,8 @@ __device__ __forceinline__ float lp_value(uint32_t key)
     if (key == 0xffffffffu) return CUDART_NAN_F;
     return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
+// an element as one number: the larger comes first
+__device__ __forceinline__ u64 lp_rank(float x, uint32_t index) { return (u64)lp_key(x) << 32 | (0xffffffffu - index); }
 
 struct LpParams {
     const void *x;
@@ -46,61 +62,296 @@ struct LpParams {
     uint32_t vocab, rows, n_targets, top;
 };
 
-// One CTA per row, the row read once for the maximum, once for the sums and once for each alternative.
-template <typename T> __global__ void __launch_bounds__(kThreads) logprobs_simple_kernel(const LpParams p)
-{
-    __shared__ float shf[2][kThreads];
-    __shared__ unsigned long long shk[kThreads];
-    const uint32_t row = blockIdx.x, t = threadIdx.x, V = p.vocab;
-    const T *x = static_cast<const T *>(p.x) + (size_t)row * V;
-    uint32_t best = 0;
-    for (uint32_t i = t; i < V; i += kThreads) best = max(best, lp_key(lp_f32(x[i])));
-    shk[t] = best;
-    __syncthreads();
-    for (int w = kThreads / 2; w; w /= 2) {
-        if (t < (uint32_t)w) shk[t] = max(shk[t], shk[t + w]);
-        __syncthreads();
+// 16 aligned bytes of a row
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ float one(const float *p) { return *p; }
+    static __device__ __forceinline__ void load(const float *p, float *x)
+    {
+        const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
     }
-    const float m = lp_value((uint32_t)shk[0]);
-    __syncthreads();
-    float s = 0.f, u = 0.f;
-    for (uint32_t i = t; i < V; i += kThreads) {
-        const float d = lp_f32(x[i]) - m, e = expf(d);
-        s += e;
-        u = fmaf(fmaxf(d, -1000.f), e, u);               // -inf * 0 is a NaN
-    }
-    shf[0][t] = s; shf[1][t] = u;
-    __syncthreads();
-    for (int w = kThreads / 2; w; w /= 2) {
-        if (t < (uint32_t)w) { shf[0][t] += shf[0][t + w]; shf[1][t] += shf[1][t + w]; }
-        __syncthreads();
-    }
-    const float log_s = logf(shf[0][0]);
-    if (t == 0) p.entropy[row] = log_s - shf[1][0] / shf[0][0];
-    for (uint32_t j = t; j < p.n_targets; j += kThreads) {
-        const uint32_t id = p.targets[(size_t)row * p.n_targets + j];
-        p.logprobs[(size_t)row * p.n_targets + j] = id < V ? (lp_f32(x[id]) - m) - log_s : CUDART_NAN_F;
-    }
-    unsigned long long last = ~0ull;                      // key and the index's complement: larger comes first
-    for (uint32_t r = 0; r < p.top; r++) {
-        unsigned long long b = 0;
-        for (uint32_t i = t; i < V; i += kThreads) {
-            const unsigned long long k = (unsigned long long)lp_key(lp_f32(x[i])) << 32 | (0xffffffffu - i);
-            if ((r == 0 || k < last) && k > b) b = k;
+};
+template <> struct Piece<__half> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ float one(const __half *p) { return __half2float(*p); }
+    static __device__ __forceinline__ void load(const __half *p, float *x)
+    {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+        const uint32_t r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r[i]));
+            x[2 * i] = f.x; x[2 * i + 1] = f.y;
         }
-        __syncthreads();
-        shk[t] = b;
-        __syncthreads();
-        for (int w = kThreads / 2; w; w /= 2) {
-            if (t < (uint32_t)w) shk[t] = max(shk[t], shk[t + w]);
+    }
+};
+
+struct Sums { float m, s, u; };
+__device__ __forceinline__ float lp_exp(float d) { float e; asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(d * kLog2e)); return e; }
+// below -1e4 e^d is 0, and (-inf) * 0 would be a NaN
+__device__ __forceinline__ float lp_clamp(float d) { return fmaxf(d, -1e4f); }
+// moves the sums to a maximum M >= m
+__device__ __forceinline__ void lp_move(Sums &a, float M)
+{
+    const float d = a.m - M, f = lp_exp(d);
+    a.u = fmaf(lp_clamp(d), a.s, a.u) * f;
+    a.s *= f;
+    a.m = M;
+}
+__device__ __forceinline__ void lp_join(Sums &a, Sums b)
+{
+    const float M = fmaxf(a.m, b.m);
+    if (a.m != M) lp_move(a, M);
+    if (b.m != M) lp_move(b, M);
+    a.s += b.s;
+    a.u += b.u;
+}
+__device__ __forceinline__ void lp_add(Sums &a, float x)
+{
+    const float d = x - a.m, e = lp_exp(d);
+    a.s += e;
+    a.u = fmaf(lp_clamp(d), e, a.u);
+}
+
+__device__ __forceinline__ uint32_t lp_mapa(const void *p, uint32_t rank)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float lp_remote_f32(uint32_t a)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ u64 lp_remote_u64(uint32_t a)
+{
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void lp_cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A cluster of `parts` CTAs per row, a contiguous run of the row's pieces each; the first also takes the few elements
+// before the first and behind the last whole piece.
+template <typename T> __global__ void __launch_bounds__(kThreads, 6) logprobs_kernel(const LpParams p, const uint32_t parts)
+{
+    constexpr int N = Piece<T>::kN, U = 16 / N;
+    __shared__ Sums sums[kWarps];
+    __shared__ Sums whole;
+    __shared__ uint32_t floors[kWarps], n_list;
+    __shared__ u64 list[kList], best[kMaxTop], all[16 * kMaxTop], slow[kWarps];
+    const uint32_t row = blockIdx.x / parts, part = blockIdx.x % parts, V = p.vocab, t = threadIdx.x;
+    const int warp = t >> 5, lane = t & 31;
+    const T *x = static_cast<const T *>(p.x) + (size_t)row * V;
+    const uint32_t head = min(V, (uint32_t)((0 - reinterpret_cast<uintptr_t>(x)) & 15) / (uint32_t)sizeof(T));
+    const uint32_t pieces = (V - head) / N, tail = head + pieces * N, n_extra = part == 0 ? head + (V - tail) : 0;
+    const uint32_t per = (pieces + parts - 1) / parts, p0 = min(part * per, pieces), p1 = min(p0 + per, pieces);
+    const T *xp = x + head;
+    const auto extra = [&](uint32_t i) { return i < head ? i : tail + (i - head); };
+
+    // ---- one pass
+    Sums a{kLowest, 0.f, 0.f};
+    for (uint32_t i = p0 + t; i < p1; i += kThreads * U) {
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            if (i + j * kThreads < p1) Piece<T>::load(xp + (size_t)(i + j * kThreads) * N, v + j * N);
+            else
+#pragma unroll
+                for (int e = 0; e < N; e++) v[j * N + e] = -CUDART_INF_F;
+        }
+        float c = v[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) c = fmaxf(c, v[e]);
+        lp_move(a, fmaxf(a.m, c));
+#pragma unroll
+        for (int e = 0; e < 16; e++) lp_add(a, v[e]);
+    }
+    if (t < n_extra) {
+        const float v = Piece<T>::one(x + extra(t));
+        lp_move(a, fmaxf(a.m, v));
+        lp_add(a, v);
+    }
+    // the thread's largest element.  a.m says it but for a NaN (which s shows), and where nothing is above -FLT_MAX
+    const bool any = p0 + t < p1 || t < n_extra;
+    uint32_t key = 0;
+    if (p.top && any) {
+        key = lp_key(a.m);
+        if (a.s != a.s || a.m == kLowest) {
+            key = 0;
+            for (uint32_t i = p0 + t; i < p1; i += kThreads)
+                for (int e = 0; e < N; e++) key = max(key, lp_key(Piece<T>::one(xp + (size_t)i * N + e)));
+            if (t < n_extra) key = max(key, lp_key(Piece<T>::one(x + extra(t))));
+        }
+    }
+#pragma unroll
+    for (int w = 16; w; w /= 2) {
+        Sums b;
+        b.m = __shfl_xor_sync(0xffffffffu, a.m, w);
+        b.s = __shfl_xor_sync(0xffffffffu, a.s, w);
+        b.u = __shfl_xor_sync(0xffffffffu, a.u, w);
+        // both sides of a pair add in the same order, so that every lane holds the same bits
+        if (lane & w) { const Sums c = a; a = b; b = c; }
+        lp_join(a, b);
+    }
+    if (lane == 0) sums[warp] = a;
+    if (p.top) {
+        const uint32_t each = (p.top + kWarps - 1) / kWarps;
+        uint32_t k = key, f = 0;
+        for (uint32_t r = 0; r < each; r++) {
+            f = __reduce_max_sync(0xffffffffu, k);
+            const uint32_t at = __ballot_sync(0xffffffffu, k == f);
+            if (lane == __ffs(at) - 1) k = 0;
+        }
+        if (lane == 0) floors[warp] = f;
+        if (t == 0) n_list = 0;
+    }
+    __syncthreads();
+    if (t == 0) {
+        Sums b = sums[0];
+        for (int i = 1; i < kWarps; i++) lp_join(b, sums[i]);
+        whole = b;
+    }
+
+    // ---- the CTA's Top largest elements, in order, into best[] (0: it has fewer)
+    if (p.top) {
+        uint32_t floor = floors[0];
+#pragma unroll
+        for (int i = 1; i < kWarps; i++) floor = min(floor, floors[i]);
+        if (t < kMaxTop) best[t] = 0;
+        // what reaches the floor; where that is more than the list holds (many ties at the floor) what passes it, and
+        // where that is too, nothing: the alternatives are then found one by one
+        bool ties = false;
+        uint32_t n;
+        for (int pass = 0;; pass++) {
+            const auto reaches = [&](uint32_t k) { return pass ? k > floor : k >= floor; };
+            const auto put = [&](float v, uint32_t index) {
+                const uint32_t k = lp_key(v);
+                if (reaches(k)) {
+                    const uint32_t at = atomicAdd(&n_list, 1);  // the places differ from run to run, what is listed does not
+                    if (at < kList) list[at] = (u64)k << 32 | (0xffffffffu - index);
+                }
+            };
+            // a warp reads the pieces of one of its threads at a time
+            for (uint32_t hold = __ballot_sync(0xffffffffu, reaches(key)); hold; hold &= hold - 1) {
+                const uint32_t who = warp * 32 + __ffs(hold) - 1;
+                for (uint32_t i = p0 + who + lane * kThreads; i < p1; i += 32 * kThreads) {
+                    float v[N];
+                    Piece<T>::load(xp + (size_t)i * N, v);
+#pragma unroll
+                    for (int e = 0; e < N; e++) put(v[e], head + i * N + e);
+                }
+                if (lane == 0 && who < n_extra) put(Piece<T>::one(x + extra(who)), extra(who));
+            }
+            __syncthreads();
+            n = n_list;
+            if (n <= kList || pass) break;
+            ties = true;
+            __syncthreads();
+            if (t == 0) n_list = 0;
             __syncthreads();
         }
-        last = shk[0];
-        if (t == 0) {
-            const size_t o = (size_t)row * p.top + r;
-            p.top_ids[o] = 0xffffffffu - (uint32_t)last;
-            p.top_logprobs[o] = (lp_value((uint32_t)(last >> 32)) - m) - log_s;
+        if (n > kList) {
+            // the largest, then the largest below it, and so on over the run
+            u64 last = ~0ull;
+            for (uint32_t r = 0; r < p.top; r++) {
+                u64 b = 0;
+                const auto take = [&](float v, uint32_t index) {
+                    const u64 k = lp_rank(v, index);
+                    if (k < last && k > b) b = k;
+                };
+                for (uint32_t i = p0 + t; i < p1; i += kThreads)
+                    for (int e = 0; e < N; e++) take(Piece<T>::one(xp + (size_t)i * N + e), head + i * N + e);
+                if (t < n_extra) take(Piece<T>::one(x + extra(t)), extra(t));
+                for (int w = 16; w; w /= 2) b = max(b, __shfl_xor_sync(0xffffffffu, b, w));
+                if (lane == 0) slow[warp] = b;
+                __syncthreads();
+                b = slow[0];
+                for (int i = 1; i < kWarps; i++) b = max(b, slow[i]);
+                if (t == 0) best[r] = b;
+                last = b;
+                __syncthreads();
+                if (b == 0) break;
+            }
+        } else {
+            for (uint32_t i = t; i < n; i += kThreads) {
+                const u64 mine = list[i];
+                uint32_t before = 0;
+                for (uint32_t j = 0; j < n; j++) before += list[j] > mine;
+                if (before < p.top) best[before] = mine;
+            }
+            if (ties && n < p.top) {
+                // and the lowest indices that equal the floor: every warp looks for them in an eighth of the run, in order
+                const uint32_t want = p.top - n;
+                const uint32_t first = part == 0 ? 0 : head + p0 * N, end = part == 0 && p1 == pieces ? V : head + p1 * N;
+                const uint32_t run = ((end - first + kWarps - 1) / kWarps + 31) & ~31u;
+                uint32_t have = 0;
+                __syncthreads();                                // list is free for them: kMaxTop to a warp
+                for (uint32_t i0 = warp * run; i0 < (warp + 1) * run && i0 < end - first && have < want; i0 += 32) {
+                    const uint32_t i = first + i0 + lane;
+                    const bool eq = i < end && lp_key(Piece<T>::one(x + i)) == floor;
+                    const uint32_t b = __ballot_sync(0xffffffffu, eq), at = have + __popc(b & ((1u << lane) - 1));
+                    if (eq && at < want) list[warp * kMaxTop + at] = (u64)floor << 32 | (0xffffffffu - i);
+                    have += __popc(b);
+                }
+                if (lane == 0) slow[warp] = min(have, want);
+                __syncthreads();
+                if (t == 0) {
+                    uint32_t at = n;
+                    for (int i = 0; i < kWarps; i++)
+                        for (uint32_t j = 0; j < (uint32_t)slow[i] && at < p.top; j++) best[at++] = list[i * kMaxTop + j];
+                    // (the first CTA of several also holds the elements behind the last whole piece)
+                    for (uint32_t i = max(tail, end); part == 0 && i < V && at < p.top; i++)
+                        if (lp_key(Piece<T>::one(x + i)) == floor) best[at++] = (u64)floor << 32 | (0xffffffffu - i);
+                }
+            }
         }
+    }
+    __syncthreads();
+
+    // ---- the row
+    Sums r = whole;
+    const u64 *order = best;
+    if (parts > 1) {
+        lp_cluster_sync();
+        if (part == 0) {
+            for (uint32_t i = 1; i < parts; i++) {
+                const uint32_t at = lp_mapa(&whole, i);
+                lp_join(r, Sums{lp_remote_f32(at), lp_remote_f32(at + 4), lp_remote_f32(at + 8)});
+            }
+            for (uint32_t i = t; i < parts * p.top; i += kThreads)
+                all[i] = lp_remote_u64(lp_mapa(best + i % p.top, i / p.top));
+        }
+        __syncthreads();
+        lp_cluster_sync();                                // nobody leaves while its part is being read
+        if (part != 0) return;
+        for (uint32_t i = t; i < parts * p.top; i += kThreads) {
+            const u64 mine = all[i];
+            uint32_t before = 0;
+            for (uint32_t j = 0; j < parts * p.top; j++) before += all[j] > mine;
+            if (mine && before < p.top) list[before] = mine;
+        }
+        __syncthreads();
+        order = list;
+    }
+    const float log_s = logf(r.s);
+    if (t == 0) p.entropy[row] = log_s - r.u / r.s;
+    for (uint32_t j = t; j < p.n_targets; j += kThreads) {
+        const uint32_t id = p.targets[(size_t)row * p.n_targets + j];
+        p.logprobs[(size_t)row * p.n_targets + j] = id < V ? (Piece<T>::one(x + id) - r.m) - log_s : CUDART_NAN_F;
+    }
+    if (t < p.top) {
+        const u64 o = order[t];
+        const size_t at = (size_t)row * p.top + t;
+        p.top_ids[at] = 0xffffffffu - (uint32_t)o;
+        p.top_logprobs[at] = (lp_value((uint32_t)(o >> 32)) - r.m) - log_s;
     }
 }
 
@@ -120,16 +371,30 @@ template <typename T> int run_logprobs(Launch &l, const char *name)
                     l.len[0], l.len[1], l.len[2], l.len[3], l.len[4], l.len[5]);
     if (p.top > kMaxTop || p.top > p.vocab)
         return fail(AB_ERR_INVALID, "%s: %u alternatives of a vocabulary of %u; at most %u", name, p.top, p.vocab, kMaxTop);
-    if (p.rows > 0x7fffffffu) return fail(AB_ERR_INVALID, "%s: %u rows", name, p.rows);
+    if (p.rows > 0x0fffffffu || p.vocab > 0x7fffffffu)
+        return fail(AB_ERR_INVALID, "%s: %u rows of %u logits", name, p.rows, p.vocab);
     if (l.query_ws || p.rows == 0) return AB_OK;
     p.x = l.b[0];
     p.targets = ptr<const uint32_t>(l, 1);
     p.logprobs = ptr<float>(l, 2); p.entropy = ptr<float>(l, 3);
     p.top_ids = ptr<uint32_t>(l, 4); p.top_logprobs = ptr<float>(l, 5);
-    logprobs_simple_kernel<T><<<p.rows, kThreads, 0, l.stream>>>(p);
+    // few rows: a row over several CTAs, as long as each has a step of every thread to do
+    uint32_t parts = 1;
+    while (parts < 8 && rows * parts * 2 <= 2ull * sm_count() && p.vocab >= parts * 2 * kThreads * 16 / 2) parts *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.rows * parts);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = l.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, p, parts);
     count_launch();
-    note_selection("%s: a CTA per row", name);
-    return check_cuda(cudaGetLastError(), name);
+    note_selection("%s: %u CTA(s) per row", name, parts);
+    return check_cuda(e, name);
 }
 
 }  // namespace

@@ -151,18 +151,54 @@ def launch(name: str, bindings: Sequence[torch.Tensor], uniform: Optional[bytes]
     _lib.check(rc)
 
 
-def launch_own(name: str, bindings: Sequence[torch.Tensor], uniform: bytes):
-    """`launch` for the operators whose scratch memory is the call's own: it comes from torch's
-    allocator, so a call captured into a CUDA graph keeps it in that graph's pool and two graphs, or
-    two streams, never share it.  A binding of more elements than 32 bits count is passed as
-    0xffffffff, which those kernels read as that many or more."""
+_arrays: dict = {}      # ctypes array types by (element type, length): making one costs more than filling it
+
+
+def _array(kind, values):
+    n = len(values)
+    t = _arrays.get((kind, n))
+    if t is None:
+        t = _arrays.setdefault((kind, n), kind * n)
+    return t(*values)
+
+
+def _on_stream(dev: torch.device, call) -> int:
+    """call(stream) with `dev` current, on its current stream."""
+    if dev.index == torch.cuda.current_device():
+        return call(torch.cuda.current_stream(dev).cuda_stream)
+    with torch.cuda.device(dev):
+        return call(torch.cuda.current_stream(dev).cuda_stream)
+
+
+def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: bytes, scratch: bool = False):
+    """`launch` for the operators whose scratch memory (scratch: they may need some) is the call's own:
+    it comes from torch's allocator, so a call captured into a CUDA graph keeps it in that graph's pool
+    and two graphs, or two streams, never share it.  A binding of None is empty; one of more elements
+    than 32 bits count is passed as 0xffffffff, which those kernels read as that many or more."""
+    L = _lib.lib()
     dev = bindings[0].device
-    lens = [min(t.numel(), 0xffffffff) for t in bindings]
+    if dev.type != "cuda":
+        raise _lib.AccelError(_lib.AB_ERR_NO_DEVICE, f"{name}: bindings live on {dev}; this backend "
+                              "runs on a CUDA device and has no CPU path")
+    ptrs, lens = [], []
+    for t in bindings:
+        if t is None:
+            ptrs.append(None)
+            lens.append(0)
+            continue
+        if t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name}: every binding is a contiguous tensor on {dev}")
+        n = t.numel()
+        ptrs.append(t.data_ptr() if n else None)
+        lens.append(n if n < 0xffffffff else 0xffffffff)
     ws = None
-    if dev.type == "cuda":
+    if scratch:
         need = workspace_bytes(name, lens, uniform)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    launch(name, bindings, uniform, lens, ws)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.check(_on_stream(dev, lambda stream: L.ab_launch(
+        name.encode(), stream, _array(C.c_void_p, ptrs), _array(C.c_uint32, lens), len(ptrs), uniform, len(uniform),
+        ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0)))
 
 
 def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], block: int):
@@ -180,10 +216,10 @@ def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
         if n:
             raise _lib.AccelError(_lib.AB_ERR_INVALID, "copy_pages: the caches are empty")
         return
-    ptrs = (C.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
-    with torch.cuda.device(dev):
-        _lib.check(L.ab_cache_copy_pages(C.c_void_p(torch.cuda.current_stream(dev).cuda_stream), ptrs, len(caches), page_bytes,
-                                         t.shape[0] // block, (C.c_uint32 * n)(*src), (C.c_uint32 * n)(*dst), n))
+    ptrs = _array(C.c_void_p, [c.data_ptr() for c in caches])
+    s, d = (C.c_uint32 * n)(*src), (C.c_uint32 * n)(*dst)
+    _lib.check(_on_stream(dev, lambda stream: L.ab_cache_copy_pages(stream, ptrs, len(caches), page_bytes,
+                                                                    t.shape[0] // block, s, d, n)))
 
 
 def last_selection() -> str:

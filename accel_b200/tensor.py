@@ -632,10 +632,9 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     lp = None if targets is None else torch.empty(targets.shape, dtype=torch.float32, device=dev)
     out = TokenLogprobs(lp, new(rows), torch.empty((rows, top), dtype=U32, device=dev), new(rows, top))
     if rows:
-        none = out.top_ids.new_empty(0)
         rt.launch_own("TokenLogprobsF16" if logits.dtype == torch.float16 else "TokenLogprobs",
-                      [_aligned(logits), none if targets is None else _aligned(targets), none if lp is None else lp,
-                       out.entropy, out.top_ids, out.top_logprobs], rt.logprob_dims(vocab, rows, n, top))
+                      [_aligned(logits), None if targets is None else _aligned(targets), lp, out.entropy,
+                       out.top_ids, out.top_logprobs], rt.logprob_dims(vocab, rows, n, top))
     return out
 
 
