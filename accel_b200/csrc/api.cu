@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "window.cuh"
 
 namespace ab {
 
@@ -1038,6 +1039,13 @@ int ab_int8_dequantize(const int8_t *quants, const uint16_t *scales, size_t n, f
 
 uint16_t ab_f32_to_f16(const float *x) { return x ? f32_to_f16_ref(*x) : 0; }
 void ab_f16_to_f32(uint16_t h, float *out) { if (out) *out = f16_bits_to_f32(h); }
+
+int ab_attention_error(void)
+{
+    const int v = window_error_flag();
+    if (v < 0) return check_cuda(cudaGetLastError(), "ab_attention_error");
+    return v ? fail(AB_ERR_TIMEOUT, "a bounded wait of a windowed prefill ran out; its output is invalid") : AB_OK;
+}
 
 // ------------------------------------------------------------------------------------------------
 // tensor.BlockPool (tensor/blockpool.go:46-133)

@@ -1,0 +1,40 @@
+// Windowed attention: what its row kernel (window_attention.cu) and its tile kernel (window_prefill.cu) share.
+#pragma once
+#include "common.cuh"
+
+namespace ab {
+
+enum Form { kDecode = 0, kBatch = 1, kRaggedStep = 2, kPrefillRows = 3 };
+
+struct WinParams {
+    const float *q;
+    const void *k, *v;
+    const uint32_t *pages, *lengths, *offsets;     // pages NULL: a contiguous cache
+    float *out;
+    uint32_t rows, batch, q_heads, kv_heads, head_dim, block, max_pages;
+    uint32_t window, sinks;
+    uint32_t reach;                                // positions the page table (or the cache) addresses
+    uint32_t capacity;                             // rows of the cache
+    uint32_t base;
+    float scale_log2;                              // Scale * log2(e)
+    int form;
+};
+
+#ifdef __CUDACC__
+// the cache row of position j; 0xffffffff where its page lies outside the cache
+__device__ __forceinline__ uint32_t win_cache_row(const WinParams &p, const uint32_t *pages, uint32_t j)
+{
+    uint64_t r = j;
+    if (pages) {
+        const uint32_t pg = j / p.block;
+        r = (uint64_t)pages[pg] * p.block + (j - pg * p.block);
+    }
+    return r < p.capacity ? (uint32_t)r : 0xffffffffu;
+}
+#endif
+
+// a prefill on 128-row tiles (window_prefill.cu); p.q_heads / p.kv_heads <= 128
+int run_window_tiles(Launch &l, const WinParams &p, bool f16, const char *name);
+int window_error_flag();
+
+}  // namespace ab

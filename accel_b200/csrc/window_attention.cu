@@ -23,28 +23,13 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "window.cuh"
 
 namespace ab {
 
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-
-enum Form { kDecode = 0, kBatch = 1, kRaggedStep = 2, kPrefillRows = 3 };
-
-struct WinParams {
-    const float *q;
-    const void *k, *v;
-    const uint32_t *pages, *lengths, *offsets;     // pages NULL: a contiguous cache
-    float *out;
-    uint32_t rows, batch, q_heads, kv_heads, head_dim, block, max_pages;
-    uint32_t window, sinks;
-    uint32_t reach;                                // positions the page table (or the cache) addresses
-    uint32_t capacity;                             // rows of the cache
-    uint32_t base;
-    float scale_log2;                              // Scale * log2(e)
-    int form;
-};
 
 // What one query row sees.
 struct WinView {
@@ -93,12 +78,7 @@ __device__ __forceinline__ WinView win_view(const WinParams &p, uint32_t row)
 __device__ __forceinline__ uint32_t win_row(const WinParams &p, const WinView &w, uint32_t i)
 {
     const uint32_t j = i < w.ns ? i : w.lo + (i - w.ns);
-    uint64_t r = j;
-    if (w.pages) {
-        const uint32_t pg = j / p.block;
-        r = (uint64_t)w.pages[pg] * p.block + (j - pg * p.block);
-    }
-    return r < p.capacity ? (uint32_t)r : 0xffffffffu;
+    return win_cache_row(p, w.pages, j);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -564,13 +544,19 @@ template <typename T, int DP> int launch_rows(Launch &l, const WinParams &p, con
     return check_cuda(e, name);
 }
 
+// query rows (tokens x heads of a KV head) of one sequence from which 128-row tiles take over
+constexpr uint32_t kTileFrom = 64;
+
 template <typename T> int run_window(Launch &l, WinParams &p, const char *name)
 {
     if ((uint64_t)p.base + p.rows > 0xffffffffull)
         return fail(AB_ERR_INVALID, "%s: Base=%u and %u rows pass 32 bits", name, p.base, p.rows);
     l.ws_need = 0;
-    if (l.query_ws) return AB_OK;
     if (p.rows == 0) return AB_OK;
+    const uint32_t group = p.q_heads / p.kv_heads;
+    if (p.form == kPrefillRows && group <= 128 && (uint64_t)p.rows * group >= kTileFrom)
+        return run_window_tiles(l, p, sizeof(T) == 2, name);
+    if (l.query_ws) return AB_OK;
     return p.head_dim <= 64 ? launch_rows<T, 64>(l, p, name) : launch_rows<T, 128>(l, p, name);
 }
 

@@ -1,0 +1,620 @@
+// Attention with a sliding window for many query rows of one sequence (a prompt, or a chunk of one), on
+// the tensor cores of sm_100a: tcgen05 with the operands in shared and tensor memory.  What it
+// computes is defined in window_attention.cu, whose row kernel does the same for few rows.
+//
+// Two kernels.  win_pack_kernel gathers the positions that any of the rows sees, through the page table, into
+// tiles of 128 positions per KV head, as the MMAs read them (K-major 8 x 8 core matrices; V transposed),
+// so that the tile kernel fetches an operand with one bulk copy, whatever the pages, strides or head
+// dimension were.  win_tile_kernel takes 128 query rows (tokens x the query heads of one KV head, so the
+// group shares every tile) over the tiles its rows see.
+//
+// Accuracy.  q, K and V have up to 24 bits and f16 holds 11, so an operand is two f16 parts, x = hi + lo,
+// and a product three MMAs, lo.hi + hi.lo + hi.hi (2^-22 is dropped); an f16 cache is exact in one
+// part and its products take two.  Powers of two keep the parts inside f16's range: one per query row
+// and one per tile of an f32 cache; the softmax weights are carried times 2^14 (window_attention.cu).
+// The accumulators of a tile start from zero, the small products first, and the sums over tiles are
+// f32 additions in registers: an accumulator in the tensor core over thousands of positions would
+// truncate at every step.
+//
+// Bound: the tensor pipe.  4 (f16 cache) or 6 (f32) MMAs of 128 x 128 x 128 for every 128 x 128 scores where
+// 2 would be the floor.  A CTA of 320 threads per SM: two groups of four warps do the softmax of the even
+// and the odd tiles, each with its own maximum, sum and output in registers, so that one group's
+// exponentials run under the other's MMAs; one lane issues the MMAs in the order QK(0) QK(1) PV(0) QK(2)
+// PV(1) ..., one lane the bulk copies, in the same order, into a ring of slots.  Tensor memory: 128 columns of
+// scores and 128 of output for each group; the weights overwrite their scores.
+#include <algorithm>
+#include <math_constants.h>
+
+#include <mutex>
+
+#include "common.cuh"
+#include "sm100.cuh"
+#include "window.cuh"
+
+namespace ab {
+
+namespace {
+
+constexpr int kKeys = 128;                  // positions of a tile
+constexpr int kRows = 128;                  // query rows of a CTA
+constexpr int kSoftWarps = 8;
+constexpr int kTileThreads = kSoftWarps * 32 + 64;
+constexpr int kSlots = 5;
+constexpr float kBias = 14.f;               // the softmax weights are carried times 2^14
+
+// What the pack kernel says about a tile.
+struct TileHead {
+    float k_scale, v_scale;                 // what the parts have to be multiplied by
+    uint32_t bad;                           // a value is not finite (it is left out of the tile)
+    uint32_t pad;
+    uint32_t seen[4];                       // a bit per position: it exists
+};
+
+// The list of positions packed for a call: sinks in front of the first row's window, then all from that on.
+struct Keys {
+    uint32_t ns, lo;                        // positions [0, ns) and [lo, ...)
+    uint32_t sink_tiles, tiles;
+};
+__host__ __device__ inline Keys win_keys(const WinParams &p)
+{
+    Keys k;
+    const uint64_t first = (uint64_t)p.base + 1, end = (uint64_t)p.base + p.rows;
+    k.lo = (uint32_t)(first > p.window ? first - p.window : 0);
+    k.ns = p.sinks < k.lo ? p.sinks : k.lo;
+    k.sink_tiles = (k.ns + kKeys - 1) / kKeys;
+    k.tiles = k.sink_tiles + (uint32_t)((end - k.lo + kKeys - 1) / kKeys);
+    return k;
+}
+__device__ __forceinline__ uint32_t win_tile_start(const Keys &k, uint32_t tile)
+{
+    return tile < k.sink_tiles ? tile * kKeys : k.lo + (tile - k.sink_tiles) * kKeys;
+}
+
+template <typename T> constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
+template <typename T, int DP> constexpr uint32_t kSlotBytes = kKeys * DP * 2;
+template <typename T, int DP> constexpr uint32_t kTileBytes = 2 * kParts<T> * kSlotBytes<T, DP>;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+
+// the power of two that brings a largest magnitude into [2^13, 2^14), as an exponent
+__device__ __forceinline__ int fit_exponent(float amax)
+{
+    const int e = amax > 0.f ? 13 - ((int)(__float_as_uint(amax) >> 23) - 127) : 0;
+    return min(max(e, -126), 126);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float x, float y)
+{
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// x = hi + lo in f16
+__device__ __forceinline__ void split_f16x2(float x, float y, uint32_t &hi, uint32_t &lo)
+{
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = pack_f16x2(x - f.x, y - f.y);
+}
+__device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo)
+{
+    split_f16x2(x[0], x[1], hi.x, lo.x);
+    split_f16x2(x[2], x[3], hi.y, lo.y);
+    split_f16x2(x[4], x[5], hi.z, lo.z);
+    split_f16x2(x[6], x[7], hi.w, lo.w);
+}
+
+// ------------------------------------------------------------------------------------------------
+// grid (tiles, KV heads of this pass, 2): K or V of one tile.  An operand's element (r, c), c along the contraction, lies
+// at (c / 8) * rows * 16 + r * 16 + (c % 8) * 2: 128 rows of positions for K, DP rows of dimensions for V.
+// Every element is read once and written once per part: HBM (or L2) bounds it.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) win_pack_kernel(const WinParams p, const Keys keys, unsigned char *tiles, TileHead *heads,
+                                                       uint32_t kvh0)
+{
+    __shared__ uint32_t rows[kKeys], amax_bits, bad_any;
+    const uint32_t tile = blockIdx.x, kvh = kvh0 + blockIdx.y, t = threadIdx.x, D = p.head_dim;
+    const size_t at = (size_t)blockIdx.y * keys.tiles + tile;
+    TileHead &head = heads[at];
+    unsigned char *dst = tiles + at * kTileBytes<T, DP> + (blockIdx.z ? kParts<T> * kSlotBytes<T, DP> : 0);
+    if (t == 0) { amax_bits = 0; bad_any = 0; }
+    if (t < kKeys) {
+        const uint64_t j = (uint64_t)win_tile_start(keys, tile) + t;
+        const uint32_t len = min(p.lengths[0], p.reach);
+        uint32_t r = 0xffffffffu;
+        if (j < len && (tile >= keys.sink_tiles || j < keys.ns) && j < (uint64_t)p.base + p.rows)
+            r = win_cache_row(p, p.pages, (uint32_t)j);
+        rows[t] = r;
+        const uint32_t seen = __ballot_sync(0xffffffffu, r != 0xffffffffu);
+        if (blockIdx.z == 0 && (t & 31) == 0) head.seen[t >> 5] = seen;
+    }
+    __syncthreads();
+    constexpr int kEach = kKeys * DP / 256;              // elements of a thread
+    float x[kEach];
+    float big = 0.f;
+    bool bad = false;
+    // K: a thread holds half the dimensions of a position; V: eight positions of a dimension at a time, neighbouring threads
+    // neighbouring dimensions
+    const uint32_t key = t & (kKeys - 1), d0 = (t >> 7) * (DP / 2), dim = t & (DP - 1), group0 = t / DP;
+    if (blockIdx.z == 0) {
+        const T *src = static_cast<const T *>(p.k) + ((uint64_t)(rows[key] == 0xffffffffu ? 0 : rows[key]) * p.kv_heads + kvh) * D;
+        const bool on = rows[key] != 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < kEach; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[i + e] = 0.f;
+            if (on && d0 + i < D) {
+                uint4 raw[sizeof(T) / 2];
+#pragma unroll
+                for (int r = 0; r < (int)sizeof(T) / 2; r++) raw[r] = __ldg(reinterpret_cast<const uint4 *>(src + d0 + i) + r);
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[i + e] = to_f32(reinterpret_cast<const T *>(raw)[e]);
+            }
+        }
+    } else {
+        const T *v = static_cast<const T *>(p.v);
+#pragma unroll
+        for (int i = 0; i < kEach; i++) {
+            const uint32_t r = rows[(i / 8 * (256 / DP) + group0) * 8 + (i & 7)];
+            x[i] = r != 0xffffffffu && dim < D ? to_f32(v[((uint64_t)r * p.kv_heads + kvh) * D + dim]) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+        const bool finite = fabsf(x[i]) <= 3.402823466e38f;
+        if (finite) big = fmaxf(big, fabsf(x[i]));
+        else bad = true;
+        // a value that is not finite would spoil rows that do not see it (0 * inf): it is left out here and added to the
+        // rows that do by the tile kernel.  A score is masked after its product, so a key may stay
+        if (!finite && blockIdx.z) x[i] = 0.f;
+    }
+    if (sizeof(T) == 4) {
+        const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+        if ((t & 31) == 0) atomicMax(&amax_bits, b);
+    }
+    if (blockIdx.z && __any_sync(0xffffffffu, bad) && (t & 31) == 0) bad_any = 1;
+    __syncthreads();
+    const int e = sizeof(T) == 4 ? fit_exponent(__uint_as_float(amax_bits)) : 0;
+    if (t == 0) {
+        if (blockIdx.z) { head.v_scale = ab_pow2(-e); head.bad = bad_any; }
+        else head.k_scale = ab_pow2(-e);
+    }
+    const float f = ab_pow2(e);
+#pragma unroll
+    for (int i = 0; i < kEach; i += 8) {
+        float y[8];
+#pragma unroll
+        for (int n = 0; n < 8; n++) y[n] = x[i + n] * f;
+        uint4 hi, lo;
+        split8(y, hi, lo);
+        const uint32_t to = blockIdx.z ? (i / 8 * (256 / DP) + group0) * (DP * 16) + dim * 16 : (d0 + i) / 8 * (kKeys * 16) + key * 16;
+        *reinterpret_cast<uint4 *>(dst + to) = hi;
+        if (kParts<T> == 2) *reinterpret_cast<uint4 *>(dst + kSlotBytes<T, DP> + to) = lo;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+template <typename T, int DP> struct TileSmem {
+    static constexpr uint32_t kQ = kRows * DP * 2;                  // one part of the query rows
+    static constexpr uint32_t kRing = 2 * kQ;
+    static constexpr uint32_t kBars = kRing + kSlots * kSlotBytes<T, DP>;
+    static constexpr uint32_t kBytes = kBars + 256;
+};
+
+// D[tmem_d] (+)= A[smem] * B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// bits [a, b) of a word, a and b clipped to it
+__device__ __forceinline__ uint32_t bit_range(int a, int b)
+{
+    a = max(a, 0);
+    b = min(b, 32);
+    return a < b ? (0xffffffffu >> (32 - (b - a))) << a : 0u;
+}
+
+// The tiles that the rows at positions [pa, pb] see: [0, sinks_end) and [begin, end).
+struct Range { uint32_t sinks_end, begin, end; };
+__device__ __forceinline__ Range win_range(const WinParams &p, const Keys &k, uint64_t pa, uint64_t pb)
+{
+    const uint32_t lo = (uint32_t)(pa + 1 > p.window ? pa + 1 - p.window : 0), s = min(p.sinks, lo);
+    Range r;
+    r.sinks_end = s <= k.ns ? (s + kKeys - 1) / kKeys : k.sink_tiles + (s - k.lo + kKeys - 1) / kKeys;
+    r.begin = max(r.sinks_end, k.sink_tiles + (lo - k.lo) / kKeys);
+    r.end = k.sink_tiles + (uint32_t)((pb + 1 - k.lo + kKeys - 1) / kKeys);
+    return r;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTileThreads, 1)
+win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, const TileHead *heads, uint32_t kvh0, uint32_t row_tiles)
+{
+    using Smem = TileSmem<T, DP>;
+    constexpr uint32_t kSlot = kSlotBytes<T, DP>;
+    constexpr uint32_t kLboRows = kRows * 16, kLboDims = DP * 16;
+    constexpr int kP = kParts<T>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + Smem::kBars), *freeb = full + kSlots;
+    uint64_t *s_ready = freeb + kSlots, *p_ready = s_ready + 2, *d_ready = p_ready + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(d_ready + 2);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // the rows: tokens x heads of the group; the last tokens, which see most, first
+    const uint32_t group = p.q_heads / p.kv_heads, per_tile = kRows / group, D = p.head_dim;
+    const uint32_t kv = blockIdx.x / row_tiles, rt = row_tiles - 1 - blockIdx.x % row_tiles;
+    const uint32_t tok0 = rt * per_tile, tokens = min(per_tile, p.rows - tok0);
+    const uint64_t pa = (uint64_t)p.base + tok0;
+    const Range range = win_range(p, keys, pa, pa + tokens - 1);
+    const uint32_t n = range.sinks_end + (range.end - range.begin);
+    const auto tile_of = [&](uint32_t i) { return i < range.sinks_end ? i : range.begin + (i - range.sinks_end); };
+    tiles += (size_t)kv * keys.tiles * kTileBytes<T, DP>;
+    heads += (size_t)kv * keys.tiles;
+
+    if (warp == kSoftWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sx_smem(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (warp == kSoftWarps + 1 && lane == 0) {
+        for (int i = 0; i < kSlots; i++) { sx_bar_init(&full[i], 1); sx_bar_init(&freeb[i], 1); }
+        for (int i = 0; i < 2; i++) { sx_bar_init(&s_ready[i], 1); sx_bar_init(&p_ready[i], 4); sx_bar_init(&d_ready[i], 1); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // the query rows, a thread half a row: scaled, split, stored as the A operand
+    const uint32_t r = tid & (kRows - 1), token = tok0 + r / group;
+    const uint32_t head = (kvh0 + kv) * group + r % group;
+    const bool live = r < tokens * group;
+    float q_scale = 1.f;
+    if (warp < kSoftWarps) {
+        const float *q = p.q + ((uint64_t)(live ? token : 0) * p.q_heads + (live ? head : 0)) * D;
+        float amax = 0.f;
+        for (uint32_t d = 0; d < D; d += 4) {
+            const float4 v = live ? __ldg(reinterpret_cast<const float4 *>(q + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        }
+        amax = fminf(amax * fabsf(p.scale_log2), 3.402823466e38f);
+        // near one: the products with keys of up to 2^14 (or f16's largest) stay far inside f32
+        const int e = min(fit_exponent(amax) - 13, 126);
+        const float f = ab_pow2(max(e, -126));
+        q_scale = ab_pow2(-max(e, -126));
+        for (uint32_t d = (tid >> 7) * (DP / 2); d < ((uint32_t)(tid >> 7) + 1) * (DP / 2); d += 8) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (live && d + i < D) v = __ldg(reinterpret_cast<const float4 *>(q + d + i));
+                x[i] = v.x * p.scale_log2 * f; x[i + 1] = v.y * p.scale_log2 * f;
+                x[i + 2] = v.z * p.scale_log2 * f; x[i + 3] = v.w * p.scale_log2 * f;
+            }
+            uint4 hi, lo;
+            split8(x, hi, lo);
+            *reinterpret_cast<uint4 *>(smem + d / 8 * kLboRows + r * 16) = hi;
+            *reinterpret_cast<uint4 *>(smem + Smem::kQ + d / 8 * kLboRows + r * 16) = lo;
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+
+    float m = -CUDART_INF_F, l = 0.f, o[DP];
+    uint32_t bad = 0;
+    if (warp == kSoftWarps + 1) {
+        // ---- the copies, in the order the MMAs take them: K(0) K(1) V(0) K(2) V(1) ...
+        if (lane == 0) {
+            uint32_t slot = 0, use = 0, issued = 0;
+            bool ok = true;
+            const auto load = [&](uint32_t i, uint32_t which) {
+                for (int part = 0; part < kP && ok; part++) {
+                    if (use) ok = sx_bar_wait(&freeb[slot], (use - 1) & 1);
+                    if (!ok) return;
+                    sx_bar_expect_tx(&full[slot], kSlot);
+                    sx_bulk_load(smem + Smem::kRing + slot * kSlot,
+                                 tiles + (size_t)tile_of(i) * kTileBytes<T, DP> + (which * kP + part) * kSlot, kSlot, &full[slot]);
+                    issued++;
+                    if (++slot == kSlots) { slot = 0; use++; }
+                }
+            };
+            if (n) load(0, 0);
+            for (uint32_t i = 0; i < n && ok; i++) {
+                if (i + 1 < n) load(i + 1, 0);
+                load(i, 1);
+            }
+            // nothing may be in flight when the CTA's shared memory goes to another
+            for (uint32_t i = issued > kSlots ? issued - kSlots : 0; i < issued; i++) sx_bar_wait(&full[i % kSlots], (i / kSlots) & 1);
+        }
+    } else if (warp == kSoftWarps) {
+        // ---- the MMAs
+        if (lane == 0) {
+            constexpr uint32_t kS = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
+            constexpr uint32_t kO = (1u << 4) | ((uint32_t)(DP >> 3) << 17) | ((kRows >> 4) << 24);
+            uint32_t slot = 0, use = 0;
+            bool ok = true;
+            const uint32_t q_at = sx_smem(smem), ring = sx_smem(smem + Smem::kRing);
+            uint32_t at[kP], sl[kP];
+            const auto take = [&]() {                           // the next operand's parts
+                for (int part = 0; part < kP && ok; part++) {
+                    ok = sx_bar_wait(&full[slot], use & 1);
+                    at[part] = ring + slot * kSlot;
+                    sl[part] = slot;
+                    if (++slot == kSlots) { slot = 0; use++; }
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            };
+            const auto scores = [&](uint32_t i) {
+                take();
+                if (!ok) return;
+                const uint32_t d = tmem + (i & 1) * 256;
+                const auto pass = [&](uint32_t q, uint32_t k, uint32_t first) {
+#pragma unroll
+                    for (int j = 0; j < DP / 16; j++)
+                        mma_ss(d, sx_desc(q + j * 2 * kLboRows, kLboRows, 128), sx_desc(k + j * 2 * kKeys * 16, kKeys * 16, 128), kS,
+                               !(first && j == 0));
+                };
+                pass(q_at + Smem::kQ, at[0], 1);
+                if (kP == 2) { pass(q_at, at[kP - 1], 0); sx_commit(&freeb[sl[kP - 1]]); }
+                pass(q_at, at[0], 0);
+                sx_commit(&freeb[sl[0]]);
+                sx_commit(&s_ready[i & 1]);
+            };
+            const auto values = [&](uint32_t i) {
+                take();
+                ok = ok && sx_bar_wait(&p_ready[i & 1], (i >> 1) & 1);
+                if (!ok) return;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t w = tmem + (i & 1) * 256, d = w + 128;
+                // 32 positions' weights: 16 columns of high parts, 16 of low ones
+                const auto pass = [&](uint32_t lo, uint32_t v, uint32_t first) {
+#pragma unroll
+                    for (int j = 0; j < kKeys / 16; j++)
+                        sx_mma_ts(d, w + (j >> 1) * 32 + lo + (j & 1) * 8, sx_desc(v + j * 2 * kLboDims, kLboDims, 128), kO,
+                                  !(first && j == 0));
+                };
+                pass(16, at[0], 1);
+                if (kP == 2) { pass(0, at[kP - 1], 0); sx_commit(&freeb[sl[kP - 1]]); }
+                pass(0, at[0], 0);
+                sx_commit(&freeb[sl[0]]);
+                sx_commit(&d_ready[i & 1]);
+            };
+            if (n) scores(0);
+            for (uint32_t i = 0; i < n && ok; i++) {
+                if (i + 1 < n) scores(i + 1);
+                if (ok) values(i);
+            }
+        }
+    } else {
+        // ---- the softmax of every other tile; a thread has a row
+        const int wg = warp >> 2;
+        const uint32_t ts = tmem + wg * 256 + ((uint32_t)(warp & 3) << 21), td = ts + 128;
+        const int64_t pos = (int64_t)p.base + (live ? token : tok0);
+        const int64_t lo_row = pos + 1 > (int64_t)p.window ? pos + 1 - (int64_t)p.window : 0;
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < DP; i++) o[i] = 0.f;
+        for (uint32_t i = wg; i < n; i += 2) {
+            const uint32_t tile = tile_of(i);
+            const int64_t j0 = win_tile_start(keys, tile);
+            const TileHead &h = heads[tile];
+            const float c = fmaxf(q_scale * __ldg(&h.k_scale), 1.2e-38f), vs = __ldg(&h.v_scale);
+            bad |= __ldg(&h.bad);
+            const uint4 seen = __ldg(reinterpret_cast<const uint4 *>(h.seen));
+            // does every row of the CTA see the whole tile?
+            const bool whole = (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && j0 + kKeys - 1 <= (int64_t)pa &&
+                               j0 + (int64_t)p.window > (int64_t)(pa + tokens - 1);
+            uint32_t mask[4] = {seen.x, seen.y, seen.z, seen.w};
+            if (!whole) {
+                const int top = (int)min(max(pos - j0 + 1, (int64_t)0), (int64_t)kKeys);
+                const int low = (int)min(max(lo_row - j0, (int64_t)0), (int64_t)kKeys);
+                const int snk = (int)min(max((int64_t)p.sinks - j0, (int64_t)0), (int64_t)kKeys);
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    mask[w] &= bit_range(0, top - 32 * w) & (bit_range(low - 32 * w, 32) | bit_range(0, snk - 32 * w));
+            }
+            ok = __all_sync(0xffffffffu, sx_bar_wait(&s_ready[wg], (i >> 1) & 1));
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float top = -CUDART_INF_F;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                uint32_t s[32];
+                tmem_ld32(ts + 32 * w, s);
+                if (whole) {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) top = fmaxf(top, __uint_as_float(s[e]));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++)
+                        if ((mask[w] >> e) & 1) top = fmaxf(top, __uint_as_float(s[e]));
+                }
+            }
+            // (rounded up to a 64th: m1 - 14 is then exact, and so the weights of all tiles are relative to the same maxima)
+            const float m1 = fmaxf(m, ceilf(top * c * 64.f) * 0.015625f), ms = (m1 == -CUDART_INF_F ? 0.f : m1) - kBias;
+            const float a = m == m1 ? 1.f : ex2(m - (ms + kBias));
+            m = m1;
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                uint32_t s[32], out[32];
+                tmem_ld32(ts + 32 * w, s);
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float x = __uint_as_float(s[e]), y = __uint_as_float(s[e + 1]);
+                    if (!whole) {
+                        if (!((mask[w] >> e) & 1)) x = -CUDART_INF_F;
+                        if (!((mask[w] >> (e + 1)) & 1)) y = -CUDART_INF_F;
+                    }
+                    x = ex2(fmaf(x, c, -ms));
+                    y = ex2(fmaf(y, c, -ms));
+                    sum += x + y;
+                    split_f16x2(x, y, out[e / 2], out[16 + e / 2]);
+                }
+                tmem_st32(ts + 32 * w, out);
+            }
+            l = fmaf(l, a, sum);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) sx_bar_arrive(&p_ready[wg]);
+            ok = __all_sync(0xffffffffu, sx_bar_wait(&d_ready[wg], (i >> 1) & 1));
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int w = 0; w < DP / 32; w++) {
+                uint32_t d[32];
+                tmem_ld32(td + 32 * w, d);
+#pragma unroll
+                for (int e = 0; e < 32; e++)
+                    o[32 * w + e] = fmaf(o[32 * w + e], a, sizeof(T) == 4 ? __uint_as_float(d[e]) * vs : __uint_as_float(d[e]));
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        }
+    }
+    // ---- both groups' parts of a row: each hands the other half of its dimensions through shared memory
+    __syncthreads();
+    float *swap = reinterpret_cast<float *>(smem), *ml = swap + kRows * DP;     // [group][DP / 2][row]; [group][m, l, bad][row]
+    const int wg = warp >> 2;
+    if (warp < kSoftWarps) {
+#pragma unroll
+        for (int i = 0; i < DP / 2; i++) swap[(wg * (DP / 2) + i) * kRows + r] = wg ? o[i] : o[DP / 2 + i];
+        ml[(wg * 3) * kRows + r] = m;
+        ml[(wg * 3 + 1) * kRows + r] = l;
+        ml[(wg * 3 + 2) * kRows + r] = __uint_as_float(bad);
+    }
+    __syncthreads();
+    if (warp < kSoftWarps && live) {
+        const float m2 = ml[((wg ^ 1) * 3) * kRows + r], l2 = ml[((wg ^ 1) * 3 + 1) * kRows + r], M = fmaxf(m, m2);
+        bad |= __float_as_uint(ml[((wg ^ 1) * 3 + 2) * kRows + r]);
+        const float f1 = m == -CUDART_INF_F ? 0.f : ex2(m - M), f2 = m2 == -CUDART_INF_F ? 0.f : ex2(m2 - M);
+        // (in the order of the groups, so that both halves divide by the same sum)
+        const float sum = wg ? fmaf(l2, f2, l * f1) : fmaf(l, f1, l2 * f2);
+        float *out = p.out + ((uint64_t)token * p.q_heads + head) * D + wg * (DP / 2);
+#pragma unroll
+        for (int i = 0; i < DP / 2; i += 4) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                x[e] = fmaf(swap[((wg ^ 1) * (DP / 2) + i + e) * kRows + r], f2, (wg ? o[DP / 2 + i + e] : o[i + e]) * f1) / sum;
+            if ((uint32_t)(wg * (DP / 2) + i) < D) *reinterpret_cast<float4 *>(out + i) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+        if (bad) {
+            // values that are not finite were left out of the tiles: a row that sees one gets it added
+            const int64_t pos = (int64_t)p.base + token;
+            const uint64_t end = min((uint64_t)min(p.lengths[0], p.reach), (uint64_t)pos + 1);
+            for (uint32_t i = 0; i < n; i++) {
+                const uint32_t tile = tile_of(i);
+                if (!heads[tile].bad) continue;
+                for (uint32_t x = 0; x < (uint32_t)kKeys; x++) {
+                    const uint64_t j = (uint64_t)win_tile_start(keys, tile) + x;
+                    if (!((heads[tile].seen[x >> 5] >> (x & 31)) & 1) || j >= end || (pos - (int64_t)j >= (int64_t)p.window && j >= p.sinks))
+                        continue;
+                    const T *v = static_cast<const T *>(p.v) +
+                                 ((uint64_t)win_cache_row(p, p.pages, (uint32_t)j) * p.kv_heads + kvh0 + kv) * D + wg * (DP / 2);
+                    for (uint32_t d = 0; d < DP / 2 && wg * (DP / 2) + d < D; d++) {
+                        const float y = to_f32(v[d]);
+                        if (!(fabsf(y) <= 3.402823466e38f)) out[d] += y;
+                    }
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == kSoftWarps) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <typename T, int DP> int tile_prepare(const char *name)
+{
+    static std::mutex mu;
+    static uint64_t done[4];                             // a bit per device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= 0 && dev < 256 && (done[dev / 64] >> (dev % 64) & 1)) return AB_OK;
+    const int rc = check_cuda(cudaFuncSetAttribute(win_tile_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   TileSmem<T, DP>::kBytes), name);
+    if (rc == AB_OK && dev >= 0 && dev < 256) done[dev / 64] |= 1ull << (dev % 64);
+    return rc;
+}
+
+constexpr uint64_t kPassBytes = 1ull << 30;              // tiles of one pass over KV heads
+
+template <typename T, int DP> int run_tiles(Launch &l, const WinParams &p, const char *name)
+{
+    static_assert(TileSmem<T, DP>::kBytes <= 232448, "shared memory of a CTA");
+    static_assert(kRows * DP * 4 + 6 * kRows * 4 <= TileSmem<T, DP>::kBars, "the parts of both groups fit where the operands were");
+    const Keys keys = win_keys(p);
+    const uint64_t per_head = (uint64_t)keys.tiles * kTileBytes<T, DP>;
+    const uint32_t pass = (uint32_t)std::min<uint64_t>(p.kv_heads, std::max<uint64_t>(1, kPassBytes / per_head));
+    const uint64_t head_bytes = align_up((size_t)pass * keys.tiles * sizeof(TileHead), 256);
+    l.ws_need = (size_t)(head_bytes + pass * per_head);
+    if (l.query_ws) return AB_OK;
+    if (l.ws_need > l.ws_bytes || !l.ws)
+        return fail(AB_ERR_INVALID, "%s: needs %zu bytes of workspace, given %zu", name, l.ws_need, l.ws_bytes);
+    const uint32_t per_tile = kRows / (p.q_heads / p.kv_heads), row_tiles = (p.rows + per_tile - 1) / per_tile;
+    if ((uint64_t)row_tiles * pass > 0x7fffffffull || keys.tiles > 0x7fffffffu || pass > 65535)
+        return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
+    int rc = tile_prepare<T, DP>(name);
+    if (rc) return rc;
+    TileHead *heads = static_cast<TileHead *>(l.ws);
+    unsigned char *tiles = static_cast<unsigned char *>(l.ws) + head_bytes;
+    for (uint32_t h = 0; h < p.kv_heads; h += pass) {
+        const uint32_t now = std::min(pass, p.kv_heads - h);
+        win_pack_kernel<T, DP><<<dim3(keys.tiles, now, 2), 256, 0, l.stream>>>(p, keys, tiles, heads, h);
+        count_launch();
+        rc = check_cuda(cudaGetLastError(), name);
+        if (rc) return rc;
+        win_tile_kernel<T, DP><<<row_tiles * now, kTileThreads, TileSmem<T, DP>::kBytes, l.stream>>>(p, keys, tiles, heads, h, row_tiles);
+        count_launch();
+        rc = check_cuda(cudaGetLastError(), name);
+        if (rc) return rc;
+    }
+    note_selection("%s: tcgen05 tiles, %u positions packed, %u x %u CTAs of 128 rows, %u pass(es)", name,
+                   keys.tiles * (uint32_t)kKeys, row_tiles, pass, (p.kv_heads + pass - 1) / pass);
+    return AB_OK;
+}
+
+}  // namespace
+
+int run_window_tiles(Launch &l, const WinParams &p, bool f16, const char *name)
+{
+    if (f16) return p.head_dim <= 64 ? run_tiles<__half, 64>(l, p, name) : run_tiles<__half, 128>(l, p, name);
+    return p.head_dim <= 64 ? run_tiles<float, 64>(l, p, name) : run_tiles<float, 128>(l, p, name);
+}
+
+int window_error_flag()
+{
+    int v = 0;
+    return cudaMemcpyFromSymbol(&v, g_sm100_error, sizeof v) == cudaSuccess ? v : -1;
+}
+
+}  // namespace ab

@@ -222,6 +222,11 @@ def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
                                                                     t.shape[0] // block, s, d, n)))
 
 
+def attention_error():
+    """Raises once a bounded device-side wait of a windowed prefill has run out (synchronous; sticky)."""
+    _lib.check(_lib.lib().ab_attention_error())
+
+
 def last_selection() -> str:
     return _lib.lib().ab_last_selection().decode()
 

@@ -393,6 +393,9 @@ AB_API int ab_int4_prepack(void *stream, const uint32_t *codes, const uint16_t *
  * (synchronous; sticky for the process). */
 AB_API int ab_int4_stream_error(void);
 
+/* The same for the windowed prefill's tile kernel (AttentionWindowPrefill... from 64 query rows of a KV head on). */
+AB_API int ab_attention_error(void);
+
 /* ---- One-shot all-reduce over NVLink peer memory (tensor-parallel decode) -----------------
  * No reference counterpart: accel is single-device (the tensor-parallel layer sits above the
  * per-device plan).  Sums `n` f32 values (a multiple of 4) over `world` <= 8 ranks, one process per

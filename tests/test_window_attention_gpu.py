@@ -306,3 +306,11 @@ def test_views_and_unaligned_tables():
     tab = table.cpu().numpy()
     phys = [int(tab[j // block]) * block + j % block for j in visible(n - 1, n, 30, 5)]
     check(got, *attend(q, k.cpu().numpy(), v.cpu().numpy(), phys, 0.2, 2), "views")
+
+
+def test_no_wait_ran_out():
+    _job(9, 300)()
+    assert "tcgen05 tiles" in rt.last_selection()
+    rt.attention_error()
+    _job(9, 3)()
+    assert "tcgen05 tiles" not in rt.last_selection()
