@@ -38,7 +38,7 @@ namespace {
 constexpr int kKeys = 128;                  // positions of a tile
 constexpr int kRows = 128;                  // query rows of a CTA
 constexpr int kSoftWarps = 8;
-constexpr int kTileThreads = kSoftWarps * 32 + 64;
+constexpr int kTileThreads = kSoftWarps * 32 + 128;
 constexpr int kSlots = 5;
 constexpr float kBias = 14.f;               // the softmax weights are carried times 2^14
 
@@ -201,6 +201,19 @@ template <typename T, int DP> struct TileSmem {
     static constexpr uint32_t kBytes = kBars + 256;
 };
 
+// sx_bar_wait without its function call: the softmax threads hold more registers than survive one
+__device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity)
+{
+    const uint32_t addr = sx_smem(bar);
+    if (sx_bar_try(addr, parity)) return true;
+    const long long t0 = clock64();
+    while (!sx_bar_try(addr, parity))
+        if (clock64() - t0 > kSxWaitCycles) {
+            atomicExch(&g_sm100_error, 1);
+            return false;
+        }
+    return true;
+}
 // D[tmem_d] (+)= A[smem] * B[smem]
 __device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
 {
@@ -219,16 +232,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
                    "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr) : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
 __device__ __forceinline__ float ex2(float x)
 {
@@ -327,93 +330,99 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
-    float m = -CUDART_INF_F, l = 0.f, o[DP];
-    uint32_t bad = 0;
-    if (warp == kSoftWarps + 1) {
-        // ---- the copies, in the order the MMAs take them: K(0) K(1) V(0) K(2) V(1) ...
-        if (lane == 0) {
-            uint32_t slot = 0, use = 0, issued = 0;
-            bool ok = true;
-            const auto load = [&](uint32_t i, uint32_t which) {
-                for (int part = 0; part < kP && ok; part++) {
-                    if (use) ok = sx_bar_wait(&freeb[slot], (use - 1) & 1);
-                    if (!ok) return;
-                    sx_bar_expect_tx(&full[slot], kSlot);
-                    sx_bulk_load(smem + Smem::kRing + slot * kSlot,
-                                 tiles + (size_t)tile_of(i) * kTileBytes<T, DP> + (which * kP + part) * kSlot, kSlot, &full[slot]);
-                    issued++;
-                    if (++slot == kSlots) { slot = 0; use++; }
+    // 168 registers a thread at launch; the softmax groups take what the other four warps do not need:
+    // 2 x 128 x 224 + 128 x 56 = 384 x 168
+    if (warp >= kSoftWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == kSoftWarps + 1) {
+            // ---- the copies, in the order the MMAs take them: K(0) K(1) V(0) K(2) V(1) ...
+            if (lane == 0) {
+                uint32_t slot = 0, use = 0, issued = 0;
+                bool ok = true;
+                const auto load = [&](uint32_t i, uint32_t which) {
+                    for (int part = 0; part < kP && ok; part++) {
+                        if (use) ok = bar_wait(&freeb[slot], (use - 1) & 1);
+                        if (!ok) return;
+                        sx_bar_expect_tx(&full[slot], kSlot);
+                        sx_bulk_load(smem + Smem::kRing + slot * kSlot,
+                                     tiles + (size_t)tile_of(i) * kTileBytes<T, DP> + (which * kP + part) * kSlot, kSlot, &full[slot]);
+                        issued++;
+                        if (++slot == kSlots) { slot = 0; use++; }
+                    }
+                };
+                if (n) load(0, 0);
+                for (uint32_t i = 0; i < n && ok; i++) {
+                    if (i + 1 < n) load(i + 1, 0);
+                    load(i, 1);
                 }
-            };
-            if (n) load(0, 0);
-            for (uint32_t i = 0; i < n && ok; i++) {
-                if (i + 1 < n) load(i + 1, 0);
-                load(i, 1);
+                // nothing may be in flight when the CTA's shared memory goes to another
+                for (uint32_t i = issued > kSlots ? issued - kSlots : 0; i < issued; i++) bar_wait(&full[i % kSlots], (i / kSlots) & 1);
             }
-            // nothing may be in flight when the CTA's shared memory goes to another
-            for (uint32_t i = issued > kSlots ? issued - kSlots : 0; i < issued; i++) sx_bar_wait(&full[i % kSlots], (i / kSlots) & 1);
-        }
-    } else if (warp == kSoftWarps) {
-        // ---- the MMAs
-        if (lane == 0) {
-            constexpr uint32_t kS = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
-            constexpr uint32_t kO = (1u << 4) | ((uint32_t)(DP >> 3) << 17) | ((kRows >> 4) << 24);
-            uint32_t slot = 0, use = 0;
-            bool ok = true;
-            const uint32_t q_at = sx_smem(smem), ring = sx_smem(smem + Smem::kRing);
-            uint32_t at[kP], sl[kP];
-            const auto take = [&]() {                           // the next operand's parts
-                for (int part = 0; part < kP && ok; part++) {
-                    ok = sx_bar_wait(&full[slot], use & 1);
-                    at[part] = ring + slot * kSlot;
-                    sl[part] = slot;
-                    if (++slot == kSlots) { slot = 0; use++; }
+        } else if (warp == kSoftWarps) {
+            // ---- the MMAs
+            if (lane == 0) {
+                constexpr uint32_t kS = (1u << 4) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
+                constexpr uint32_t kO = (1u << 4) | ((uint32_t)(DP >> 3) << 17) | ((kRows >> 4) << 24);
+                uint32_t slot = 0, use = 0;
+                bool ok = true;
+                const uint32_t q_at = sx_smem(smem), ring = sx_smem(smem + Smem::kRing);
+                uint32_t at[kP], sl[kP];
+                const auto take = [&]() {                           // the next operand's parts
+                    for (int part = 0; part < kP && ok; part++) {
+                        ok = bar_wait(&full[slot], use & 1);
+                        at[part] = ring + slot * kSlot;
+                        sl[part] = slot;
+                        if (++slot == kSlots) { slot = 0; use++; }
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                };
+                const auto scores = [&](uint32_t i) {
+                    take();
+                    if (!ok) return;
+                    const uint32_t d = tmem + (i & 1) * 256;
+                    const auto pass = [&](uint32_t q, uint32_t k, uint32_t first) {
+#pragma unroll
+                        for (int j = 0; j < DP / 16; j++)
+                            mma_ss(d, sx_desc(q + j * 2 * kLboRows, kLboRows, 128), sx_desc(k + j * 2 * kKeys * 16, kKeys * 16, 128), kS,
+                                   !(first && j == 0));
+                    };
+                    pass(q_at + Smem::kQ, at[0], 1);
+                    if (kP == 2) { pass(q_at, at[kP - 1], 0); sx_commit(&freeb[sl[kP - 1]]); }
+                    pass(q_at, at[0], 0);
+                    sx_commit(&freeb[sl[0]]);
+                    sx_commit(&s_ready[i & 1]);
+                };
+                const auto values = [&](uint32_t i) {
+                    take();
+                    ok = ok && bar_wait(&p_ready[i & 1], (i >> 1) & 1);
+                    if (!ok) return;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t w = tmem + (i & 1) * 256, d = w + 128;
+                    // 16 positions' weights: 8 columns of high parts, 8 of low ones
+                    const auto pass = [&](uint32_t lo, uint32_t v, uint32_t first) {
+#pragma unroll
+                        for (int j = 0; j < kKeys / 16; j++)
+                            sx_mma_ts(d, w + j * 16 + lo, sx_desc(v + j * 2 * kLboDims, kLboDims, 128), kO,
+                                      !(first && j == 0));
+                    };
+                    pass(8, at[0], 1);
+                    if (kP == 2) { pass(0, at[kP - 1], 0); sx_commit(&freeb[sl[kP - 1]]); }
+                    pass(0, at[0], 0);
+                    sx_commit(&freeb[sl[0]]);
+                    sx_commit(&d_ready[i & 1]);
+                };
+                if (n) scores(0);
+                for (uint32_t i = 0; i < n && ok; i++) {
+                    if (i + 1 < n) scores(i + 1);
+                    if (ok) values(i);
                 }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            };
-            const auto scores = [&](uint32_t i) {
-                take();
-                if (!ok) return;
-                const uint32_t d = tmem + (i & 1) * 256;
-                const auto pass = [&](uint32_t q, uint32_t k, uint32_t first) {
-#pragma unroll
-                    for (int j = 0; j < DP / 16; j++)
-                        mma_ss(d, sx_desc(q + j * 2 * kLboRows, kLboRows, 128), sx_desc(k + j * 2 * kKeys * 16, kKeys * 16, 128), kS,
-                               !(first && j == 0));
-                };
-                pass(q_at + Smem::kQ, at[0], 1);
-                if (kP == 2) { pass(q_at, at[kP - 1], 0); sx_commit(&freeb[sl[kP - 1]]); }
-                pass(q_at, at[0], 0);
-                sx_commit(&freeb[sl[0]]);
-                sx_commit(&s_ready[i & 1]);
-            };
-            const auto values = [&](uint32_t i) {
-                take();
-                ok = ok && sx_bar_wait(&p_ready[i & 1], (i >> 1) & 1);
-                if (!ok) return;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t w = tmem + (i & 1) * 256, d = w + 128;
-                // 32 positions' weights: 16 columns of high parts, 16 of low ones
-                const auto pass = [&](uint32_t lo, uint32_t v, uint32_t first) {
-#pragma unroll
-                    for (int j = 0; j < kKeys / 16; j++)
-                        sx_mma_ts(d, w + (j >> 1) * 32 + lo + (j & 1) * 8, sx_desc(v + j * 2 * kLboDims, kLboDims, 128), kO,
-                                  !(first && j == 0));
-                };
-                pass(16, at[0], 1);
-                if (kP == 2) { pass(0, at[kP - 1], 0); sx_commit(&freeb[sl[kP - 1]]); }
-                pass(0, at[0], 0);
-                sx_commit(&freeb[sl[0]]);
-                sx_commit(&d_ready[i & 1]);
-            };
-            if (n) scores(0);
-            for (uint32_t i = 0; i < n && ok; i++) {
-                if (i + 1 < n) scores(i + 1);
-                if (ok) values(i);
             }
         }
     } else {
         // ---- the softmax of every other tile; a thread has a row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        float m = -CUDART_INF_F, l = 0.f, o[DP];
+        uint32_t bad = 0;
         const int wg = warp >> 2;
         const uint32_t ts = tmem + wg * 256 + ((uint32_t)(warp & 3) << 21), td = ts + 128;
         const int64_t pos = (int64_t)p.base + (live ? token : tok0);
@@ -440,11 +449,12 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
                 for (int w = 0; w < 4; w++)
                     mask[w] &= bit_range(0, top - 32 * w) & (bit_range(low - 32 * w, 32) | bit_range(0, snk - 32 * w));
             }
-            ok = __all_sync(0xffffffffu, sx_bar_wait(&s_ready[wg], (i >> 1) & 1));
+            const auto word = [&](int w) { return w < 2 ? (w ? mask[1] : mask[0]) : (w == 2 ? mask[2] : mask[3]); };
+            ok = __all_sync(0xffffffffu, bar_wait(&s_ready[wg], (i >> 1) & 1));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float top = -CUDART_INF_F;
-#pragma unroll
+#pragma unroll 1
             for (int w = 0; w < 4; w++) {
                 uint32_t s[32];
                 tmem_ld32(ts + 32 * w, s);
@@ -454,7 +464,7 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e++)
-                        if ((mask[w] >> e) & 1) top = fmaxf(top, __uint_as_float(s[e]));
+                        if ((word(w) >> e) & 1) top = fmaxf(top, __uint_as_float(s[e]));
                 }
             }
             // (rounded up to a 64th: m1 - 14 is then exact, and so the weights of all tiles are relative to the same maxima)
@@ -462,30 +472,35 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
             const float a = m == m1 ? 1.f : ex2(m - (ms + kBias));
             m = m1;
             float sum = 0.f;
-#pragma unroll
+#pragma unroll 1
             for (int w = 0; w < 4; w++) {
-                uint32_t s[32], out[32];
+                uint32_t s[32];
+                const uint32_t bits = word(w);
                 tmem_ld32(ts + 32 * w, s);
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float x = __uint_as_float(s[e]), y = __uint_as_float(s[e + 1]);
-                    if (!whole) {
-                        if (!((mask[w] >> e) & 1)) x = -CUDART_INF_F;
-                        if (!((mask[w] >> (e + 1)) & 1)) y = -CUDART_INF_F;
+                for (int k = 0; k < 32; k += 16) {
+                    uint32_t out[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        float x = __uint_as_float(s[k + e]), y = __uint_as_float(s[k + e + 1]);
+                        if (!whole) {
+                            if (!((bits >> (k + e)) & 1)) x = -CUDART_INF_F;
+                            if (!((bits >> (k + e + 1)) & 1)) y = -CUDART_INF_F;
+                        }
+                        x = ex2(fmaf(x, c, -ms));
+                        y = ex2(fmaf(y, c, -ms));
+                        sum += x + y;
+                        split_f16x2(x, y, out[e / 2], out[8 + e / 2]);
                     }
-                    x = ex2(fmaf(x, c, -ms));
-                    y = ex2(fmaf(y, c, -ms));
-                    sum += x + y;
-                    split_f16x2(x, y, out[e / 2], out[16 + e / 2]);
+                    sx_tmem_st16(ts + 32 * w + k, out);
                 }
-                tmem_st32(ts + 32 * w, out);
             }
             l = fmaf(l, a, sum);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) sx_bar_arrive(&p_ready[wg]);
-            ok = __all_sync(0xffffffffu, sx_bar_wait(&d_ready[wg], (i >> 1) & 1));
+            ok = __all_sync(0xffffffffu, bar_wait(&d_ready[wg], (i >> 1) & 1));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -498,50 +513,49 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
-    }
-    // ---- both groups' parts of a row: each hands the other half of its dimensions through shared memory
-    __syncthreads();
-    float *swap = reinterpret_cast<float *>(smem), *ml = swap + kRows * DP;     // [group][DP / 2][row]; [group][m, l, bad][row]
-    const int wg = warp >> 2;
-    if (warp < kSoftWarps) {
+        // ---- both groups' parts of a row: each hands the other half of its dimensions through shared memory
+        asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
+        float *swap = reinterpret_cast<float *>(smem), *ml = swap + kRows * DP;     // [group][DP / 2][row]; [group][m, l, bad][row]
+        {
 #pragma unroll
-        for (int i = 0; i < DP / 2; i++) swap[(wg * (DP / 2) + i) * kRows + r] = wg ? o[i] : o[DP / 2 + i];
-        ml[(wg * 3) * kRows + r] = m;
-        ml[(wg * 3 + 1) * kRows + r] = l;
-        ml[(wg * 3 + 2) * kRows + r] = __uint_as_float(bad);
-    }
-    __syncthreads();
-    if (warp < kSoftWarps && live) {
-        const float m2 = ml[((wg ^ 1) * 3) * kRows + r], l2 = ml[((wg ^ 1) * 3 + 1) * kRows + r], M = fmaxf(m, m2);
-        bad |= __float_as_uint(ml[((wg ^ 1) * 3 + 2) * kRows + r]);
-        const float f1 = m == -CUDART_INF_F ? 0.f : ex2(m - M), f2 = m2 == -CUDART_INF_F ? 0.f : ex2(m2 - M);
-        // (in the order of the groups, so that both halves divide by the same sum)
-        const float sum = wg ? fmaf(l2, f2, l * f1) : fmaf(l, f1, l2 * f2);
-        float *out = p.out + ((uint64_t)token * p.q_heads + head) * D + wg * (DP / 2);
-#pragma unroll
-        for (int i = 0; i < DP / 2; i += 4) {
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                x[e] = fmaf(swap[((wg ^ 1) * (DP / 2) + i + e) * kRows + r], f2, (wg ? o[DP / 2 + i + e] : o[i + e]) * f1) / sum;
-            if ((uint32_t)(wg * (DP / 2) + i) < D) *reinterpret_cast<float4 *>(out + i) = make_float4(x[0], x[1], x[2], x[3]);
+            for (int i = 0; i < DP / 2; i++) swap[(wg * (DP / 2) + i) * kRows + r] = wg ? o[i] : o[DP / 2 + i];
+            ml[(wg * 3) * kRows + r] = m;
+            ml[(wg * 3 + 1) * kRows + r] = l;
+            ml[(wg * 3 + 2) * kRows + r] = __uint_as_float(bad);
         }
-        if (bad) {
-            // values that are not finite were left out of the tiles: a row that sees one gets it added
-            const int64_t pos = (int64_t)p.base + token;
-            const uint64_t end = min((uint64_t)min(p.lengths[0], p.reach), (uint64_t)pos + 1);
-            for (uint32_t i = 0; i < n; i++) {
-                const uint32_t tile = tile_of(i);
-                if (!heads[tile].bad) continue;
-                for (uint32_t x = 0; x < (uint32_t)kKeys; x++) {
-                    const uint64_t j = (uint64_t)win_tile_start(keys, tile) + x;
-                    if (!((heads[tile].seen[x >> 5] >> (x & 31)) & 1) || j >= end || (pos - (int64_t)j >= (int64_t)p.window && j >= p.sinks))
-                        continue;
-                    const T *v = static_cast<const T *>(p.v) +
-                                 ((uint64_t)win_cache_row(p, p.pages, (uint32_t)j) * p.kv_heads + kvh0 + kv) * D + wg * (DP / 2);
-                    for (uint32_t d = 0; d < DP / 2 && wg * (DP / 2) + d < D; d++) {
-                        const float y = to_f32(v[d]);
-                        if (!(fabsf(y) <= 3.402823466e38f)) out[d] += y;
+        asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
+        if (live) {
+            const float m2 = ml[((wg ^ 1) * 3) * kRows + r], l2 = ml[((wg ^ 1) * 3 + 1) * kRows + r], M = fmaxf(m, m2);
+            bad |= __float_as_uint(ml[((wg ^ 1) * 3 + 2) * kRows + r]);
+            const float f1 = m == -CUDART_INF_F ? 0.f : ex2(m - M), f2 = m2 == -CUDART_INF_F ? 0.f : ex2(m2 - M);
+            // (in the order of the groups, so that both halves divide by the same sum)
+            const float sum = wg ? fmaf(l2, f2, l * f1) : fmaf(l, f1, l2 * f2);
+            float *out = p.out + ((uint64_t)token * p.q_heads + head) * D + wg * (DP / 2);
+#pragma unroll
+            for (int i = 0; i < DP / 2; i += 4) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    x[e] = fmaf(swap[((wg ^ 1) * (DP / 2) + i + e) * kRows + r], f2, (wg ? o[DP / 2 + i + e] : o[i + e]) * f1) / sum;
+                if ((uint32_t)(wg * (DP / 2) + i) < D) *reinterpret_cast<float4 *>(out + i) = make_float4(x[0], x[1], x[2], x[3]);
+            }
+            if (bad) {
+                // values that are not finite were left out of the tiles: a row that sees one gets it added
+                const int64_t pos = (int64_t)p.base + token;
+                const uint64_t end = min((uint64_t)min(p.lengths[0], p.reach), (uint64_t)pos + 1);
+                for (uint32_t i = 0; i < n; i++) {
+                    const uint32_t tile = tile_of(i);
+                    if (!heads[tile].bad) continue;
+                    for (uint32_t x = 0; x < (uint32_t)kKeys; x++) {
+                        const uint64_t j = (uint64_t)win_tile_start(keys, tile) + x;
+                        if (!((heads[tile].seen[x >> 5] >> (x & 31)) & 1) || j >= end || (pos - (int64_t)j >= (int64_t)p.window && j >= p.sinks))
+                            continue;
+                        const T *v = static_cast<const T *>(p.v) +
+                                     ((uint64_t)win_cache_row(p, p.pages, (uint32_t)j) * p.kv_heads + kvh0 + kv) * D + wg * (DP / 2);
+                        for (uint32_t d = 0; d < DP / 2 && wg * (DP / 2) + d < D; d++) {
+                            const float y = to_f32(v[d]);
+                            if (!(fabsf(y) <= 3.402823466e38f)) out[d] += y;
+                        }
                     }
                 }
             }
