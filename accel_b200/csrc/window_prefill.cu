@@ -247,6 +247,13 @@ __device__ __forceinline__ uint32_t bit_range(int a, int b)
     return a < b ? (0xffffffffu >> (32 - (b - a))) << a : 0u;
 }
 
+// scores whose bit is not set become -inf
+__device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t bits)
+{
+#pragma unroll
+    for (int e = 0; e < 32; e++) s[e] = (bits >> e) & 1 ? s[e] : 0xff800000u;
+}
+
 // The tiles that the rows at positions [pa, pb] see: [0, sinks_end) and [begin, end).
 struct Range { uint32_t sinks_end, begin, end; };
 __device__ __forceinline__ Range win_range(const WinParams &p, const Keys &k, uint64_t pa, uint64_t pb)
@@ -430,13 +437,19 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
         bool ok = true;
 #pragma unroll
         for (int i = 0; i < DP; i++) o[i] = 0.f;
+        uint4 next_scale = make_uint4(0, 0, 0, 0), next_seen = next_scale;
+        const auto look = [&](uint32_t i) {                         // a tile's header, a tile ahead of its use
+            const uint4 *h = reinterpret_cast<const uint4 *>(heads + tile_of(i));
+            next_scale = __ldg(h);
+            next_seen = __ldg(h + 1);
+        };
+        if ((uint32_t)wg < n) look(wg);
         for (uint32_t i = wg; i < n; i += 2) {
-            const uint32_t tile = tile_of(i);
-            const int64_t j0 = win_tile_start(keys, tile);
-            const TileHead &h = heads[tile];
-            const float c = fmaxf(q_scale * __ldg(&h.k_scale), 1.2e-38f), vs = __ldg(&h.v_scale);
-            bad |= __ldg(&h.bad);
-            const uint4 seen = __ldg(reinterpret_cast<const uint4 *>(h.seen));
+            const int64_t j0 = win_tile_start(keys, tile_of(i));
+            const float c = fmaxf(q_scale * __uint_as_float(next_scale.x), 1.2e-38f), vs = __uint_as_float(next_scale.y);
+            bad |= next_scale.z;
+            const uint4 seen = next_seen;
+            if (i + 2 < n) look(i + 2);
             // does every row of the CTA see the whole tile?
             const bool whole = (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && j0 + kKeys - 1 <= (int64_t)pa &&
                                j0 + (int64_t)p.window > (int64_t)(pa + tokens - 1);
@@ -458,44 +471,38 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
             for (int w = 0; w < 4; w++) {
                 uint32_t s[32];
                 tmem_ld32(ts + 32 * w, s);
-                if (whole) {
+                if (!whole) hide(s, word(w));
+                float x[4];
 #pragma unroll
-                    for (int e = 0; e < 32; e++) top = fmaxf(top, __uint_as_float(s[e]));
-                } else {
+                for (int e = 0; e < 4; e++) x[e] = __uint_as_float(s[e]);
 #pragma unroll
-                    for (int e = 0; e < 32; e++)
-                        if ((word(w) >> e) & 1) top = fmaxf(top, __uint_as_float(s[e]));
-                }
+                for (int e = 4; e < 32; e++) x[e & 3] = fmaxf(x[e & 3], __uint_as_float(s[e]));
+                top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
             }
             // (rounded up to a 64th: m1 - 14 is then exact, and so the weights of all tiles are relative to the same maxima)
             const float m1 = fmaxf(m, ceilf(top * c * 64.f) * 0.015625f), ms = (m1 == -CUDART_INF_F ? 0.f : m1) - kBias;
             const float a = m == m1 ? 1.f : ex2(m - (ms + kBias));
             m = m1;
-            float sum = 0.f;
+            float sum[2] = {0.f, 0.f};
 #pragma unroll 1
             for (int w = 0; w < 4; w++) {
                 uint32_t s[32];
-                const uint32_t bits = word(w);
                 tmem_ld32(ts + 32 * w, s);
+                if (!whole) hide(s, word(w));
 #pragma unroll
                 for (int k = 0; k < 32; k += 16) {
                     uint32_t out[16];
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        float x = __uint_as_float(s[k + e]), y = __uint_as_float(s[k + e + 1]);
-                        if (!whole) {
-                            if (!((bits >> (k + e)) & 1)) x = -CUDART_INF_F;
-                            if (!((bits >> (k + e + 1)) & 1)) y = -CUDART_INF_F;
-                        }
-                        x = ex2(fmaf(x, c, -ms));
-                        y = ex2(fmaf(y, c, -ms));
-                        sum += x + y;
+                        const float x = ex2(fmaf(__uint_as_float(s[k + e]), c, -ms)), y = ex2(fmaf(__uint_as_float(s[k + e + 1]), c, -ms));
+                        sum[0] += x;
+                        sum[1] += y;
                         split_f16x2(x, y, out[e / 2], out[8 + e / 2]);
                     }
                     sx_tmem_st16(ts + 32 * w + k, out);
                 }
             }
-            l = fmaf(l, a, sum);
+            l = fmaf(l, a, sum[0] + sum[1]);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
