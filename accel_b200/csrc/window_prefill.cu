@@ -239,6 +239,32 @@ __device__ __forceinline__ float ex2(float x)
     asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two f32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 // bits [a, b) of a word, a and b clipped to it
 __device__ __forceinline__ uint32_t bit_range(int a, int b)
 {
@@ -305,30 +331,36 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
     const bool live = r < tokens * group;
     float q_scale = 1.f;
     if (warp < kSoftWarps) {
+        // both halves of a row find its largest element together, each with its own in registers
         const float *q = p.q + ((uint64_t)(live ? token : 0) * p.q_heads + (live ? head : 0)) * D;
-        float amax = 0.f;
-        for (uint32_t d = 0; d < D; d += 4) {
-            const float4 v = live ? __ldg(reinterpret_cast<const float4 *>(q + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        const uint32_t d0 = (tid >> 7) * (DP / 2);
+        float x[DP / 2], amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < DP / 2; i += 4) {
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (live && d0 + i < D) v = __ldg(reinterpret_cast<const float4 *>(q + d0 + i));
+            x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
         }
+#pragma unroll
+        for (int i = 0; i < DP / 2; i++) amax = fmaxf(amax, fabsf(x[i]));
+        float *both = reinterpret_cast<float *>(smem + Smem::kRing);
+        both[tid] = amax;
+        asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
+        amax = fmaxf(amax, both[tid ^ kRows]);
         amax = fminf(amax * fabsf(p.scale_log2), 3.402823466e38f);
         // near one: the products with keys of up to 2^14 (or f16's largest) stay far inside f32
-        const int e = min(fit_exponent(amax) - 13, 126);
-        const float f = ab_pow2(max(e, -126));
-        q_scale = ab_pow2(-max(e, -126));
-        for (uint32_t d = (tid >> 7) * (DP / 2); d < ((uint32_t)(tid >> 7) + 1) * (DP / 2); d += 8) {
-            float x[8];
+        const int e = max(fit_exponent(amax) - 13, -126);
+        const float f = ab_pow2(e);
+        q_scale = ab_pow2(-e);
 #pragma unroll
-            for (int i = 0; i < 8; i += 4) {
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (live && d + i < D) v = __ldg(reinterpret_cast<const float4 *>(q + d + i));
-                x[i] = v.x * p.scale_log2 * f; x[i + 1] = v.y * p.scale_log2 * f;
-                x[i + 2] = v.z * p.scale_log2 * f; x[i + 3] = v.w * p.scale_log2 * f;
-            }
+        for (int i = 0; i < DP / 2; i += 8) {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) y[k] = x[i + k] * p.scale_log2 * f;
             uint4 hi, lo;
-            split8(x, hi, lo);
-            *reinterpret_cast<uint4 *>(smem + d / 8 * kLboRows + r * 16) = hi;
-            *reinterpret_cast<uint4 *>(smem + Smem::kQ + d / 8 * kLboRows + r * 16) = lo;
+            split8(y, hi, lo);
+            *reinterpret_cast<uint4 *>(smem + (d0 + i) / 8 * kLboRows + r * 16) = hi;
+            *reinterpret_cast<uint4 *>(smem + Smem::kQ + (d0 + i) / 8 * kLboRows + r * 16) = lo;
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -483,7 +515,8 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
             const float m1 = fmaxf(m, ceilf(top * c * 64.f) * 0.015625f), ms = (m1 == -CUDART_INF_F ? 0.f : m1) - kBias;
             const float a = m == m1 ? 1.f : ex2(m - (ms + kBias));
             m = m1;
-            float sum[2] = {0.f, 0.f};
+            float2 sum = make_float2(0.f, 0.f);
+            const float2 c2 = make_float2(c, c), ms2 = make_float2(-ms, -ms);
 #pragma unroll 1
             for (int w = 0; w < 4; w++) {
                 uint32_t s[32];
@@ -494,15 +527,18 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
                     uint32_t out[16];
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float x = ex2(fmaf(__uint_as_float(s[k + e]), c, -ms)), y = ex2(fmaf(__uint_as_float(s[k + e + 1]), c, -ms));
-                        sum[0] += x;
-                        sum[1] += y;
-                        split_f16x2(x, y, out[e / 2], out[8 + e / 2]);
+                        const float2 z = fma2(make_float2(__uint_as_float(s[k + e]), __uint_as_float(s[k + e + 1])), c2, ms2);
+                        const float2 x = make_float2(ex2(z.x), ex2(z.y));
+                        sum = add2(sum, x);
+                        // the high part is cut off (11 bits), what is left of it rounded
+                        const float2 h = make_float2(cut(x.x), cut(x.y)), d = add2(x, make_float2(-h.x, -h.y));
+                        out[e / 2] = pack_f16x2(h.x, h.y);
+                        out[8 + e / 2] = pack_f16x2(d.x, d.y);
                     }
                     sx_tmem_st16(ts + 32 * w + k, out);
                 }
             }
-            l = fmaf(l, a, sum[0] + sum[1]);
+            l = fmaf(l, a, sum.x + sum.y);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -515,8 +551,13 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
                 uint32_t d[32];
                 tmem_ld32(td + 32 * w, d);
 #pragma unroll
-                for (int e = 0; e < 32; e++)
-                    o[32 * w + e] = fmaf(o[32 * w + e], a, sizeof(T) == 4 ? __uint_as_float(d[e]) * vs : __uint_as_float(d[e]));
+                for (int e = 0; e < 32; e += 2) {
+                    float2 x = make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1]));
+                    if (sizeof(T) == 4) x = mul2(x, make_float2(vs, vs));
+                    x = fma2(make_float2(o[32 * w + e], o[32 * w + e + 1]), make_float2(a, a), x);
+                    o[32 * w + e] = x.x;
+                    o[32 * w + e + 1] = x.y;
+                }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
