@@ -198,7 +198,8 @@ template <typename T, int DP> struct TileSmem {
     static constexpr uint32_t kQ = kRows * DP * 2;                  // one part of the query rows
     static constexpr uint32_t kRing = 2 * kQ;
     static constexpr uint32_t kBars = kRing + kSlots * kSlotBytes<T, DP>;
-    static constexpr uint32_t kBytes = kBars + 256;
+    static constexpr uint32_t kScale = kBars + 256;                 // a power of two per query row
+    static constexpr uint32_t kBytes = kScale + kRows * 4;
 };
 
 // sx_bar_wait without its function call: the softmax threads hold more registers than survive one
@@ -325,42 +326,42 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
         for (int i = 0; i < 2; i++) { sx_bar_init(&s_ready[i], 1); sx_bar_init(&p_ready[i], 4); sx_bar_init(&d_ready[i], 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // the query rows, a thread half a row: scaled, split, stored as the A operand
+    // The query rows, scaled, split, stored as the A operand.  A warp takes 16 rows, eight at a time, four lanes to a row:
+    // 64 bytes of each of eight rows a load, and stores that meet every bank twice
     const uint32_t r = tid & (kRows - 1), token = tok0 + r / group;
-    const uint32_t head = (kvh0 + kv) * group + r % group;
     const bool live = r < tokens * group;
-    float q_scale = 1.f;
+    float *row_scale = reinterpret_cast<float *>(smem + Smem::kScale);
     if (warp < kSoftWarps) {
-        // both halves of a row find its largest element together, each with its own in registers
-        const float *q = p.q + ((uint64_t)(live ? token : 0) * p.q_heads + (live ? head : 0)) * D;
-        const uint32_t d0 = (tid >> 7) * (DP / 2);
-        float x[DP / 2], amax = 0.f;
+        const uint32_t at = (lane & 3) * 4;
 #pragma unroll
-        for (int i = 0; i < DP / 2; i += 4) {
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (live && d0 + i < D) v = __ldg(reinterpret_cast<const float4 *>(q + d0 + i));
-            x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
-        }
+        for (int g = 0; g < 2; g++) {
+            const uint32_t row = warp * 16 + g * 8 + (lane >> 2);
+            const bool on = row < tokens * group;
+            const float *q = p.q + ((uint64_t)(tok0 + (on ? row / group : 0)) * p.q_heads + (kvh0 + kv) * group + (on ? row % group : 0)) * D;
+            float4 x[DP / 16];
+            float amax = 0.f;
 #pragma unroll
-        for (int i = 0; i < DP / 2; i++) amax = fmaxf(amax, fabsf(x[i]));
-        float *both = reinterpret_cast<float *>(smem + Smem::kRing);
-        both[tid] = amax;
-        asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
-        amax = fmaxf(amax, both[tid ^ kRows]);
-        amax = fminf(amax * fabsf(p.scale_log2), 3.402823466e38f);
-        // near one: the products with keys of up to 2^14 (or f16's largest) stay far inside f32
-        const int e = max(fit_exponent(amax) - 13, -126);
-        const float f = ab_pow2(e);
-        q_scale = ab_pow2(-e);
+            for (int i = 0; i < DP / 16; i++)
+                x[i] = on && 16 * i + at < D ? __ldg(reinterpret_cast<const float4 *>(q + 16 * i + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < DP / 2; i += 8) {
-            float y[8];
+            for (int i = 0; i < DP / 16; i++)
+                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            amax = fminf(amax * fabsf(p.scale_log2), 3.402823466e38f);
+            // near one: the products with keys of up to 2^14 (or f16's largest) stay far inside f32
+            const int e = max(fit_exponent(amax) - 13, -126);
+            const float f = ab_pow2(e);
+            if ((lane & 3) == 0) row_scale[row] = ab_pow2(-e);
 #pragma unroll
-            for (int k = 0; k < 8; k++) y[k] = x[i + k] * p.scale_log2 * f;
-            uint4 hi, lo;
-            split8(y, hi, lo);
-            *reinterpret_cast<uint4 *>(smem + (d0 + i) / 8 * kLboRows + r * 16) = hi;
-            *reinterpret_cast<uint4 *>(smem + Smem::kQ + (d0 + i) / 8 * kLboRows + r * 16) = lo;
+            for (int i = 0; i < DP / 16; i++) {
+                uint2 hi, lo;
+                split_f16x2(x[i].x * p.scale_log2 * f, x[i].y * p.scale_log2 * f, hi.x, lo.x);
+                split_f16x2(x[i].z * p.scale_log2 * f, x[i].w * p.scale_log2 * f, hi.y, lo.y);
+                unsigned char *to = smem + (16 * i + at) / 8 * kLboRows + row * 16 + (at & 4) * 2;
+                *reinterpret_cast<uint2 *>(to) = hi;
+                *reinterpret_cast<uint2 *>(to + Smem::kQ) = lo;
+            }
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -460,6 +461,7 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
     } else {
         // ---- the softmax of every other tile; a thread has a row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const float q_scale = row_scale[r];
         float m = -CUDART_INF_F, l = 0.f, o[DP];
         uint32_t bad = 0;
         const int wg = warp >> 2;
@@ -471,9 +473,11 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
         for (int i = 0; i < DP; i++) o[i] = 0.f;
         uint4 next_scale = make_uint4(0, 0, 0, 0), next_seen = next_scale;
         const auto look = [&](uint32_t i) {                         // a tile's header, a tile ahead of its use
-            const uint4 *h = reinterpret_cast<const uint4 *>(heads + tile_of(i));
-            next_scale = __ldg(h);
-            next_seen = __ldg(h + 1);
+            const TileHead *h = heads + tile_of(i);
+            asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(next_scale.x), "=r"(next_scale.y), "=r"(next_scale.z), "=r"(next_scale.w) : "l"(h));
+            asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4 + 16];"
+                         : "=r"(next_seen.x), "=r"(next_seen.y), "=r"(next_seen.z), "=r"(next_seen.w) : "l"(h));
         };
         if ((uint32_t)wg < n) look(wg);
         for (uint32_t i = wg; i < n; i += 2) {
@@ -561,52 +565,60 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
-        // ---- both groups' parts of a row: each hands the other half of its dimensions through shared memory
+        // ---- both groups' parts of a row: each gives away half of its dimensions through shared memory, finishes the other
+        // half there, and whole rows go out (row stride DP + 4: 16 bytes of eight neighbouring rows meet every bank once)
+        constexpr uint32_t kPitch = DP + 4;
+        float *rows = reinterpret_cast<float *>(smem), *mine = rows + r * kPitch + wg * (DP / 2);
+        float *give = rows + r * kPitch + (wg ^ 1) * (DP / 2), *ml = rows + kRows * kPitch + r;      // [group][m, l, bad][row]
         asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
-        float *swap = reinterpret_cast<float *>(smem), *ml = swap + kRows * DP;     // [group][DP / 2][row]; [group][m, l, bad][row]
-        {
 #pragma unroll
-            for (int i = 0; i < DP / 2; i++) swap[(wg * (DP / 2) + i) * kRows + r] = wg ? o[i] : o[DP / 2 + i];
-            ml[(wg * 3) * kRows + r] = m;
-            ml[(wg * 3 + 1) * kRows + r] = l;
-            ml[(wg * 3 + 2) * kRows + r] = __uint_as_float(bad);
+        for (int i = 0; i < DP / 2; i += 4)
+            *reinterpret_cast<float4 *>(give + i) = wg ? make_float4(o[i], o[i + 1], o[i + 2], o[i + 3])
+                                                       : make_float4(o[DP / 2 + i], o[DP / 2 + i + 1], o[DP / 2 + i + 2], o[DP / 2 + i + 3]);
+        ml[wg * 3 * kRows] = m;
+        ml[(wg * 3 + 1) * kRows] = l;
+        ml[(wg * 3 + 2) * kRows] = __uint_as_float(bad);
+        asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
+        const float m0 = ml[0], m1 = ml[3 * kRows], M = fmaxf(m0, m1);
+        const float f0 = m0 == -CUDART_INF_F ? 0.f : ex2(m0 - M), f1 = m1 == -CUDART_INF_F ? 0.f : ex2(m1 - M);
+        const float sum = fmaf(ml[kRows], f0, ml[4 * kRows] * f1), fm = (wg ? f1 : f0) / sum, fo = (wg ? f0 : f1) / sum;
+#pragma unroll
+        for (int i = 0; i < DP / 2; i += 4) {
+            float4 x = *reinterpret_cast<float4 *>(mine + i);
+            x.x = fmaf(x.x, fo, (wg ? o[DP / 2 + i] : o[i]) * fm);
+            x.y = fmaf(x.y, fo, (wg ? o[DP / 2 + i + 1] : o[i + 1]) * fm);
+            x.z = fmaf(x.z, fo, (wg ? o[DP / 2 + i + 2] : o[i + 2]) * fm);
+            x.w = fmaf(x.w, fo, (wg ? o[DP / 2 + i + 3] : o[i + 3]) * fm);
+            *reinterpret_cast<float4 *>(mine + i) = x;
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
-        if (live) {
-            const float m2 = ml[((wg ^ 1) * 3) * kRows + r], l2 = ml[((wg ^ 1) * 3 + 1) * kRows + r], M = fmaxf(m, m2);
-            bad |= __float_as_uint(ml[((wg ^ 1) * 3 + 2) * kRows + r]);
-            const float f1 = m == -CUDART_INF_F ? 0.f : ex2(m - M), f2 = m2 == -CUDART_INF_F ? 0.f : ex2(m2 - M);
-            // (in the order of the groups, so that both halves divide by the same sum)
-            const float sum = wg ? fmaf(l2, f2, l * f1) : fmaf(l, f1, l2 * f2);
-            float *out = p.out + ((uint64_t)token * p.q_heads + head) * D + wg * (DP / 2);
-#pragma unroll
-            for (int i = 0; i < DP / 2; i += 4) {
-                float x[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    x[e] = fmaf(swap[((wg ^ 1) * (DP / 2) + i + e) * kRows + r], f2, (wg ? o[DP / 2 + i + e] : o[i + e]) * f1) / sum;
-                if ((uint32_t)(wg * (DP / 2) + i) < D) *reinterpret_cast<float4 *>(out + i) = make_float4(x[0], x[1], x[2], x[3]);
-            }
-            if (bad) {
-                // values that are not finite were left out of the tiles: a row that sees one gets it added
-                const int64_t pos = (int64_t)p.base + token;
-                const uint64_t end = min((uint64_t)min(p.lengths[0], p.reach), (uint64_t)pos + 1);
-                for (uint32_t i = 0; i < n; i++) {
-                    const uint32_t tile = tile_of(i);
-                    if (!heads[tile].bad) continue;
-                    for (uint32_t x = 0; x < (uint32_t)kKeys; x++) {
-                        const uint64_t j = (uint64_t)win_tile_start(keys, tile) + x;
-                        if (!((heads[tile].seen[x >> 5] >> (x & 31)) & 1) || j >= end || (pos - (int64_t)j >= (int64_t)p.window && j >= p.sinks))
-                            continue;
-                        const T *v = static_cast<const T *>(p.v) +
-                                     ((uint64_t)win_cache_row(p, p.pages, (uint32_t)j) * p.kv_heads + kvh0 + kv) * D + wg * (DP / 2);
-                        for (uint32_t d = 0; d < DP / 2 && wg * (DP / 2) + d < D; d++) {
-                            const float y = to_f32(v[d]);
-                            if (!(fabsf(y) <= 3.402823466e38f)) out[d] += y;
-                        }
+        if (live && (__float_as_uint(ml[2 * kRows]) | __float_as_uint(ml[5 * kRows]))) {
+            // values that are not finite were left out of the tiles: a row that sees one gets it added
+            const uint64_t end = min((uint64_t)min(p.lengths[0], p.reach), (uint64_t)pos + 1);
+            for (uint32_t i = 0; i < n; i++) {
+                const uint32_t tile = tile_of(i);
+                if (!heads[tile].bad) continue;
+                for (uint32_t x = 0; x < (uint32_t)kKeys; x++) {
+                    const uint64_t j = (uint64_t)win_tile_start(keys, tile) + x;
+                    if (!((heads[tile].seen[x >> 5] >> (x & 31)) & 1) || j >= end || (pos - (int64_t)j >= (int64_t)p.window && j >= p.sinks))
+                        continue;
+                    const T *v = static_cast<const T *>(p.v) +
+                                 ((uint64_t)win_cache_row(p, p.pages, (uint32_t)j) * p.kv_heads + kvh0 + kv) * D + wg * (DP / 2);
+                    for (uint32_t d = 0; d < DP / 2 && wg * (DP / 2) + d < D; d++) {
+                        const float y = to_f32(v[d]);
+                        if (!(fabsf(y) <= 3.402823466e38f)) mine[d] += y;
                     }
                 }
             }
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
+        // a warp writes a row (two, of a head of 64) at a time
+        constexpr int kLanes = DP / 4, kTogether = 32 / kLanes;
+#pragma unroll 4
+        for (int i = 0; i < kRows / kSoftWarps; i += kTogether) {
+            const uint32_t row = warp * (kRows / kSoftWarps) + i + lane / kLanes, d = lane % kLanes * 4;
+            if (row < tokens * group && d < D)
+                *reinterpret_cast<float4 *>(p.out + ((uint64_t)(tok0 + row / group) * p.q_heads + (kvh0 + kv) * group + row % group) * D + d) =
+                    *reinterpret_cast<const float4 *>(rows + row * kPitch + d);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -633,7 +645,7 @@ constexpr uint64_t kPassBytes = 1ull << 30;              // tiles of one pass ov
 template <typename T, int DP> int run_tiles(Launch &l, const WinParams &p, const char *name)
 {
     static_assert(TileSmem<T, DP>::kBytes <= 232448, "shared memory of a CTA");
-    static_assert(kRows * DP * 4 + 6 * kRows * 4 <= TileSmem<T, DP>::kBars, "the parts of both groups fit where the operands were");
+    static_assert(kRows * (DP + 4) * 4 + 6 * kRows * 4 <= TileSmem<T, DP>::kBars, "the parts of both groups fit where the operands were");
     const Keys keys = win_keys(p);
     const uint64_t per_head = (uint64_t)keys.tiles * kTileBytes<T, DP>;
     const uint32_t pass = (uint32_t)std::min<uint64_t>(p.kv_heads, std::max<uint64_t>(1, kPassBytes / per_head));
