@@ -89,7 +89,7 @@ template <> struct Piece<__half> {
 };
 
 struct Sums { float m, s, u; };
-__device__ __forceinline__ float lp_exp(float d) { float e; asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(d * kLog2e)); return e; }
+__device__ __forceinline__ float lp_exp(float d) { float e; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * kLog2e)); return e; }
 // below -1e4 e^d is 0, and (-inf) * 0 would be a NaN
 __device__ __forceinline__ float lp_clamp(float d) { return fmaxf(d, -1e4f); }
 // moves the sums to a maximum M >= m
@@ -140,7 +140,7 @@ __device__ __forceinline__ void lp_cluster_sync()
 
 // A cluster of `parts` CTAs per row, a contiguous run of the row's pieces each; the first also takes the few elements
 // before the first and behind the last whole piece.
-template <typename T> __global__ void __launch_bounds__(kThreads, 6) logprobs_kernel(const LpParams p, const uint32_t parts)
+template <typename T> __global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const LpParams p, const uint32_t parts)
 {
     constexpr int N = Piece<T>::kN, U = 16 / N;
     __shared__ Sums sums[kWarps];
