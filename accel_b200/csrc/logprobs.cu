@@ -15,11 +15,11 @@
 // once per 16 elements, and threads, warps and CTAs are joined by the same rule in a fixed order.  One
 // exponential and seven instructions per element: HBM bounds it.
 //
-// The alternatives cost no second pass.  A warp's `each`-th largest thread maximum is reached by `each` of
-// its elements; with `each` = ceil(Top / warps) at least Top elements reach the smallest of these over
-// the warps, the floor.  Only threads whose maximum reaches it can hold an alternative (some tens); their
-// pieces are read again (L2), what reaches the floor is listed, and an element's place among the
-// alternatives is the number of listed ones before it.
+// The alternatives cost no second pass.  With `each` = ceil(Top / warps) + 2 the warps' `each` largest thread maxima
+// are at least Top numbers, every one reached by an element of its own, so at least Top elements reach
+// the Top-th largest of them, the floor.  Only threads whose maximum reaches it can hold an alternative (about
+// Top of 256); their pieces are read again (L2, all at once), what reaches the floor is listed, and an
+// element's place among the alternatives is the number of listed ones before it.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -140,12 +140,13 @@ __device__ __forceinline__ void lp_cluster_sync()
 
 // A cluster of `parts` CTAs per row, a contiguous run of the row's pieces each; the first also takes the few elements
 // before the first and behind the last whole piece.
-template <typename T> __global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(const LpParams p, const uint32_t parts)
+template <typename T> __global__ void __launch_bounds__(kThreads, 6) logprobs_kernel(const LpParams p, const uint32_t parts)
 {
     constexpr int N = Piece<T>::kN, U = 16 / N;
     __shared__ Sums sums[kWarps];
     __shared__ Sums whole;
-    __shared__ uint32_t floors[kWarps], n_list;
+    __shared__ uint32_t maxima[kWarps * (kMaxTop / kWarps + 2)], at_floor, n_list, n_held;
+    __shared__ uint8_t held[kThreads];
     __shared__ u64 list[kList], best[kMaxTop], all[16 * kMaxTop], slow[kWarps];
     const uint32_t row = blockIdx.x / parts, part = blockIdx.x % parts, V = p.vocab, t = threadIdx.x;
     const int warp = t >> 5, lane = t & 31;
@@ -203,15 +204,14 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 8) logprobs_ke
     }
     if (lane == 0) sums[warp] = a;
     if (p.top) {
-        const uint32_t each = (p.top + kWarps - 1) / kWarps;
-        uint32_t k = key, f = 0;
+        const uint32_t each = (p.top + kWarps - 1) / kWarps + 2;
+        uint32_t k = key;
         for (uint32_t r = 0; r < each; r++) {
-            f = __reduce_max_sync(0xffffffffu, k);
-            const uint32_t at = __ballot_sync(0xffffffffu, k == f);
+            const uint32_t f = __reduce_max_sync(0xffffffffu, k), at = __ballot_sync(0xffffffffu, k == f);
             if (lane == __ffs(at) - 1) k = 0;
+            if (lane == 0) maxima[warp * each + r] = f;
         }
-        if (lane == 0) floors[warp] = f;
-        if (t == 0) n_list = 0;
+        if (t == 0) { n_list = 0; n_held = 0; }
     }
     __syncthreads();
     if (t == 0) {
@@ -222,9 +222,25 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 8) logprobs_ke
 
     // ---- the CTA's Top largest elements, in order, into best[] (0: it has fewer)
     if (p.top) {
-        uint32_t floor = floors[0];
-#pragma unroll
-        for (int i = 1; i < kWarps; i++) floor = min(floor, floors[i]);
+        const uint32_t n_max = kWarps * ((p.top + kWarps - 1) / kWarps + 2);
+        if (t < n_max) {
+            const uint32_t mine = maxima[t];
+            uint32_t before = 0;
+            for (uint32_t j = 0; j < n_max; j++) before += maxima[j] > mine || (maxima[j] == mine && j < t);
+            if (before == p.top - 1) at_floor = mine;
+        }
+        __syncthreads();
+        const uint32_t floor = at_floor;
+        {
+            // the threads to look at (a floor of 0: fewer than Top threads have elements at all)
+            const uint32_t b = __ballot_sync(0xffffffffu, key >= floor && key != 0);
+            uint32_t at = 0;
+            if (lane == 0 && b) at = atomicAdd(&n_held, __popc(b));
+            at = __shfl_sync(0xffffffffu, at, 0);
+            if ((b >> lane) & 1) held[at + __popc(b & ((1u << lane) - 1))] = (uint8_t)t;
+        }
+        __syncthreads();
+        const uint32_t n_who = n_held, todo = n_who * ((p1 - p0 + kThreads - 1) / kThreads);
         if (t < kMaxTop) best[t] = 0;
         // what reaches the floor; where that is more than the list holds (many ties at the floor) what passes it, and
         // where that is too, nothing: the alternatives are then found one by one
@@ -239,17 +255,22 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 8) logprobs_ke
                     if (at < kList) list[at] = (u64)k << 32 | (0xffffffffu - index);
                 }
             };
-            // a warp reads the pieces of one of its threads at a time
-            for (uint32_t hold = __ballot_sync(0xffffffffu, reaches(key)); hold; hold &= hold - 1) {
-                const uint32_t who = warp * 32 + __ffs(hold) - 1;
-                for (uint32_t i = p0 + who + lane * kThreads; i < p1; i += 32 * kThreads) {
-                    float v[N];
-                    Piece<T>::load(xp + (size_t)i * N, v);
+            for (uint32_t j0 = t; j0 < todo; j0 += 4 * kThreads) {
+                float v[4][N];
+                uint32_t at[4];
 #pragma unroll
-                    for (int e = 0; e < N; e++) put(v[e], head + i * N + e);
+                for (int u = 0; u < 4; u++) {
+                    const uint32_t j = j0 + u * kThreads, i = p0 + j / n_who * kThreads + held[j % n_who];
+                    at[u] = j < todo && i < p1 ? i : 0xffffffffu;
+                    if (at[u] != 0xffffffffu) Piece<T>::load(xp + (size_t)i * N, v[u]);
                 }
-                if (lane == 0 && who < n_extra) put(Piece<T>::one(x + extra(who)), extra(who));
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (at[u] != 0xffffffffu)
+#pragma unroll
+                        for (int e = 0; e < N; e++) put(v[u][e], head + at[u] * N + e);
             }
+            if (t < n_extra) put(Piece<T>::one(x + extra(t)), extra(t));
             __syncthreads();
             n = n_list;
             if (n <= kList || pass) break;
