@@ -67,18 +67,18 @@ template <typename T> struct Piece;
 template <> struct Piece<float> {
     static constexpr int kN = 4;
     static __device__ __forceinline__ float one(const float *p) { return *p; }
-    static __device__ __forceinline__ void load(const float *p, float *x)
+    static constexpr uint32_t kNone = 0xff800000u;        // -inf in every element
+    static __device__ __forceinline__ void open(const uint4 &v, float *x)
     {
-        const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
     }
 };
 template <> struct Piece<__half> {
     static constexpr int kN = 8;
     static __device__ __forceinline__ float one(const __half *p) { return __half2float(*p); }
-    static __device__ __forceinline__ void load(const __half *p, float *x)
+    static constexpr uint32_t kNone = 0xfc00fc00u;
+    static __device__ __forceinline__ void open(const uint4 &v, float *x)
     {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
         const uint32_t r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -89,7 +89,7 @@ template <> struct Piece<__half> {
 };
 
 struct Sums { float m, s, u; };
-__device__ __forceinline__ float lp_exp(float d) { float e; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * kLog2e)); return e; }
+__device__ __forceinline__ float lp_exp(float d) { return ab_ex2(d * kLog2e); }
 // below -1e4 e^d is 0, and (-inf) * 0 would be a NaN
 __device__ __forceinline__ float lp_clamp(float d) { return fmaxf(d, -1e4f); }
 // moves the sums to a maximum M >= m
@@ -108,11 +108,13 @@ __device__ __forceinline__ void lp_join(Sums &a, Sums b)
     a.s += b.s;
     a.u += b.u;
 }
-__device__ __forceinline__ void lp_add(Sums &a, float x)
+// two elements, into sums of their own
+__device__ __forceinline__ void lp_add(float2 x, float2 m, float2 &s, float2 &u)
 {
-    const float d = x - a.m, e = lp_exp(d);
-    a.s += e;
-    a.u = fmaf(lp_clamp(d), e, a.u);
+    const float2 d = ab_add2(x, make_float2(-m.x, -m.y)), z = ab_mul2(d, make_float2(kLog2e, kLog2e));
+    const float2 e = make_float2(ab_ex2(z.x), ab_ex2(z.y));
+    s = ab_add2(s, e);
+    u = ab_fma2(make_float2(lp_clamp(d.x), lp_clamp(d.y)), e, u);
 }
 
 __device__ __forceinline__ uint32_t lp_mapa(const void *p, uint32_t rank)
@@ -159,26 +161,35 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 6) logprobs_ke
 
     // ---- one pass
     Sums a{kLowest, 0.f, 0.f};
+    const auto fetch = [&](uint32_t i) {
+        return i < p1 ? __ldg(reinterpret_cast<const uint4 *>(xp) + i) : make_uint4(Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone);
+    };
+    uint4 next[U];
+#pragma unroll
+    for (int j = 0; j < U; j++) next[j] = fetch(p0 + t + j * kThreads);
     for (uint32_t i = p0 + t; i < p1; i += kThreads * U) {
         float v[16];
 #pragma unroll
         for (int j = 0; j < U; j++) {
-            if (i + j * kThreads < p1) Piece<T>::load(xp + (size_t)(i + j * kThreads) * N, v + j * N);
-            else
-#pragma unroll
-                for (int e = 0; e < N; e++) v[j * N + e] = -CUDART_INF_F;
+            Piece<T>::open(next[j], v + j * N);
+            next[j] = fetch(i + (U + j) * kThreads);                // the next 16 are on their way
         }
         float c = v[0];
 #pragma unroll
         for (int e = 1; e < 16; e++) c = fmaxf(c, v[e]);
         lp_move(a, fmaxf(a.m, c));
+        float2 s = make_float2(a.s, 0.f), u = make_float2(a.u, 0.f);
 #pragma unroll
-        for (int e = 0; e < 16; e++) lp_add(a, v[e]);
+        for (int e = 0; e < 16; e += 2) lp_add(make_float2(v[e], v[e + 1]), make_float2(a.m, a.m), s, u);
+        a.s = s.x + s.y;
+        a.u = u.x + u.y;
     }
     if (t < n_extra) {
         const float v = Piece<T>::one(x + extra(t));
         lp_move(a, fmaxf(a.m, v));
-        lp_add(a, v);
+        const float d = v - a.m, e = lp_exp(d);
+        a.s += e;
+        a.u = fmaf(lp_clamp(d), e, a.u);
     }
     // the thread's largest element.  a.m says it but for a NaN (which s shows), and where nothing is above -FLT_MAX
     const bool any = p0 + t < p1 || t < n_extra;
@@ -255,20 +266,23 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 6) logprobs_ke
                     if (at < kList) list[at] = (u64)k << 32 | (0xffffffffu - index);
                 }
             };
-            for (uint32_t j0 = t; j0 < todo; j0 += 4 * kThreads) {
-                float v[4][N];
-                uint32_t at[4];
+            for (uint32_t j0 = t; j0 < todo; j0 += U * kThreads) {
+                uint4 raw[U];
+                uint32_t at[U];
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
+                for (int u = 0; u < U; u++) {
                     const uint32_t j = j0 + u * kThreads, i = p0 + j / n_who * kThreads + held[j % n_who];
                     at[u] = j < todo && i < p1 ? i : 0xffffffffu;
-                    if (at[u] != 0xffffffffu) Piece<T>::load(xp + (size_t)i * N, v[u]);
+                    raw[u] = fetch(at[u]);
                 }
 #pragma unroll
-                for (int u = 0; u < 4; u++)
+                for (int u = 0; u < U; u++) {
+                    float v[N];
+                    Piece<T>::open(raw[u], v);
                     if (at[u] != 0xffffffffu)
 #pragma unroll
-                        for (int e = 0; e < N; e++) put(v[u][e], head + at[u] * N + e);
+                        for (int e = 0; e < N; e++) put(v[e], head + at[u] * N + e);
+                }
             }
             if (t < n_extra) put(Piece<T>::one(x + extra(t)), extra(t));
             __syncthreads();

@@ -149,12 +149,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float4 lds128(uint32_t addr)
 {
     float4 v;
@@ -437,9 +431,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
             const float m1 = fmaxf(m[c], x), ms = m1 == -CUDART_INF_F ? 0.f : m1;
             const float bias = sizeof(T) == 2 ? kWeightBias : 0.f;
-            a[c] = m[c] == m1 ? 1.f : ex2(m[c] - ms);
-            pr[c] = ex2(s[c] - ms + bias);
-            pr[c + 2] = ex2(s[c + 2] - ms + bias);
+            a[c] = m[c] == m1 ? 1.f : ab_ex2(m[c] - ms);
+            pr[c] = ab_ex2(s[c] - ms + bias);
+            pr[c + 2] = ab_ex2(s[c + 2] - ms + bias);
             m[c] = m1;
             l[c] = fmaf(l[c], a[c], pr[c] + pr[c + 2]);
         }
@@ -475,7 +469,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
         for (int i = 1; i < kRowWarps; i++) M = fmaxf(M, part_ml[i * 16 + c]);
         float ls = 0.f, os = 0.f;
         for (int i = 0; i < kRowWarps; i++) {
-            const float f = part_ml[i * 16 + c] == -CUDART_INF_F ? 0.f : ex2(part_ml[i * 16 + c] - M);
+            const float f = part_ml[i * 16 + c] == -CUDART_INF_F ? 0.f : ab_ex2(part_ml[i * 16 + c] - M);
             ls = fmaf(part_ml[i * 16 + 8 + c], f, ls);
             os = fmaf(part_o[(i * 8 + c) * DP + d], f, os);
         }
@@ -496,7 +490,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
         for (uint32_t i = 0; i < parts; i++) M = fmaxf(M, ld_cluster(ml_at + c * 4, i));
         float ls = 0.f, os = 0.f;
         for (uint32_t i = 0; i < parts; i++) {
-            const float mi = ld_cluster(ml_at + c * 4, i), f = mi == -CUDART_INF_F ? 0.f : ex2(mi - M);
+            const float mi = ld_cluster(ml_at + c * 4, i), f = mi == -CUDART_INF_F ? 0.f : ab_ex2(mi - M);
             ls = fmaf(ld_cluster(ml_at + (8 + c) * 4, i), f, ls);
             os = fmaf(ld_cluster(o_at + (c * DP + d) * 4, i), f, os);
         }

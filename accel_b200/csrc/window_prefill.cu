@@ -234,37 +234,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
                  : "r"(taddr) : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ex2(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// two f32 operations in one instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
-{
-    float2 d;
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
-        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b)
-{
-    float2 d;
-    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b)
-{
-    float2 d;
-    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
-        "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
 __device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 // bits [a, b) of a word, a and b clipped to it
 __device__ __forceinline__ uint32_t bit_range(int a, int b)
@@ -517,7 +486,7 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
             }
             // (rounded up to a 64th: m1 - 14 is then exact, and so the weights of all tiles are relative to the same maxima)
             const float m1 = fmaxf(m, ceilf(top * c * 64.f) * 0.015625f), ms = (m1 == -CUDART_INF_F ? 0.f : m1) - kBias;
-            const float a = m == m1 ? 1.f : ex2(m - (ms + kBias));
+            const float a = m == m1 ? 1.f : ab_ex2(m - (ms + kBias));
             m = m1;
             float2 sum = make_float2(0.f, 0.f);
             const float2 c2 = make_float2(c, c), ms2 = make_float2(-ms, -ms);
@@ -531,11 +500,11 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
                     uint32_t out[16];
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
-                        const float2 z = fma2(make_float2(__uint_as_float(s[k + e]), __uint_as_float(s[k + e + 1])), c2, ms2);
-                        const float2 x = make_float2(ex2(z.x), ex2(z.y));
-                        sum = add2(sum, x);
+                        const float2 z = ab_fma2(make_float2(__uint_as_float(s[k + e]), __uint_as_float(s[k + e + 1])), c2, ms2);
+                        const float2 x = make_float2(ab_ex2(z.x), ab_ex2(z.y));
+                        sum = ab_add2(sum, x);
                         // the high part is cut off (11 bits), what is left of it rounded
-                        const float2 h = make_float2(cut(x.x), cut(x.y)), d = add2(x, make_float2(-h.x, -h.y));
+                        const float2 h = make_float2(cut(x.x), cut(x.y)), d = ab_add2(x, make_float2(-h.x, -h.y));
                         out[e / 2] = pack_f16x2(h.x, h.y);
                         out[8 + e / 2] = pack_f16x2(d.x, d.y);
                     }
@@ -557,8 +526,8 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     float2 x = make_float2(__uint_as_float(d[e]), __uint_as_float(d[e + 1]));
-                    if (sizeof(T) == 4) x = mul2(x, make_float2(vs, vs));
-                    x = fma2(make_float2(o[32 * w + e], o[32 * w + e + 1]), make_float2(a, a), x);
+                    if (sizeof(T) == 4) x = ab_mul2(x, make_float2(vs, vs));
+                    x = ab_fma2(make_float2(o[32 * w + e], o[32 * w + e + 1]), make_float2(a, a), x);
                     o[32 * w + e] = x.x;
                     o[32 * w + e + 1] = x.y;
                 }
@@ -580,7 +549,7 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
         ml[(wg * 3 + 2) * kRows] = __uint_as_float(bad);
         asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
         const float m0 = ml[0], m1 = ml[3 * kRows], M = fmaxf(m0, m1);
-        const float f0 = m0 == -CUDART_INF_F ? 0.f : ex2(m0 - M), f1 = m1 == -CUDART_INF_F ? 0.f : ex2(m1 - M);
+        const float f0 = m0 == -CUDART_INF_F ? 0.f : ab_ex2(m0 - M), f1 = m1 == -CUDART_INF_F ? 0.f : ab_ex2(m1 - M);
         const float sum = fmaf(ml[kRows], f0, ml[4 * kRows] * f1), fm = (wg ? f1 : f0) / sum, fo = (wg ? f0 : f1) / sum;
 #pragma unroll
         for (int i = 0; i < DP / 2; i += 4) {
