@@ -336,6 +336,51 @@ __device__ __forceinline__ void cluster_sync()
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The parts of a row's heads, one per warp (or group of lanes), then one per CTA of the cluster, joined in their order:
+// [part][maxima of C columns, sums of C columns] and [part][C][DP] in shared memory, the CTA's own result behind them.
+template <int N, int C, int DP>
+__device__ __forceinline__ void join_parts(const WinParams &p, float *part_ml, float *part_o, uint32_t row, uint32_t h0, uint32_t heads,
+                                           uint32_t part, uint32_t parts, bool zero)
+{
+    float *cta_ml = part_o + N * C * DP, *cta_o = cta_ml + 2 * C;
+    const uint32_t D = p.head_dim;
+    __syncthreads();
+    for (uint32_t x = threadIdx.x; x < heads * DP; x += blockDim.x) {
+        const uint32_t c = x / DP, d = x % DP;
+        float M = part_ml[c];
+        for (int i = 1; i < N; i++) M = fmaxf(M, part_ml[i * 2 * C + c]);
+        float ls = 0.f, os = 0.f;
+        for (int i = 0; i < N; i++) {
+            const float mi = part_ml[i * 2 * C + c], f = mi == -CUDART_INF_F ? 0.f : ab_ex2(mi - M);
+            ls = fmaf(part_ml[i * 2 * C + C + c], f, ls);
+            os = fmaf(part_o[(i * C + c) * DP + d], f, os);
+        }
+        if (parts == 1) {
+            if (d < D) p.out[((uint64_t)row * p.q_heads + h0 + c) * D + d] = zero ? 0.f : os / ls;
+        } else {
+            cta_o[c * DP + d] = os;
+            if (d == 0) { cta_ml[c] = M; cta_ml[C + c] = ls; }
+        }
+    }
+    if (parts == 1) return;
+    cluster_sync();
+    const uint32_t ml_at = (uint32_t)__cvta_generic_to_shared(cta_ml), o_at = (uint32_t)__cvta_generic_to_shared(cta_o);
+    for (uint32_t x = part * blockDim.x + threadIdx.x; x < heads * DP; x += parts * blockDim.x) {
+        const uint32_t c = x / DP, d = x % DP;
+        if (d >= D) continue;
+        float M = -CUDART_INF_F;
+        for (uint32_t i = 0; i < parts; i++) M = fmaxf(M, ld_cluster(ml_at + c * 4, i));
+        float ls = 0.f, os = 0.f;
+        for (uint32_t i = 0; i < parts; i++) {
+            const float mi = ld_cluster(ml_at + c * 4, i), f = mi == -CUDART_INF_F ? 0.f : ab_ex2(mi - M);
+            ls = fmaf(ld_cluster(ml_at + (C + c) * 4, i), f, ls);
+            os = fmaf(ld_cluster(o_at + (c * DP + d) * 4, i), f, os);
+        }
+        p.out[((uint64_t)row * p.q_heads + h0 + c) * D + d] = zero ? 0.f : os / ls;
+    }
+    cluster_sync();                                                 // nobody leaves while its parts are being read
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_rows_kernel(const WinParams p, const uint32_t parts)
 {
@@ -448,9 +493,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
     __syncthreads();
 
     // ---- the warps' parts, then the CTAs'
-    // per warp and column: maximum, sum, DP values; then the same of the CTA
     float *part_ml = reinterpret_cast<float *>(smem), *part_o = part_ml + kRowWarps * 16;
-    float *cta_ml = part_o + kRowWarps * 8 * DP, *cta_o = cta_ml + 16;
 #pragma unroll
     for (int c = 0; c < 2; c++) {
         l[c] += __shfl_xor_sync(0xffffffffu, l[c], 4);
@@ -462,41 +505,110 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
     for (int i = 0; i < DP / 16; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) part_o[(warp * 8 + 2 * t + (e & 1)) * DP + Math::dim(i, e, g)] = o[i][e];
-    __syncthreads();
-    for (uint32_t x = threadIdx.x; x < heads * DP; x += kRowWarps * 32) {
-        const uint32_t c = x / DP, d = x % DP;
-        float M = part_ml[c];
-        for (int i = 1; i < kRowWarps; i++) M = fmaxf(M, part_ml[i * 16 + c]);
-        float ls = 0.f, os = 0.f;
-        for (int i = 0; i < kRowWarps; i++) {
-            const float f = part_ml[i * 16 + c] == -CUDART_INF_F ? 0.f : ab_ex2(part_ml[i * 16 + c] - M);
-            ls = fmaf(part_ml[i * 16 + 8 + c], f, ls);
-            os = fmaf(part_o[(i * 8 + c) * DP + d], f, os);
-        }
-        if (parts == 1) {
-            if (d < D) p.out[((uint64_t)row * p.q_heads + h0 + c) * D + d] = w.zero ? 0.f : os / ls;
-        } else {
-            cta_o[c * DP + d] = os;
-            if (d == 0) { cta_ml[c] = M; cta_ml[8 + c] = ls; }
+    join_parts<kRowWarps, 8, DP>(p, part_ml, part_o, row, h0, heads, part, parts, w.zero);
+}
+
+// ------------------------------------------------------------------------------------------------
+// The lane kernel: an f32 cache and one to four query heads per KV head, on the CUDA cores.
+//
+// LR lanes hold a position's row, four dimensions each (LR = 32 for a head of up to 128, 16 of up to 64, 8 of up to
+// 32), and take eight positions at a time: their K and V rows are loaded at once, straight into registers, and the
+// eight dot products of a head are reduced over the lanes together (4 + 2 + 1 exchanges that halve what is left,
+// then whole ones), so that a lane ends with one position's score and takes one exponential for it.  Every
+// group of LR lanes has its own maximum, sum and output.  f32 throughout.
+//
+// Per position 23 warp instructions with one head and 68 with four, where the tensor-core form above takes 84
+// whatever the heads (up to eight) and is bound by them: it stays for more heads and for f16 caches.
+// ------------------------------------------------------------------------------------------------
+template <int G, int LR>
+__global__ void __launch_bounds__(kRowWarps * 32, G <= 2 ? 4 : 3) win_lanes_kernel(const WinParams p, const uint32_t parts)
+{
+    constexpr int S = 32 / LR, DP = 4 * LR, kPart = kRowWarps * S;
+    __shared__ __align__(16) float smem[kPart * G * (DP + 2) + G * (DP + 2)];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LR, ll = lane % LR;
+    const uint32_t row = blockIdx.x / parts, part = blockIdx.x % parts, kvh = blockIdx.y, h0 = kvh * G, D = p.head_dim;
+    const bool on = (uint32_t)ll * 4 < D;
+    const WinView w = win_view(p, row);
+    const uint32_t n_batches = (w.n + 7) / 8, step = parts * kPart;
+    const auto rows_of = [&](uint32_t b) -> uint32_t {                 // lanes 0..7 of a group: its eight positions
+        const uint32_t i = b * 8 + (ll & 7);
+        return i < w.n ? win_row(p, w, i) : 0xffffffffu;
+    };
+    uint32_t b0 = (part * kRowWarps + warp) * S;
+    uint32_t rows = b0 < n_batches ? rows_of(b0 + sub) : 0xffffffffu;
+    float4 q[G], o[G];
+    float m[G], l[G];
+#pragma unroll
+    for (int h = 0; h < G; h++) {
+        q[h] = on ? *reinterpret_cast<const float4 *>(p.q + ((uint64_t)row * p.q_heads + h0 + h) * D + ll * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        q[h].x *= p.scale_log2; q[h].y *= p.scale_log2; q[h].z *= p.scale_log2; q[h].w *= p.scale_log2;
+        o[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+        m[h] = -CUDART_INF_F;
+        l[h] = 0.f;
+    }
+    const uint64_t pitch = (uint64_t)p.kv_heads * D;
+    const float *kb = static_cast<const float *>(p.k) + (uint64_t)kvh * D + ll * 4, *vb = static_cast<const float *>(p.v) + (uint64_t)kvh * D + ll * 4;
+    const auto row4 = [&](const float *base, uint32_t r) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (on && r != 0xffffffffu)
+            asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(base + r * pitch));
+        return x;
+    };
+    for (; b0 < n_batches; b0 += step) {
+        float4 k[8], v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) k[j] = row4(kb, __shfl_sync(0xffffffffu, rows, sub * LR + j));
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = row4(vb, __shfl_sync(0xffffffffu, rows, sub * LR + j));
+        // the position whose score a lane ends with
+        const bool seen = __shfl_sync(0xffffffffu, rows, sub * LR + ll / (LR / 8)) != 0xffffffffu;
+        rows = b0 + step < n_batches ? rows_of(b0 + step + sub) : 0xffffffffu;
+#pragma unroll
+        for (int h = 0; h < G; h++) {
+            float s[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) s[j] = fmaf(q[h].w, k[j].w, fmaf(q[h].z, k[j].z, fmaf(q[h].y, k[j].y, q[h].x * k[j].x)));
+#pragma unroll
+            for (int i = 0; i < 3; i++) {                              // a group's halves keep half of the scores each
+                const int width = LR >> (i + 1), n = 4 >> i;
+                const bool upper = (ll & width) != 0;
+#pragma unroll
+                for (int j = 0; j < n; j++) {
+                    const float give = upper ? s[j] : s[j + n], keep = upper ? s[j + n] : s[j];
+                    s[j] = keep + __shfl_xor_sync(0xffffffffu, give, width);
+                }
+            }
+            float x = s[0];
+#pragma unroll
+            for (int width = LR / 16; width; width /= 2) x += __shfl_xor_sync(0xffffffffu, x, width);
+            if (!seen) x = -CUDART_INF_F;
+            float top = x;
+#pragma unroll
+            for (int i = 1; i <= 3; i++) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, LR >> i));
+            const float m1 = fmaxf(m[h], top), ms = m1 == -CUDART_INF_F ? 0.f : m1;
+            const float a = m[h] == m1 ? 1.f : ab_ex2(m[h] - ms), e = ab_ex2(x - ms);
+            m[h] = m1;
+            l[h] = fmaf(l[h], a, e);
+            o[h].x *= a; o[h].y *= a; o[h].z *= a; o[h].w *= a;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float pj = __shfl_sync(0xffffffffu, e, sub * LR + j * (LR / 8));
+                o[h].x = fmaf(pj, v[j].x, o[h].x); o[h].y = fmaf(pj, v[j].y, o[h].y);
+                o[h].z = fmaf(pj, v[j].z, o[h].z); o[h].w = fmaf(pj, v[j].w, o[h].w);
+            }
         }
     }
-    if (parts == 1) return;
-    cluster_sync();
-    const uint32_t ml_at = (uint32_t)__cvta_generic_to_shared(cta_ml), o_at = (uint32_t)__cvta_generic_to_shared(cta_o);
-    for (uint32_t x = part * (kRowWarps * 32) + threadIdx.x; x < heads * DP; x += parts * kRowWarps * 32) {
-        const uint32_t c = x / DP, d = x % DP;
-        if (d >= D) continue;
-        float M = -CUDART_INF_F;
-        for (uint32_t i = 0; i < parts; i++) M = fmaxf(M, ld_cluster(ml_at + c * 4, i));
-        float ls = 0.f, os = 0.f;
-        for (uint32_t i = 0; i < parts; i++) {
-            const float mi = ld_cluster(ml_at + c * 4, i), f = mi == -CUDART_INF_F ? 0.f : ab_ex2(mi - M);
-            ls = fmaf(ld_cluster(ml_at + (8 + c) * 4, i), f, ls);
-            os = fmaf(ld_cluster(o_at + (c * DP + d) * 4, i), f, os);
-        }
-        p.out[((uint64_t)row * p.q_heads + h0 + c) * D + d] = w.zero ? 0.f : os / ls;
+    float *part_ml = smem, *part_o = part_ml + kPart * 2 * G;
+    const int unit = warp * S + sub;
+#pragma unroll
+    for (int h = 0; h < G; h++) {
+#pragma unroll
+        for (int i = 1; i <= 3; i++) l[h] += __shfl_xor_sync(0xffffffffu, l[h], LR >> i);
+        if (ll == 0) { part_ml[unit * 2 * G + h] = m[h]; part_ml[unit * 2 * G + G + h] = l[h]; }
+        *reinterpret_cast<float4 *>(part_o + (unit * G + h) * DP + ll * 4) = o[h];
     }
-    cluster_sync();                                                 // nobody leaves while its parts are being read
+    join_parts<kPart, G, DP>(p, part_ml, part_o, row, h0, G, part, parts, w.zero);
 }
 
 // the kernel's dynamic shared memory and cluster sizes beyond what a kernel gets unasked: once per device
@@ -515,22 +627,20 @@ template <typename T, int DP> int rows_prepare(const char *name)
     return AB_OK;
 }
 
-template <typename T, int DP> int launch_rows(Launch &l, const WinParams &p, const char *name)
+// grid: a cluster of CTAs per row (blockIdx.x) and group of heads (blockIdx.y).  parts: CTAs that share a row's list, enough
+// to give the SMs their resident CTAs as long as every warp still has `chunk` positions of its own.
+int launch_split(Launch &l, const WinParams &p, void (*kernel)(const WinParams, const uint32_t), uint32_t groups, uint32_t resident,
+                 uint32_t chunk, size_t smem, const char *how, const char *name)
 {
-    const uint32_t group = p.q_heads / p.kv_heads, groups = p.kv_heads * ((group + 7) / 8);
-    // CTAs of a cluster that share a row's list: enough to give the SMs their three resident CTAs, as long as every warp
-    // still has a tile of its own
-    const uint64_t longest = std::min<uint64_t>((uint64_t)p.window + p.sinks, p.reach), want = 3ull * sm_count();
+    const uint64_t longest = std::min<uint64_t>((uint64_t)p.window + p.sinks, p.reach), want = (uint64_t)resident * sm_count();
     uint32_t parts = 1;
-    while (parts < 8 && (uint64_t)p.rows * groups * parts < want && longest > (uint64_t)parts * kRowWarps * kTile) parts *= 2;
+    while (parts < 8 && (uint64_t)p.rows * groups * parts < want && longest > (uint64_t)parts * kRowWarps * chunk) parts *= 2;
     if ((uint64_t)p.rows * parts > 0x7fffffffull || groups > 65535)
         return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
-    const int rc = rows_prepare<T, DP>(name);
-    if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.rows * parts, groups);
     cfg.blockDim = dim3(kRowWarps * 32);
-    cfg.dynamicSmemBytes = RowTile<T, DP>::kSmem;
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = l.stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -538,10 +648,25 @@ template <typename T, int DP> int launch_rows(Launch &l, const WinParams &p, con
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, win_rows_kernel<T, DP>, p, parts);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, parts);
     count_launch();
-    note_selection("%s: %u rows, %u group(s) of up to 8 query heads, a list split over %u CTA(s)", name, p.rows, groups, parts);
+    note_selection("%s: %s, %u rows, %u group(s) of heads, a list split over %u CTA(s)", name, how, p.rows, groups, parts);
     return check_cuda(e, name);
+}
+
+template <typename T, int DP> int launch_rows(Launch &l, const WinParams &p, const char *name)
+{
+    const uint32_t group = p.q_heads / p.kv_heads;
+    const int rc = rows_prepare<T, DP>(name);
+    if (rc) return rc;
+    return launch_split(l, p, win_rows_kernel<T, DP>, p.kv_heads * ((group + 7) / 8), 3, kTile, RowTile<T, DP>::kSmem,
+                        "up to 8 heads a CTA on the tensor cores", name);
+}
+
+template <int G> int launch_lanes(Launch &l, const WinParams &p, const char *name)
+{
+    void (*kernel)(const WinParams, const uint32_t) = p.head_dim > 64 ? win_lanes_kernel<G, 32> : (p.head_dim > 32 ? win_lanes_kernel<G, 16> : win_lanes_kernel<G, 8>);
+    return launch_split(l, p, kernel, p.kv_heads, G <= 2 ? 4 : 3, p.head_dim > 64 ? 8 : (p.head_dim > 32 ? 16 : 32), 0, "a row a group of lanes", name);
 }
 
 // query rows (tokens x heads of a KV head) of one sequence from which 128-row tiles take over
@@ -557,6 +682,15 @@ template <typename T> int run_window(Launch &l, WinParams &p, const char *name)
     if (p.form == kPrefillRows && group <= 128 && (uint64_t)p.rows * group >= kTileFrom)
         return run_window_tiles(l, p, sizeof(T) == 2, name);
     if (l.query_ws) return AB_OK;
+    if (sizeof(T) == 4) {
+        switch (group) {
+        case 1: return launch_lanes<1>(l, p, name);
+        case 2: return launch_lanes<2>(l, p, name);
+        case 3: return launch_lanes<3>(l, p, name);
+        case 4: return launch_lanes<4>(l, p, name);
+        default: break;
+        }
+    }
     return p.head_dim <= 64 ? launch_rows<T, 64>(l, p, name) : launch_rows<T, 128>(l, p, name);
 }
 
