@@ -74,11 +74,23 @@ __device__ __forceinline__ WinView win_view(const WinParams &p, uint32_t row)
     return w;
 }
 
-// the cache row of the list's entry i; 0xffffffff where its page lies outside the cache
-__device__ __forceinline__ uint32_t win_row(const WinParams &p, const WinView &w, uint32_t i)
+// The list's entry i: its position; the page that holds it (loaded now, looked at later: a page's number is asked for
+// two tiles ahead of its rows, so that nothing waits for the table); its cache row, 0xffffffff where that page lies outside
+// the cache.
+__device__ __forceinline__ uint32_t win_position(const WinView &w, uint32_t i) { return i < w.ns ? i : w.lo + (i - w.ns); }
+__device__ __forceinline__ uint32_t win_page(const WinParams &p, const WinView &w, uint32_t i)
 {
-    const uint32_t j = i < w.ns ? i : w.lo + (i - w.ns);
-    return win_cache_row(p, w.pages, j);
+    uint32_t pg = 0xffffffffu;
+    if (i < w.n && w.pages)
+        asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(pg) : "l"(w.pages + win_position(w, i) / p.block));
+    return pg;
+}
+__device__ __forceinline__ uint32_t win_row(const WinParams &p, const WinView &w, uint32_t i, uint32_t page)
+{
+    if (i >= w.n) return 0xffffffffu;
+    const uint32_t j = win_position(w, i);
+    const uint64_t r = w.pages ? (uint64_t)page * p.block + j % p.block : j;
+    return r < p.capacity ? (uint32_t)r : 0xffffffffu;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -401,7 +413,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
     // lanes 0..15 know the cache rows of a tile's positions (lanes 16..31 the same again)
     const auto rows_of = [&](uint32_t tl) -> uint32_t {
         const uint32_t i = tl * kTile + (lane & 15);
-        return i < w.n ? win_row(p, w, i) : 0xffffffffu;
+        return win_row(p, w, i, win_page(p, w, i));
     };
     const uint32_t row_bytes = D * sizeof(T), chunks = row_bytes / 16;
     const int span = chunks > 16 ? 32 : (chunks > 8 ? 16 : 8);      // lanes that copy one row
@@ -512,30 +524,58 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
 // The lane kernel: an f32 cache and one to four query heads per KV head, on the CUDA cores.
 //
 // LR lanes hold a position's row, four dimensions each (LR = 32 for a head of up to 128, 16 of up to 64, 8 of up to
-// 32), and take eight positions at a time: their K and V rows are loaded at once, straight into registers, and the
-// eight dot products of a head are reduced over the lanes together (4 + 2 + 1 exchanges that halve what is left,
-// then whole ones), so that a lane ends with one position's score and takes one exponential for it.  Every
-// group of LR lanes has its own maximum, sum and output.  f32 throughout.
+// 32), and take eight positions at a time: the eight dot products of a head are reduced over the lanes together (4 + 2
+// + 1 exchanges that halve what is left, then whole ones), so that a lane ends with one position's score and takes one
+// exponential for it.  Every group of LR lanes has its own maximum, sum and output.  f32 throughout.
 //
-// Per position 23 warp instructions with one head and 68 with four, where the tensor-core form above takes 84
+// The rows come by cp.async into a ring of two stages per warp, and a lane reads back what it copied itself, so a stage
+// needs no barrier, and one is in flight while the other is worked on.  (In registers, loads for the next eight
+// positions cost more than they hid: 148 us for the f32 batch, and 97 us without them.)
+//
+// Per position 25 warp instructions with one head and 70 with four, where the tensor-core form above takes 84
 // whatever the heads (up to eight) and is bound by them: it stays for more heads and for f16 caches.
 // ------------------------------------------------------------------------------------------------
+constexpr uint32_t kStageBytes = 8192;                              // of a warp: eight positions' rows of K and V in every group of lanes
+constexpr uint32_t kLanesSmem = kRowWarps * 2 * kStageBytes;
+
 template <int G, int LR>
-__global__ void __launch_bounds__(kRowWarps * 32, G <= 2 ? 4 : 3) win_lanes_kernel(const WinParams p, const uint32_t parts)
+__global__ void __launch_bounds__(kRowWarps * 32, 3) win_lanes_kernel(const WinParams p, const uint32_t parts)
 {
     constexpr int S = 32 / LR, DP = 4 * LR, kPart = kRowWarps * S;
-    __shared__ __align__(16) float smem[kPart * G * (DP + 2) + G * (DP + 2)];
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    static_assert((kPart + 1) * G * (DP + 2) * 4 <= kLanesSmem, "the parts fit where the rows were");
+    float *smem = reinterpret_cast<float *>(smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LR, ll = lane % LR;
     const uint32_t row = blockIdx.x / parts, part = blockIdx.x % parts, kvh = blockIdx.y, h0 = kvh * G, D = p.head_dim;
     const bool on = (uint32_t)ll * 4 < D;
     const WinView w = win_view(p, row);
     const uint32_t n_batches = (w.n + 7) / 8, step = parts * kPart;
-    const auto rows_of = [&](uint32_t b) -> uint32_t {                 // lanes 0..7 of a group: its eight positions
-        const uint32_t i = b * 8 + (ll & 7);
-        return i < w.n ? win_row(p, w, i) : 0xffffffffu;
+    // lanes 0..7 of a group: its eight positions (past the last batch there is nothing to see)
+    const auto page_of = [&](uint32_t b) { return win_page(p, w, (b + sub) * 8 + (ll & 7)); };
+    const auto rows_of = [&](uint32_t b, uint32_t page) { return win_row(p, w, (b + sub) * 8 + (ll & 7), page); };
+    const uint64_t pitch = (uint64_t)p.kv_heads * D;
+    const float *kb = static_cast<const float *>(p.k) + (uint64_t)kvh * D + ll * 4, *vb = static_cast<const float *>(p.v) + (uint64_t)kvh * D + ll * 4;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem_raw) + warp * 2 * kStageBytes + lane * 16;
+    const auto copy = [&](uint32_t stage, uint32_t rows) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t r = __shfl_sync(0xffffffffu, rows, sub * LR + j);
+            const bool load = on && r != 0xffffffffu;
+            const uint64_t at = load ? r * pitch : 0;
+            cp16(ring + stage * kStageBytes + j * 512, kb + at, load);
+            cp16(ring + stage * kStageBytes + 4096 + j * 512, vb + at, load);
+        }
+        cp_commit();
     };
-    uint32_t b0 = (part * kRowWarps + warp) * S;
-    uint32_t rows = b0 < n_batches ? rows_of(b0 + sub) : 0xffffffffu;
+    uint32_t b0 = (part * kRowWarps + warp) * S, seen0, seen1;
+    {
+        const uint32_t page0 = page_of(b0), page1 = page_of(b0 + step);
+        seen0 = rows_of(b0, page0);
+        copy(0, seen0);
+        seen1 = rows_of(b0 + step, page1);
+        copy(1, seen1);
+    }
+    uint32_t page = page_of(b0 + 2 * step);
     float4 q[G], o[G];
     float m[G], l[G];
 #pragma unroll
@@ -546,24 +586,15 @@ __global__ void __launch_bounds__(kRowWarps * 32, G <= 2 ? 4 : 3) win_lanes_kern
         m[h] = -CUDART_INF_F;
         l[h] = 0.f;
     }
-    const uint64_t pitch = (uint64_t)p.kv_heads * D;
-    const float *kb = static_cast<const float *>(p.k) + (uint64_t)kvh * D + ll * 4, *vb = static_cast<const float *>(p.v) + (uint64_t)kvh * D + ll * 4;
-    const auto row4 = [&](const float *base, uint32_t r) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (on && r != 0xffffffffu)
-            asm volatile("ld.global.nc.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(base + r * pitch));
-        return x;
-    };
-    for (; b0 < n_batches; b0 += step) {
-        float4 k[8], v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) k[j] = row4(kb, __shfl_sync(0xffffffffu, rows, sub * LR + j));
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = row4(vb, __shfl_sync(0xffffffffu, rows, sub * LR + j));
+    uint32_t stage = 0;
+    for (; b0 < n_batches; b0 += step, stage ^= 1) {
         // the position whose score a lane ends with
-        const bool seen = __shfl_sync(0xffffffffu, rows, sub * LR + ll / (LR / 8)) != 0xffffffffu;
-        rows = b0 + step < n_batches ? rows_of(b0 + step + sub) : 0xffffffffu;
+        const bool seen = __shfl_sync(0xffffffffu, seen0, sub * LR + ll / (LR / 8)) != 0xffffffffu;
+        float4 k[8];
+        float x[G];
+        cp_wait<1>();
+#pragma unroll
+        for (int j = 0; j < 8; j++) k[j] = lds128(ring + stage * kStageBytes + j * 512);
 #pragma unroll
         for (int h = 0; h < G; h++) {
             float s[8];
@@ -579,26 +610,37 @@ __global__ void __launch_bounds__(kRowWarps * 32, G <= 2 ? 4 : 3) win_lanes_kern
                     s[j] = keep + __shfl_xor_sync(0xffffffffu, give, width);
                 }
             }
-            float x = s[0];
+            x[h] = s[0];
 #pragma unroll
-            for (int width = LR / 16; width; width /= 2) x += __shfl_xor_sync(0xffffffffu, x, width);
-            if (!seen) x = -CUDART_INF_F;
-            float top = x;
+            for (int width = LR / 16; width; width /= 2) x[h] += __shfl_xor_sync(0xffffffffu, x[h], width);
+            if (!seen) x[h] = -CUDART_INF_F;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) k[j] = lds128(ring + stage * kStageBytes + 4096 + j * 512);
+        seen0 = seen1;
+        seen1 = rows_of(b0 + 2 * step, page);
+        copy(stage, seen1);
+        page = page_of(b0 + 3 * step);
+#pragma unroll
+        for (int h = 0; h < G; h++) {
+            float top = x[h];
 #pragma unroll
             for (int i = 1; i <= 3; i++) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, LR >> i));
             const float m1 = fmaxf(m[h], top), ms = m1 == -CUDART_INF_F ? 0.f : m1;
-            const float a = m[h] == m1 ? 1.f : ab_ex2(m[h] - ms), e = ab_ex2(x - ms);
+            const float a = m[h] == m1 ? 1.f : ab_ex2(m[h] - ms), e = ab_ex2(x[h] - ms);
             m[h] = m1;
             l[h] = fmaf(l[h], a, e);
             o[h].x *= a; o[h].y *= a; o[h].z *= a; o[h].w *= a;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float pj = __shfl_sync(0xffffffffu, e, sub * LR + j * (LR / 8));
-                o[h].x = fmaf(pj, v[j].x, o[h].x); o[h].y = fmaf(pj, v[j].y, o[h].y);
-                o[h].z = fmaf(pj, v[j].z, o[h].z); o[h].w = fmaf(pj, v[j].w, o[h].w);
+                o[h].x = fmaf(pj, k[j].x, o[h].x); o[h].y = fmaf(pj, k[j].y, o[h].y);
+                o[h].z = fmaf(pj, k[j].z, o[h].z); o[h].w = fmaf(pj, k[j].w, o[h].w);
             }
         }
     }
+    cp_wait<0>();
+    __syncthreads();
     float *part_ml = smem, *part_o = part_ml + kPart * 2 * G;
     const int unit = warp * S + sub;
 #pragma unroll
@@ -611,30 +653,35 @@ __global__ void __launch_bounds__(kRowWarps * 32, G <= 2 ? 4 : 3) win_lanes_kern
     join_parts<kPart, G, DP>(p, part_ml, part_o, row, h0, G, part, parts, w.zero);
 }
 
-// the kernel's dynamic shared memory and cluster sizes beyond what a kernel gets unasked: once per device
-template <typename T, int DP> int rows_prepare(const char *name)
+// a kernel's shared memory and clusters of 16 CTAs, beyond what it gets unasked: once per device (`done`: a bit for each)
+int prepare(void (*kernel)(const WinParams, const uint32_t), size_t bytes, uint64_t (&done)[4], const char *name)
 {
     static std::mutex mu;
-    static uint64_t done[4];                                        // a bit per device
     int dev = 0;
     cudaGetDevice(&dev);
     std::lock_guard<std::mutex> lock(mu);
     if (dev >= 0 && dev < 256 && (done[dev / 64] >> (dev % 64) & 1)) return AB_OK;
-    int rc = check_cuda(cudaFuncSetAttribute(win_rows_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             RowTile<T, DP>::kSmem), name);
-    if (rc) return rc;
-    if (dev >= 0 && dev < 256) done[dev / 64] |= 1ull << (dev % 64);
-    return AB_OK;
+    int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), name);
+    if (rc == AB_OK) rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), name);
+    if (rc == AB_OK && dev >= 0 && dev < 256) done[dev / 64] |= 1ull << (dev % 64);
+    return rc;
 }
 
-// grid: a cluster of CTAs per row (blockIdx.x) and group of heads (blockIdx.y).  parts: CTAs that share a row's list, enough
-// to give the SMs their resident CTAs as long as every warp still has `chunk` positions of its own.
+// Grid: a cluster of `parts` CTAs that share the list of a row (blockIdx.x) and group of heads (blockIdx.y).  The time of a
+// launch is about the rounds of resident CTAs it takes times the steps of a CTA, `unit` positions each, and three more
+// to start and to join, and an eighth of one per part; parts is what makes that least.  (The f32 batch above, 512 x parts CTAs on 444 places: 98.6, 91.7,
+// 94.8 and 119 us for 1, 2, 4 and 8 parts; the f16 one, 256 x parts on 592: 109, 101, 102 and 112 us.)
 int launch_split(Launch &l, const WinParams &p, void (*kernel)(const WinParams, const uint32_t), uint32_t groups, uint32_t resident,
-                 uint32_t chunk, size_t smem, const char *how, const char *name)
+                 uint32_t unit, size_t smem, const char *how, const char *name)
 {
-    const uint64_t longest = std::min<uint64_t>((uint64_t)p.window + p.sinks, p.reach), want = (uint64_t)resident * sm_count();
+    const uint64_t longest = std::min<uint64_t>((uint64_t)p.window + p.sinks, p.reach), places = (uint64_t)resident * sm_count();
     uint32_t parts = 1;
-    while (parts < 8 && (uint64_t)p.rows * groups * parts < want && longest > (uint64_t)parts * kRowWarps * chunk) parts *= 2;
+    uint64_t least = ~0ull;
+    for (uint32_t n = 1; n <= 16; n *= 2) {
+        const uint64_t rounds = ((uint64_t)p.rows * groups * n + places - 1) / places, steps = (longest + (uint64_t)n * unit - 1) / ((uint64_t)n * unit);
+        const uint64_t cost = rounds * (8 * (steps + 3) + n);
+        if (cost < least) { least = cost; parts = n; }
+    }
     if ((uint64_t)p.rows * parts > 0x7fffffffull || groups > 65535)
         return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
     cudaLaunchConfig_t cfg = {};
@@ -657,16 +704,23 @@ int launch_split(Launch &l, const WinParams &p, void (*kernel)(const WinParams, 
 template <typename T, int DP> int launch_rows(Launch &l, const WinParams &p, const char *name)
 {
     const uint32_t group = p.q_heads / p.kv_heads;
-    const int rc = rows_prepare<T, DP>(name);
+    static uint64_t done[4];
+    const int rc = prepare(win_rows_kernel<T, DP>, RowTile<T, DP>::kSmem, done, name);
     if (rc) return rc;
-    return launch_split(l, p, win_rows_kernel<T, DP>, p.kv_heads * ((group + 7) / 8), 3, kTile, RowTile<T, DP>::kSmem,
+    return launch_split(l, p, win_rows_kernel<T, DP>, p.kv_heads * ((group + 7) / 8), sizeof(T) == 4 ? 3 : 4, kRowWarps * kTile, RowTile<T, DP>::kSmem,
                         "up to 8 heads a CTA on the tensor cores", name);
 }
 
+template <int G, int LR> int launch_lanes(Launch &l, const WinParams &p, const char *name)
+{
+    static uint64_t done[4];
+    const int rc = prepare(win_lanes_kernel<G, LR>, kLanesSmem, done, name);
+    if (rc) return rc;
+    return launch_split(l, p, win_lanes_kernel<G, LR>, p.kv_heads, 3, kRowWarps * 8 * (32 / LR), kLanesSmem, "a row a group of lanes", name);
+}
 template <int G> int launch_lanes(Launch &l, const WinParams &p, const char *name)
 {
-    void (*kernel)(const WinParams, const uint32_t) = p.head_dim > 64 ? win_lanes_kernel<G, 32> : (p.head_dim > 32 ? win_lanes_kernel<G, 16> : win_lanes_kernel<G, 8>);
-    return launch_split(l, p, kernel, p.kv_heads, G <= 2 ? 4 : 3, p.head_dim > 64 ? 8 : (p.head_dim > 32 ? 16 : 32), 0, "a row a group of lanes", name);
+    return p.head_dim > 64 ? launch_lanes<G, 32>(l, p, name) : (p.head_dim > 32 ? launch_lanes<G, 16>(l, p, name) : launch_lanes<G, 8>(l, p, name));
 }
 
 // query rows (tokens x heads of a KV head) of one sequence from which 128-row tiles take over
