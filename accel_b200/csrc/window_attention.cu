@@ -36,11 +36,12 @@ struct WinView {
     const uint32_t *pages;
     uint32_t lo, ns, n;
     bool zero;                                     // a ragged padding row: written as zeros
+    bool skip;                                     // a row of a sequence that went on tiles: not written here
 };
 
 __device__ __forceinline__ WinView win_view(const WinParams &p, uint32_t row)
 {
-    WinView w{p.pages, 0, 0, 0, false};
+    WinView w{p.pages, 0, 0, 0, false, false};
     uint64_t pos1;                                 // the row's position + 1
     uint32_t len;
     if (p.form == kRaggedStep) {
@@ -51,6 +52,7 @@ __device__ __forceinline__ WinView win_view(const WinParams &p, uint32_t row)
             if (p.offsets[m + 1] <= row) a = m + 1; else b = m;
         }
         if (a >= p.batch) { w.zero = true; return w; }
+        if (p.tiled && p.tiled[a]) { w.skip = true; return w; }
         const uint32_t i = row - p.offsets[a], n = p.offsets[a + 1] - p.offsets[a];
         len = p.lengths[a];
         if ((uint64_t)len + i < n) { w.zero = true; return w; }
@@ -407,6 +409,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
     const uint32_t tile_k = (uint32_t)__cvta_generic_to_shared(smem) + warp * Tile::kWarpBytes, tile_v = tile_k + Tile::kBytesK;
 
     const WinView w = win_view(p, row);
+    if (w.skip) return;
     const uint32_t n_tiles = (w.n + kTile - 1) / kTile, step = parts * kRowWarps;
     uint32_t tile = part * kRowWarps + warp;
 
@@ -549,6 +552,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) win_lanes_kernel(const WinP
     const uint32_t row = blockIdx.x / parts, part = blockIdx.x % parts, kvh = blockIdx.y, h0 = kvh * G, D = p.head_dim;
     const bool on = (uint32_t)ll * 4 < D;
     const WinView w = win_view(p, row);
+    if (w.skip) return;
     const uint32_t n_batches = (w.n + 7) / 8, step = parts * kPart;
     // lanes 0..7 of a group: its eight positions (past the last batch there is nothing to see)
     const auto page_of = [&](uint32_t b) { return win_page(p, w, (b + sub) * 8 + (ll & 7)); };
@@ -674,11 +678,13 @@ int prepare(void (*kernel)(const WinParams, const uint32_t), size_t bytes, uint6
 int launch_split(Launch &l, const WinParams &p, void (*kernel)(const WinParams, const uint32_t), uint32_t groups, uint32_t resident,
                  uint32_t unit, size_t smem, const char *how, const char *name)
 {
+    // (beside tiles, the rows left are mostly one of each sequence)
+    const uint64_t rows = p.tiled ? std::min(p.rows, 2 * p.batch) : p.rows;
     const uint64_t longest = std::min<uint64_t>((uint64_t)p.window + p.sinks, p.reach), places = (uint64_t)resident * sm_count();
     uint32_t parts = 1;
     uint64_t least = ~0ull;
     for (uint32_t n = 1; n <= 16; n *= 2) {
-        const uint64_t rounds = ((uint64_t)p.rows * groups * n + places - 1) / places, steps = (longest + (uint64_t)n * unit - 1) / ((uint64_t)n * unit);
+        const uint64_t rounds = (rows * groups * n + places - 1) / places, steps = (longest + (uint64_t)n * unit - 1) / ((uint64_t)n * unit);
         const uint64_t cost = rounds * (8 * (steps + 3) + n);
         if (cost < least) { least = cost; parts = n; }
     }
@@ -723,9 +729,6 @@ template <int G> int launch_lanes(Launch &l, const WinParams &p, const char *nam
     return p.head_dim > 64 ? launch_lanes<G, 32>(l, p, name) : (p.head_dim > 32 ? launch_lanes<G, 16>(l, p, name) : launch_lanes<G, 8>(l, p, name));
 }
 
-// query rows (tokens x heads of a KV head) of one sequence from which 128-row tiles take over
-constexpr uint32_t kTileFrom = 64;
-
 template <typename T> int run_window(Launch &l, WinParams &p, const char *name)
 {
     if ((uint64_t)p.base + p.rows > 0xffffffffull)
@@ -733,8 +736,10 @@ template <typename T> int run_window(Launch &l, WinParams &p, const char *name)
     l.ws_need = 0;
     if (p.rows == 0) return AB_OK;
     const uint32_t group = p.q_heads / p.kv_heads;
-    if (p.form == kPrefillRows && group <= 128 && (uint64_t)p.rows * group >= kTileFrom)
-        return run_window_tiles(l, p, sizeof(T) == 2, name);
+    if ((p.form == kPrefillRows || p.form == kRaggedStep) && group <= 128 && (uint64_t)p.rows * group >= kTileFrom) {
+        const int rc = run_window_tiles(l, p, sizeof(T) == 2, name);
+        if (rc || p.form == kPrefillRows) return rc;
+    }
     if (l.query_ws) return AB_OK;
     if (sizeof(T) == 4) {
         switch (group) {

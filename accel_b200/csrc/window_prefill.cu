@@ -50,24 +50,39 @@ struct TileHead {
     uint32_t seen[4];                       // a bit per position: it exists
 };
 
-// The list of positions packed for a call: sinks in front of the first row's window, then all from that on.
-struct Keys {
-    uint32_t ns, lo;                        // positions [0, ns) and [lo, ...)
-    uint32_t sink_tiles, tiles;
+// A sequence whose rows go on tiles, and the list of positions packed for it: sinks in front of the first row's window,
+// then all from that on.
+struct Segment {
+    uint32_t row0, rows;                    // its query rows: tokens of the call
+    uint32_t base, end;                     // the first row's position; the positions that may exist for any of them
+    uint32_t seq;                           // its row of the page table
+    uint32_t ns, lo;                        // the list: positions [0, ns) and [lo, end)
+    uint32_t sink_tiles, tiles, tile0;      // tiles of 128 of them, and where they start among the call's
 };
-__host__ __device__ inline Keys win_keys(const WinParams &p)
+__host__ __device__ inline void segment_list(Segment &s, uint32_t window, uint32_t sinks)
 {
-    Keys k;
-    const uint64_t first = (uint64_t)p.base + 1, end = (uint64_t)p.base + p.rows;
-    k.lo = (uint32_t)(first > p.window ? first - p.window : 0);
-    k.ns = p.sinks < k.lo ? p.sinks : k.lo;
-    k.sink_tiles = (k.ns + kKeys - 1) / kKeys;
-    k.tiles = k.sink_tiles + (uint32_t)((end - k.lo + kKeys - 1) / kKeys);
-    return k;
+    s.lo = (uint64_t)s.base + 1 > window ? s.base + 1 - window : 0;
+    s.ns = sinks < s.lo ? sinks : s.lo;
+    if (s.ns > s.end) s.ns = s.end;
+    s.sink_tiles = (s.ns + kKeys - 1) / kKeys;
+    s.tiles = s.sink_tiles + (s.end > s.lo ? (s.end - s.lo + kKeys - 1) / kKeys : 0);
 }
-__device__ __forceinline__ uint32_t win_tile_start(const Keys &k, uint32_t tile)
+// What a call's tiles are: one segment (a prefill), or those that win_plan_kernel found in a ragged step.
+struct TilePlan {
+    Segment one;
+    const Segment *segments;                // NULL: one
+    const uint2 *key_tiles, *row_tiles;     // (segment, tile) of each
+    const uint32_t *counts;                 // how many of either
+    uint32_t max_key_tiles, max_row_tiles;
+};
+__device__ __forceinline__ uint32_t win_tile_start(const Segment &s, uint32_t tile)
 {
-    return tile < k.sink_tiles ? tile * kKeys : k.lo + (tile - k.sink_tiles) * kKeys;
+    return tile < s.sink_tiles ? tile * kKeys : s.lo + (tile - s.sink_tiles) * kKeys;
+}
+// positions below it exist in the cache
+__device__ __forceinline__ uint32_t win_end(const WinParams &p, const TilePlan &plan, const Segment &s)
+{
+    return plan.segments ? s.end : min(s.end, p.lengths[0]);
 }
 
 template <typename T> constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
@@ -109,21 +124,29 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo
 // at (c / 8) * rows * 16 + r * 16 + (c % 8) * 2: 128 rows of positions for K, DP rows of dimensions for V.
 // Every element is read once and written once per part: HBM (or L2) bounds it.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) win_pack_kernel(const WinParams p, const Keys keys, unsigned char *tiles, TileHead *heads,
+__global__ void __launch_bounds__(256) win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, TileHead *heads,
                                                        uint32_t kvh0)
 {
     __shared__ uint32_t rows[kKeys], amax_bits, bad_any;
-    const uint32_t tile = blockIdx.x, kvh = kvh0 + blockIdx.y, t = threadIdx.x, D = p.head_dim;
-    const size_t at = (size_t)blockIdx.y * keys.tiles + tile;
+    Segment s = plan.one;
+    uint32_t tile = blockIdx.x;
+    if (plan.segments) {
+        if (blockIdx.x >= plan.counts[0]) return;
+        const uint2 e = plan.key_tiles[blockIdx.x];
+        if (e.x == 0xffffffffu) return;
+        s = plan.segments[e.x];
+        tile = e.y;
+    }
+    const uint32_t kvh = kvh0 + blockIdx.y, t = threadIdx.x, D = p.head_dim;
+    const size_t at = (size_t)blockIdx.y * plan.max_key_tiles + blockIdx.x;
     TileHead &head = heads[at];
     unsigned char *dst = tiles + at * kTileBytes<T, DP> + (blockIdx.z ? kParts<T> * kSlotBytes<T, DP> : 0);
     if (t == 0) { amax_bits = 0; bad_any = 0; }
     if (t < kKeys) {
-        const uint64_t j = (uint64_t)win_tile_start(keys, tile) + t;
-        const uint32_t len = min(p.lengths[0], p.reach);
+        const uint64_t j = (uint64_t)win_tile_start(s, tile) + t;
         uint32_t r = 0xffffffffu;
-        if (j < len && (tile >= keys.sink_tiles || j < keys.ns) && j < (uint64_t)p.base + p.rows)
-            r = win_cache_row(p, p.pages, (uint32_t)j);
+        if (j < win_end(p, plan, s) && (tile >= s.sink_tiles || j < s.ns))
+            r = win_cache_row(p, p.pages ? p.pages + (size_t)s.seq * p.max_pages : nullptr, (uint32_t)j);
         rows[t] = r;
         const uint32_t seen = __ballot_sync(0xffffffffu, r != 0xffffffffu);
         if (blockIdx.z == 0 && (t & 31) == 0) head.seen[t >> 5] = seen;
@@ -252,19 +275,20 @@ __device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t bits)
 
 // The tiles that the rows at positions [pa, pb] see: [0, sinks_end) and [begin, end).
 struct Range { uint32_t sinks_end, begin, end; };
-__device__ __forceinline__ Range win_range(const WinParams &p, const Keys &k, uint64_t pa, uint64_t pb)
+__device__ __forceinline__ Range win_range(const WinParams &p, const Segment &k, uint64_t pa, uint64_t pb)
 {
-    const uint32_t lo = (uint32_t)(pa + 1 > p.window ? pa + 1 - p.window : 0), s = min(p.sinks, lo);
+    const uint32_t lo = (uint32_t)(pa + 1 > p.window ? pa + 1 - p.window : 0), s = min(min(p.sinks, lo), k.end);
     Range r;
     r.sinks_end = s <= k.ns ? (s + kKeys - 1) / kKeys : k.sink_tiles + (s - k.lo + kKeys - 1) / kKeys;
-    r.begin = max(r.sinks_end, k.sink_tiles + (lo - k.lo) / kKeys);
-    r.end = k.sink_tiles + (uint32_t)((pb + 1 - k.lo + kKeys - 1) / kKeys);
+    r.end = (uint32_t)min((uint64_t)k.tiles, k.sink_tiles + (pb + 1 - k.lo + kKeys - 1) / kKeys);
+    r.sinks_end = min(r.sinks_end, r.end);
+    r.begin = min(max(r.sinks_end, k.sink_tiles + (lo - k.lo) / kKeys), r.end);
     return r;
 }
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTileThreads, 1)
-win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, const TileHead *heads, uint32_t kvh0, uint32_t row_tiles)
+win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *tiles, const TileHead *heads, uint32_t kvh0)
 {
     using Smem = TileSmem<T, DP>;
     constexpr uint32_t kSlot = kSlotBytes<T, DP>;
@@ -278,14 +302,23 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
 
     // the rows: tokens x heads of the group; the last tokens, which see most, first
     const uint32_t group = p.q_heads / p.kv_heads, per_tile = kRows / group, D = p.head_dim;
-    const uint32_t kv = blockIdx.x / row_tiles, rt = row_tiles - 1 - blockIdx.x % row_tiles;
-    const uint32_t tok0 = rt * per_tile, tokens = min(per_tile, p.rows - tok0);
-    const uint64_t pa = (uint64_t)p.base + tok0;
+    const uint32_t kv = blockIdx.x / plan.max_row_tiles;
+    Segment keys = plan.one;
+    uint32_t rt = plan.max_row_tiles - 1 - blockIdx.x % plan.max_row_tiles;
+    if (plan.segments) {
+        if (rt >= plan.counts[1]) return;
+        const uint2 e = plan.row_tiles[rt];
+        if (e.x == 0xffffffffu) return;
+        keys = plan.segments[e.x];
+        rt = e.y;
+    }
+    const uint32_t first = rt * per_tile, tok0 = keys.row0 + first, tokens = min(per_tile, keys.rows - first);
+    const uint64_t pa = (uint64_t)keys.base + first;
     const Range range = win_range(p, keys, pa, pa + tokens - 1);
     const uint32_t n = range.sinks_end + (range.end - range.begin);
     const auto tile_of = [&](uint32_t i) { return i < range.sinks_end ? i : range.begin + (i - range.sinks_end); };
-    tiles += (size_t)kv * keys.tiles * kTileBytes<T, DP>;
-    heads += (size_t)kv * keys.tiles;
+    tiles += ((size_t)kv * plan.max_key_tiles + keys.tile0) * kTileBytes<T, DP>;
+    heads += (size_t)kv * plan.max_key_tiles + keys.tile0;
 
     if (warp == kSoftWarps) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sx_smem(tmem_slot)) : "memory");
@@ -297,7 +330,7 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
     }
     // The query rows, scaled, split, stored as the A operand.  A warp takes 16 rows, eight at a time, four lanes to a row:
     // 64 bytes of each of eight rows a load, and stores that meet every bank twice
-    const uint32_t r = tid & (kRows - 1), token = tok0 + r / group;
+    const uint32_t r = tid & (kRows - 1);
     const bool live = r < tokens * group;
     float *row_scale = reinterpret_cast<float *>(smem + Smem::kScale);
     if (warp < kSoftWarps) {
@@ -435,7 +468,7 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
         uint32_t bad = 0;
         const int wg = warp >> 2;
         const uint32_t ts = tmem + wg * 256 + ((uint32_t)(warp & 3) << 21), td = ts + 128;
-        const int64_t pos = (int64_t)p.base + (live ? token : tok0);
+        const int64_t pos = (int64_t)pa + (live ? r / group : 0);
         const int64_t lo_row = pos + 1 > (int64_t)p.window ? pos + 1 - (int64_t)p.window : 0;
         bool ok = true;
 #pragma unroll
@@ -562,7 +595,8 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
         }
         if (live && (__float_as_uint(ml[2 * kRows]) | __float_as_uint(ml[5 * kRows]))) {
             // values that are not finite were left out of the tiles: a row that sees one gets it added
-            const uint64_t end = min((uint64_t)min(p.lengths[0], p.reach), (uint64_t)pos + 1);
+            const uint64_t end = min((uint64_t)win_end(p, plan, keys), (uint64_t)pos + 1);
+            const uint32_t *pages = p.pages ? p.pages + (size_t)keys.seq * p.max_pages : nullptr;
             for (uint32_t i = 0; i < n; i++) {
                 const uint32_t tile = tile_of(i);
                 if (!heads[tile].bad) continue;
@@ -571,7 +605,7 @@ win_tile_kernel(const WinParams p, const Keys keys, const unsigned char *tiles, 
                     if (!((heads[tile].seen[x >> 5] >> (x & 31)) & 1) || j >= end || (pos - (int64_t)j >= (int64_t)p.window && j >= p.sinks))
                         continue;
                     const T *v = static_cast<const T *>(p.v) +
-                                 ((uint64_t)win_cache_row(p, p.pages, (uint32_t)j) * p.kv_heads + kvh0 + kv) * D + wg * (DP / 2);
+                                 ((uint64_t)win_cache_row(p, pages, (uint32_t)j) * p.kv_heads + kvh0 + kv) * D + wg * (DP / 2);
                     for (uint32_t d = 0; d < DP / 2 && wg * (DP / 2) + d < D; d++) {
                         const float y = to_f32(v[d]);
                         if (!(fabsf(y) <= 3.402823466e38f)) mine[d] += y;
@@ -609,46 +643,140 @@ template <typename T, int DP> int tile_prepare(const char *name)
     return rc;
 }
 
+// ------------------------------------------------------------------------------------------------
+// A ragged step: the sequences with at least `from` rows (tokens x heads of a group) become segments, the others are left
+// to the row kernel.  One block; tiled[s] says which they are.
+__global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32_t from, uint32_t max_segments, Segment *segments,
+                                                       uint2 *key_tiles, uint2 *row_tiles, uint32_t *counts, uint32_t max_key_tiles,
+                                                       uint32_t max_row_tiles, uint32_t *tiled)
+{
+    __shared__ uint3 part[8];
+    const uint32_t t = threadIdx.x, lane = t & 31, group = p.q_heads / p.kv_heads, per_tile = kRows / group;
+    uint3 before = make_uint3(0, 0, 0);                  // segments, key tiles, row tiles of the sequences so far
+    for (uint32_t s0 = 0; s0 < p.batch; s0 += 256) {
+        const uint32_t s = s0 + t;
+        Segment g{};
+        uint3 mine = make_uint3(0, 0, 0);
+        if (s < p.batch) {
+            const uint32_t a = p.offsets[s], b = p.offsets[s + 1], len = p.lengths[s];
+            // (a sequence with more tokens than positions has rows of zeros: the row kernel knows)
+            if (b > a && b <= p.rows && (uint64_t)(b - a) * group >= from && len >= b - a) {
+                g.row0 = a; g.rows = b - a; g.base = len - (b - a); g.seq = s;
+                g.end = min(len, p.reach);
+                segment_list(g, p.window, p.sinks);
+                mine = make_uint3(1, g.tiles, (g.rows + per_tile - 1) / per_tile);
+            }
+        }
+        uint3 sum = mine;                                // inclusive scan over the warp, then over the warps
+#pragma unroll
+        for (int w = 1; w < 32; w *= 2) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, sum.x, w), y = __shfl_up_sync(0xffffffffu, sum.y, w),
+                           z = __shfl_up_sync(0xffffffffu, sum.z, w);
+            if (lane >= (uint32_t)w) { sum.x += x; sum.y += y; sum.z += z; }
+        }
+        if (lane == 31) part[t >> 5] = sum;
+        __syncthreads();
+        uint3 at = before;
+        for (uint32_t w = 0; w < 8; w++) {
+            if (w < t >> 5) { at.x += part[w].x; at.y += part[w].y; at.z += part[w].z; }
+            before.x += part[w].x; before.y += part[w].y; before.z += part[w].z;
+        }
+        at.x += sum.x - mine.x; at.y += sum.y - mine.y; at.z += sum.z - mine.z;
+        // (the host's bounds hold for any offsets that ascend; what passes them all the same goes row by row)
+        const bool fits = mine.x && at.x < max_segments && (uint64_t)at.y + mine.y <= max_key_tiles && (uint64_t)at.z + mine.z <= max_row_tiles;
+        if (s < p.batch) tiled[s] = fits;
+        if (fits) {
+            g.tile0 = at.y;
+            segments[at.x] = g;
+            for (uint32_t i = 0; i < mine.y; i++) key_tiles[at.y + i] = make_uint2(at.x, i);
+            for (uint32_t i = 0; i < mine.z; i++) row_tiles[at.z + i] = make_uint2(at.x, i);
+        } else if (mine.x) {
+            // nobody's tiles in between
+            for (uint32_t i = at.y; i < max_key_tiles && i - at.y < mine.y; i++) key_tiles[i] = make_uint2(0xffffffffu, 0);
+            for (uint32_t i = at.z; i < max_row_tiles && i - at.z < mine.z; i++) row_tiles[i] = make_uint2(0xffffffffu, 0);
+        }
+        __syncthreads();
+    }
+    if (t == 0) { counts[0] = min(before.y, max_key_tiles); counts[1] = min(before.z, max_row_tiles); }
+}
+
 constexpr uint64_t kPassBytes = 1ull << 30;              // tiles of one pass over KV heads
 
-template <typename T, int DP> int run_tiles(Launch &l, const WinParams &p, const char *name)
+template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char *name)
 {
     static_assert(TileSmem<T, DP>::kBytes <= 232448, "shared memory of a CTA");
-    static_assert(kRows * (DP + 4) * 4 + 6 * kRows * 4 <= TileSmem<T, DP>::kBars, "the parts of both groups fit where the operands were");
-    const Keys keys = win_keys(p);
-    const uint64_t per_head = (uint64_t)keys.tiles * kTileBytes<T, DP>;
+    static_assert(kRows * (DP + 4) * 4 + 6 * kRows * 4 <= TileSmem<T, DP>::kBars, "the parts of all groups fit where the operands were");
+    const uint32_t group = p.q_heads / p.kv_heads, per_tile = kRows / group;
+    const bool ragged = p.form == kRaggedStep;
+    TilePlan plan{};
+    uint64_t key_tiles, row_tiles, segments = 0;
+    if (ragged) {
+        // at most: a segment has kTileFrom rows; its list ends in two unfilled tiles, its rows in one
+        segments = std::min<uint64_t>(p.batch, (uint64_t)p.rows * group / kTileFrom);
+        key_tiles = segments * ((uint64_t)std::min(p.sinks, p.reach) / kKeys + std::min<uint64_t>(p.window, p.reach) / kKeys + 3) + p.rows / kKeys;
+        row_tiles = segments + p.rows / per_tile;
+    } else {
+        plan.one.rows = p.rows;
+        plan.one.base = p.base;
+        plan.one.end = (uint32_t)std::min<uint64_t>((uint64_t)p.base + p.rows, p.reach);
+        segment_list(plan.one, p.window, p.sinks);
+        key_tiles = plan.one.tiles;
+        row_tiles = (p.rows + per_tile - 1) / per_tile;
+    }
+    const uint64_t per_head = std::max<uint64_t>(1, key_tiles) * kTileBytes<T, DP>;
     const uint32_t pass = (uint32_t)std::min<uint64_t>(p.kv_heads, std::max<uint64_t>(1, kPassBytes / per_head));
-    const uint64_t head_bytes = align_up((size_t)pass * keys.tiles * sizeof(TileHead), 256);
-    l.ws_need = (size_t)(head_bytes + pass * per_head);
+    const size_t head_bytes = align_up((size_t)(pass * key_tiles) * sizeof(TileHead), 256);
+    const size_t seg_bytes = align_up((size_t)segments * sizeof(Segment), 256), key_bytes = ragged ? align_up((size_t)key_tiles * 8, 256) : 0;
+    const size_t row_bytes = ragged ? align_up((size_t)row_tiles * 8, 256) : 0, flag_bytes = ragged ? align_up((size_t)p.batch * 4 + 8, 256) : 0;
+    l.ws_need = seg_bytes + key_bytes + row_bytes + flag_bytes + head_bytes + (size_t)(pass * per_head);
+    if (row_tiles * pass > 0x7fffffffull || key_tiles > 0x7fffffffull || pass > 65535)
+        return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
     if (l.query_ws) return AB_OK;
     if (l.ws_need > l.ws_bytes || !l.ws)
         return fail(AB_ERR_INVALID, "%s: needs %zu bytes of workspace, given %zu", name, l.ws_need, l.ws_bytes);
-    const uint32_t per_tile = kRows / (p.q_heads / p.kv_heads), row_tiles = (p.rows + per_tile - 1) / per_tile;
-    if ((uint64_t)row_tiles * pass > 0x7fffffffull || keys.tiles > 0x7fffffffu || pass > 65535)
-        return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
     int rc = tile_prepare<T, DP>(name);
     if (rc) return rc;
-    TileHead *heads = static_cast<TileHead *>(l.ws);
-    unsigned char *tiles = static_cast<unsigned char *>(l.ws) + head_bytes;
-    for (uint32_t h = 0; h < p.kv_heads; h += pass) {
-        const uint32_t now = std::min(pass, p.kv_heads - h);
-        win_pack_kernel<T, DP><<<dim3(keys.tiles, now, 2), 256, 0, l.stream>>>(p, keys, tiles, heads, h);
-        count_launch();
-        rc = check_cuda(cudaGetLastError(), name);
-        if (rc) return rc;
-        win_tile_kernel<T, DP><<<row_tiles * now, kTileThreads, TileSmem<T, DP>::kBytes, l.stream>>>(p, keys, tiles, heads, h, row_tiles);
+    unsigned char *ws = static_cast<unsigned char *>(l.ws);
+    plan.max_key_tiles = (uint32_t)key_tiles;
+    plan.max_row_tiles = (uint32_t)row_tiles;
+    if (ragged) {
+        Segment *segs = reinterpret_cast<Segment *>(ws);
+        uint2 *kt = reinterpret_cast<uint2 *>(ws + seg_bytes), *rt = reinterpret_cast<uint2 *>(ws + seg_bytes + key_bytes);
+        uint32_t *counts = reinterpret_cast<uint32_t *>(ws + seg_bytes + key_bytes + row_bytes);
+        plan.segments = segs;
+        plan.key_tiles = kt;
+        plan.row_tiles = rt;
+        plan.counts = counts;
+        p.tiled = counts + 2;
+        win_plan_kernel<<<1, 256, 0, l.stream>>>(p, kTileFrom, (uint32_t)segments, segs, kt, rt, counts, plan.max_key_tiles,
+                                                 plan.max_row_tiles, counts + 2);
         count_launch();
         rc = check_cuda(cudaGetLastError(), name);
         if (rc) return rc;
     }
-    note_selection("%s: tcgen05 tiles, %u positions packed, %u x %u CTAs of 128 rows, %u pass(es)", name,
-                   keys.tiles * (uint32_t)kKeys, row_tiles, pass, (p.kv_heads + pass - 1) / pass);
+    TileHead *heads = reinterpret_cast<TileHead *>(ws + seg_bytes + key_bytes + row_bytes + flag_bytes);
+    unsigned char *tiles = reinterpret_cast<unsigned char *>(heads) + head_bytes;
+    for (uint32_t h = 0; h < p.kv_heads && row_tiles; h += pass) {
+        const uint32_t now = std::min(pass, p.kv_heads - h);
+        if (key_tiles) {
+            win_pack_kernel<T, DP><<<dim3((uint32_t)key_tiles, now, 2), 256, 0, l.stream>>>(p, plan, tiles, heads, h);
+            count_launch();
+            rc = check_cuda(cudaGetLastError(), name);
+            if (rc) return rc;
+        }
+        win_tile_kernel<T, DP><<<(uint32_t)row_tiles * now, kTileThreads, TileSmem<T, DP>::kBytes, l.stream>>>(p, plan, tiles, heads, h);
+        count_launch();
+        rc = check_cuda(cudaGetLastError(), name);
+        if (rc) return rc;
+    }
+    note_selection("%s: tcgen05 tiles, up to %u tiles of 128 positions and %u of 128 rows, %u pass(es)", name, plan.max_key_tiles,
+                   plan.max_row_tiles, (p.kv_heads + pass - 1) / pass);
     return AB_OK;
 }
 
 }  // namespace
 
-int run_window_tiles(Launch &l, const WinParams &p, bool f16, const char *name)
+int run_window_tiles(Launch &l, WinParams &p, bool f16, const char *name)
 {
     if (f16) return p.head_dim <= 64 ? run_tiles<__half, 64>(l, p, name) : run_tiles<__half, 128>(l, p, name);
     return p.head_dim <= 64 ? run_tiles<float, 64>(l, p, name) : run_tiles<float, 128>(l, p, name);

@@ -274,7 +274,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
             b = [q, k, v] + [_aligned(t) for t in (pages, opts.lengths, offsets) if t is not None] + [out]
             rt.launch_own("AttentionWindow" + form + ("F16" if f16 else ""), b,
                           rt.window_dims(batch, q_heads, kv_heads, head_dim, opts.block, max_pages, scale, opts.window,
-                                         opts.sinks, k.shape[0], rows, base), scratch=prefill)
+                                         opts.sinks, k.shape[0], rows, base), scratch=prefill or ragged)
         return out
 
     if prefill:

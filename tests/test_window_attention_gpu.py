@@ -314,3 +314,67 @@ def test_no_wait_ran_out():
     rt.attention_error()
     _job(9, 3)()
     assert "tcgen05 tiles" not in rt.last_selection()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("qH,kv,D,block", [(8, 2, 128, 16), (6, 2, 40, 5), (2, 2, 64, 8), (30, 1, 128, 16)])
+def test_ragged_steps_of_chunks_and_tokens(qH, kv, D, block, f16):
+    # prompts' chunks (on tiles) between single tokens (row by row), in more than one block of the plan; sequences without
+    # tokens, with one position, with fewer positions than tokens; padding rows behind the last
+    rng = np.random.default_rng(11)
+    batch = 300
+    counts = np.where(rng.random(batch) < 0.05, rng.integers(64, 200, batch), rng.integers(0, 3, batch))
+    counts[[0, 255, 256, 299]] = (130, 64, 70, 129)
+    lengths = counts + rng.integers(0, 300, batch) * (rng.random(batch) < 0.8)
+    lengths[7], counts[7] = 3, 5                                  # two rows have no position: zeros
+    lengths[8], counts[8] = 60, 100
+    lengths = np.maximum(lengths, 1)
+    for window, sinks in ((90, 5), (1, 0), (5000, 3)):
+        first = np.maximum(lengths - np.maximum(counts, 1), 0)
+        c = Cache(window, kv, D, block, lengths.tolist(), first.tolist(), window, sinks, f16)
+        tokens = int(counts.sum()) + 3
+        q = rng.standard_normal((tokens, qH, D)).astype(np.float32)
+        got = T.attention(dev(q), dev(c.pk), dev(c.pv), T.AttentionOptions(
+            lengths=dev(lengths.astype(np.uint32)), pages=dev(c.pages), block=block, scale=attn_scale(D),
+            query_extents=dev(counts.astype(np.uint32)), window=window, sinks=sinks)).cpu().numpy()
+        assert not got[-3:].any()
+        r = 0
+        for b, (n, m) in enumerate(zip(lengths.tolist(), counts.tolist())):
+            if b not in (0, 1, 7, 8, 255, 256, 299) and m < 64 and b % 9:
+                r += m
+                continue
+            for i in range(m):
+                if n - m + i < 0:
+                    assert not got[r].any()
+                elif i % 7 == 0 or i == m - 1:
+                    check(got[r], *attend(q[r], c.k[b], c.v[b], visible(n - m + i, n, window, sinks), attn_scale(D), qH // kv),
+                          f"sequence {b} token {i} window {window}")
+                r += 1
+
+
+def test_ragged_chunks_in_graphs_on_two_streams():
+    def job(seed):
+        rng = np.random.default_rng(seed)
+        counts, lengths = [70, 1, 200, 3], [300, 41, 200, 9]
+        c = Cache(seed, 2, 128, 16, lengths, [n - m for n, m in zip(lengths, counts)], 100, 4, False)
+        q, k, v = dev(rng.standard_normal((sum(counts), 8, 128)).astype(np.float32)), dev(c.pk), dev(c.pv)
+        o = T.AttentionOptions(lengths=dev(np.array(lengths, np.uint32)), pages=dev(c.pages), block=16, scale=0.1,
+                               query_extents=dev(np.array(counts, np.uint32)), window=100, sinks=4)
+        return lambda: T.attention(q, k, v, o)
+
+    jobs = [job(1), job(2)]
+    want = [j().cpu() for j in jobs]
+    graphs, outs = [], []
+    for j in jobs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(j())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o.cpu(), w) for o, w in zip(outs, want))
