@@ -16,7 +16,7 @@ struct WinParams {
     uint32_t reach;                                // positions the page table (or the cache) addresses
     uint32_t capacity;                             // rows of the cache
     uint32_t base;
-    const uint32_t *tiled;                         // a ragged step: nonzero for the sequences whose rows went on tiles; or NULL
+    const uint32_t *left;                          // a ragged step some of whose rows went on tiles: how many did not, and which; or NULL
     float scale_log2;                              // Scale * log2(e)
     int form;
 };
@@ -36,7 +36,7 @@ __device__ __forceinline__ uint32_t win_cache_row(const WinParams &p, const uint
 
 // query rows (tokens x heads of a KV head) of one sequence from which 128-row tiles take over
 constexpr uint32_t kTileFrom = 64;
-// a prefill, or the sequences of a ragged step that have that many rows (it then sets p.tiled), on 128-row tiles
+// a prefill, or the sequences of a ragged step that have that many rows (it then sets p.left), on 128-row tiles
 // (window_prefill.cu); p.q_heads / p.kv_heads <= 128
 int run_window_tiles(Launch &l, WinParams &p, bool f16, const char *name);
 int window_error_flag();

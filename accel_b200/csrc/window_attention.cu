@@ -36,12 +36,11 @@ struct WinView {
     const uint32_t *pages;
     uint32_t lo, ns, n;
     bool zero;                                     // a ragged padding row: written as zeros
-    bool skip;                                     // a row of a sequence that went on tiles: not written here
 };
 
 __device__ __forceinline__ WinView win_view(const WinParams &p, uint32_t row)
 {
-    WinView w{p.pages, 0, 0, 0, false, false};
+    WinView w{p.pages, 0, 0, 0, false};
     uint64_t pos1;                                 // the row's position + 1
     uint32_t len;
     if (p.form == kRaggedStep) {
@@ -52,7 +51,6 @@ __device__ __forceinline__ WinView win_view(const WinParams &p, uint32_t row)
             if (p.offsets[m + 1] <= row) a = m + 1; else b = m;
         }
         if (a >= p.batch) { w.zero = true; return w; }
-        if (p.tiled && p.tiled[a]) { w.skip = true; return w; }
         const uint32_t i = row - p.offsets[a], n = p.offsets[a + 1] - p.offsets[a];
         len = p.lengths[a];
         if ((uint64_t)len + i < n) { w.zero = true; return w; }
@@ -75,6 +73,10 @@ __device__ __forceinline__ WinView win_view(const WinParams &p, uint32_t row)
     w.n = w.ns + (hi > w.lo ? hi - w.lo : 0u);
     return w;
 }
+
+// The rows of a launch: all of the call's, or those that are left beside tiles.
+__device__ __forceinline__ uint32_t win_rows(const WinParams &p) { return p.left ? p.left[0] : p.rows; }
+__device__ __forceinline__ uint32_t win_row_of(const WinParams &p, uint32_t turn) { return p.left ? p.left[1 + turn] : turn; }
 
 // The list's entry i: its position; the page that holds it (loaded now, looked at later: a page's number is asked for
 // two tiles ahead of its rows, so that nothing waits for the table); its cache row, 0xffffffff where that page lies outside
@@ -402,14 +404,15 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
     using Math = RowMath<T, DP>;
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t row = blockIdx.x / parts, part = blockIdx.x % parts;
+    const uint32_t part = blockIdx.x % parts;
     const uint32_t D = p.head_dim, group = p.q_heads / p.kv_heads, per_kv = (group + 7) / 8;
     const uint32_t kvh = blockIdx.y / per_kv, h0 = kvh * group + (blockIdx.y % per_kv) * 8;
     const uint32_t heads = min(8u, (kvh + 1) * group - h0);
     const uint32_t tile_k = (uint32_t)__cvta_generic_to_shared(smem) + warp * Tile::kWarpBytes, tile_v = tile_k + Tile::kBytesK;
 
+    for (uint32_t turn = blockIdx.x / parts; turn < win_rows(p); turn += gridDim.x / parts) {
+    const uint32_t row = win_row_of(p, turn);
     const WinView w = win_view(p, row);
-    if (w.skip) return;
     const uint32_t n_tiles = (w.n + kTile - 1) / kTile, step = parts * kRowWarps;
     uint32_t tile = part * kRowWarps + warp;
 
@@ -521,6 +524,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
 #pragma unroll
         for (int e = 0; e < 4; e++) part_o[(warp * 8 + 2 * t + (e & 1)) * DP + Math::dim(i, e, g)] = o[i][e];
     join_parts<kRowWarps, 8, DP>(p, part_ml, part_o, row, h0, heads, part, parts, w.zero);
+    __syncthreads();                                                // (the next turn's rows go where the parts are)
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -549,10 +554,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) win_lanes_kernel(const WinP
     static_assert((kPart + 1) * G * (DP + 2) * 4 <= kLanesSmem, "the parts fit where the rows were");
     float *smem = reinterpret_cast<float *>(smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LR, ll = lane % LR;
-    const uint32_t row = blockIdx.x / parts, part = blockIdx.x % parts, kvh = blockIdx.y, h0 = kvh * G, D = p.head_dim;
+    const uint32_t part = blockIdx.x % parts, kvh = blockIdx.y, h0 = kvh * G, D = p.head_dim;
     const bool on = (uint32_t)ll * 4 < D;
+    for (uint32_t turn = blockIdx.x / parts; turn < win_rows(p); turn += gridDim.x / parts) {
+    const uint32_t row = win_row_of(p, turn);
     const WinView w = win_view(p, row);
-    if (w.skip) return;
     const uint32_t n_batches = (w.n + 7) / 8, step = parts * kPart;
     // lanes 0..7 of a group: its eight positions (past the last batch there is nothing to see)
     const auto page_of = [&](uint32_t b) { return win_page(p, w, (b + sub) * 8 + (ll & 7)); };
@@ -655,6 +661,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) win_lanes_kernel(const WinP
         *reinterpret_cast<float4 *>(part_o + (unit * G + h) * DP + ll * 4) = o[h];
     }
     join_parts<kPart, G, DP>(p, part_ml, part_o, row, h0, G, part, parts, w.zero);
+    __syncthreads();
+    }
 }
 
 // a kernel's shared memory and clusters of 16 CTAs, beyond what it gets unasked: once per device (`done`: a bit for each)
@@ -678,8 +686,8 @@ int prepare(void (*kernel)(const WinParams, const uint32_t), size_t bytes, uint6
 int launch_split(Launch &l, const WinParams &p, void (*kernel)(const WinParams, const uint32_t), uint32_t groups, uint32_t resident,
                  uint32_t unit, size_t smem, const char *how, const char *name)
 {
-    // (beside tiles, the rows left are mostly one of each sequence)
-    const uint64_t rows = p.tiled ? std::min(p.rows, 2 * p.batch) : p.rows;
+    // (beside tiles, the rows left are mostly one of each sequence; the device knows how many)
+    const uint64_t rows = p.left ? std::min(p.rows, p.batch) : p.rows;
     const uint64_t longest = std::min<uint64_t>((uint64_t)p.window + p.sinks, p.reach), places = (uint64_t)resident * sm_count();
     uint32_t parts = 1;
     uint64_t least = ~0ull;
@@ -688,10 +696,11 @@ int launch_split(Launch &l, const WinParams &p, void (*kernel)(const WinParams, 
         const uint64_t cost = rounds * (8 * (steps + 3) + n);
         if (cost < least) { least = cost; parts = n; }
     }
-    if ((uint64_t)p.rows * parts > 0x7fffffffull || groups > 65535)
+    const uint64_t turns = p.left ? std::min<uint64_t>(p.rows, std::max<uint64_t>(rows, 2 * places / ((uint64_t)groups * parts) + 1)) : rows;
+    if (turns * parts > 0x7fffffffull || groups > 65535)
         return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.rows * parts, groups);
+    cfg.gridDim = dim3((uint32_t)turns * parts, groups);
     cfg.blockDim = dim3(kRowWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = l.stream;

@@ -123,8 +123,9 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo
 // grid (tiles, KV heads of this pass, 2): K or V of one tile.  An operand's element (r, c), c along the contraction, lies
 // at (c / 8) * rows * 16 + r * 16 + (c % 8) * 2: 128 rows of positions for K, DP rows of dimensions for V.
 // Every element is read once and written once per part: HBM (or L2) bounds it.
+constexpr int kPackThreads = 512;
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, TileHead *heads,
+__global__ void __launch_bounds__(kPackThreads, 2) win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, TileHead *heads,
                                                        uint32_t kvh0)
 {
     __shared__ uint32_t rows[kKeys], amax_bits, bad_any;
@@ -152,13 +153,13 @@ __global__ void __launch_bounds__(256) win_pack_kernel(const WinParams p, const 
         if (blockIdx.z == 0 && (t & 31) == 0) head.seen[t >> 5] = seen;
     }
     __syncthreads();
-    constexpr int kEach = kKeys * DP / 256;              // elements of a thread
+    constexpr int kEach = kKeys * DP / kPackThreads, kTogether = kPackThreads / DP;              // elements of a thread
     float x[kEach];
     float big = 0.f;
     bool bad = false;
-    // K: a thread holds half the dimensions of a position; V: eight positions of a dimension at a time, neighbouring threads
+    // K: a thread holds a quarter of the dimensions of a position; V: eight positions of a dimension at a time, neighbouring threads
     // neighbouring dimensions
-    const uint32_t key = t & (kKeys - 1), d0 = (t >> 7) * (DP / 2), dim = t & (DP - 1), group0 = t / DP;
+    const uint32_t key = t & (kKeys - 1), d0 = (t >> 7) * kEach, dim = t & (DP - 1), group0 = t / DP;
     if (blockIdx.z == 0) {
         const T *src = static_cast<const T *>(p.k) + ((uint64_t)(rows[key] == 0xffffffffu ? 0 : rows[key]) * p.kv_heads + kvh) * D;
         const bool on = rows[key] != 0xffffffffu;
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(256) win_pack_kernel(const WinParams p, const 
         const T *v = static_cast<const T *>(p.v);
 #pragma unroll
         for (int i = 0; i < kEach; i++) {
-            const uint32_t r = rows[(i / 8 * (256 / DP) + group0) * 8 + (i & 7)];
+            const uint32_t r = rows[(i / 8 * kTogether + group0) * 8 + (i & 7)];
             x[i] = r != 0xffffffffu && dim < D ? to_f32(v[((uint64_t)r * p.kv_heads + kvh) * D + dim]) : 0.f;
         }
     }
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(256) win_pack_kernel(const WinParams p, const 
         for (int n = 0; n < 8; n++) y[n] = x[i + n] * f;
         uint4 hi, lo;
         split8(y, hi, lo);
-        const uint32_t to = blockIdx.z ? (i / 8 * (256 / DP) + group0) * (DP * 16) + dim * 16 : (d0 + i) / 8 * (kKeys * 16) + key * 16;
+        const uint32_t to = blockIdx.z ? (i / 8 * kTogether + group0) * (DP * 16) + dim * 16 : (d0 + i) / 8 * (kKeys * 16) + key * 16;
         *reinterpret_cast<uint4 *>(dst + to) = hi;
         if (kParts<T> == 2) *reinterpret_cast<uint4 *>(dst + kSlotBytes<T, DP> + to) = lo;
     }
@@ -644,59 +645,63 @@ template <typename T, int DP> int tile_prepare(const char *name)
 }
 
 // ------------------------------------------------------------------------------------------------
-// A ragged step: the sequences with at least `from` rows (tokens x heads of a group) become segments, the others are left
-// to the row kernel.  One block; tiled[s] says which they are.
+// A ragged step: the sequences with at least `from` rows (tokens x heads of a group) become segments, the rows of the
+// others, and those behind the last sequence, are left to the row kernel: left[0] of them, listed behind.  One block.
 __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32_t from, uint32_t max_segments, Segment *segments,
                                                        uint2 *key_tiles, uint2 *row_tiles, uint32_t *counts, uint32_t max_key_tiles,
-                                                       uint32_t max_row_tiles, uint32_t *tiled)
+                                                       uint32_t max_row_tiles, uint32_t *left)
 {
-    __shared__ uint3 part[8];
+    __shared__ uint4 part[8];
     const uint32_t t = threadIdx.x, lane = t & 31, group = p.q_heads / p.kv_heads, per_tile = kRows / group;
-    uint3 before = make_uint3(0, 0, 0);                  // segments, key tiles, row tiles of the sequences so far
+    uint4 before = make_uint4(0, 0, 0, 0);               // segments, key tiles, row tiles, rows left of the sequences so far
     for (uint32_t s0 = 0; s0 < p.batch; s0 += 256) {
         const uint32_t s = s0 + t;
         Segment g{};
-        uint3 mine = make_uint3(0, 0, 0);
+        uint4 mine = make_uint4(0, 0, 0, 0);
+        uint32_t first = 0;
         if (s < p.batch) {
-            const uint32_t a = p.offsets[s], b = p.offsets[s + 1], len = p.lengths[s];
+            const uint32_t a = min(p.offsets[s], p.rows), b = min(p.offsets[s + 1], p.rows), len = p.lengths[s];
+            first = a;
+            mine.w = b > a ? b - a : 0;
             // (a sequence with more tokens than positions has rows of zeros: the row kernel knows)
-            if (b > a && b <= p.rows && (uint64_t)(b - a) * group >= from && len >= b - a) {
+            if (b > a && b == p.offsets[s + 1] && (uint64_t)(b - a) * group >= from && len >= b - a) {
                 g.row0 = a; g.rows = b - a; g.base = len - (b - a); g.seq = s;
                 g.end = min(len, p.reach);
                 segment_list(g, p.window, p.sinks);
-                mine = make_uint3(1, g.tiles, (g.rows + per_tile - 1) / per_tile);
+                mine = make_uint4(1, g.tiles, (g.rows + per_tile - 1) / per_tile, 0);
             }
         }
-        uint3 sum = mine;                                // inclusive scan over the warp, then over the warps
+        uint4 sum = mine;                                // inclusive scan over the warp, then over the warps
 #pragma unroll
         for (int w = 1; w < 32; w *= 2) {
             const uint32_t x = __shfl_up_sync(0xffffffffu, sum.x, w), y = __shfl_up_sync(0xffffffffu, sum.y, w),
-                           z = __shfl_up_sync(0xffffffffu, sum.z, w);
-            if (lane >= (uint32_t)w) { sum.x += x; sum.y += y; sum.z += z; }
+                           z = __shfl_up_sync(0xffffffffu, sum.z, w), u = __shfl_up_sync(0xffffffffu, sum.w, w);
+            if (lane >= (uint32_t)w) { sum.x += x; sum.y += y; sum.z += z; sum.w += u; }
         }
         if (lane == 31) part[t >> 5] = sum;
         __syncthreads();
-        uint3 at = before;
+        uint4 at = before;
         for (uint32_t w = 0; w < 8; w++) {
-            if (w < t >> 5) { at.x += part[w].x; at.y += part[w].y; at.z += part[w].z; }
-            before.x += part[w].x; before.y += part[w].y; before.z += part[w].z;
+            if (w < t >> 5) { at.x += part[w].x; at.y += part[w].y; at.z += part[w].z; at.w += part[w].w; }
+            before.x += part[w].x; before.y += part[w].y; before.z += part[w].z; before.w += part[w].w;
         }
-        at.x += sum.x - mine.x; at.y += sum.y - mine.y; at.z += sum.z - mine.z;
-        // (the host's bounds hold for any offsets that ascend; what passes them all the same goes row by row)
-        const bool fits = mine.x && at.x < max_segments && (uint64_t)at.y + mine.y <= max_key_tiles && (uint64_t)at.z + mine.z <= max_row_tiles;
-        if (s < p.batch) tiled[s] = fits;
-        if (fits) {
+        at.x += sum.x - mine.x; at.y += sum.y - mine.y; at.z += sum.z - mine.z; at.w += sum.w - mine.w;
+        // (the host's bounds hold for all offsets that ascend, as a prefix sum's do; with others no tile is given away twice)
+        if (mine.x && at.x < max_segments && (uint64_t)at.y + mine.y <= max_key_tiles && (uint64_t)at.z + mine.z <= max_row_tiles) {
             g.tile0 = at.y;
             segments[at.x] = g;
             for (uint32_t i = 0; i < mine.y; i++) key_tiles[at.y + i] = make_uint2(at.x, i);
             for (uint32_t i = 0; i < mine.z; i++) row_tiles[at.z + i] = make_uint2(at.x, i);
         } else if (mine.x) {
-            // nobody's tiles in between
             for (uint32_t i = at.y; i < max_key_tiles && i - at.y < mine.y; i++) key_tiles[i] = make_uint2(0xffffffffu, 0);
             for (uint32_t i = at.z; i < max_row_tiles && i - at.z < mine.z; i++) row_tiles[i] = make_uint2(0xffffffffu, 0);
         }
+        for (uint32_t i = 0; i < mine.w && at.w + i < p.rows; i++) left[1 + at.w + i] = first + i;
         __syncthreads();
     }
+    const uint32_t end = min(p.offsets[p.batch], p.rows);
+    for (uint32_t i = end + t; i < p.rows && before.w + (i - end) < p.rows; i += 256) left[1 + before.w + (i - end)] = i;
+    if (t == 0) left[0] = min(before.w + (p.rows - end), p.rows);
     if (t == 0) { counts[0] = min(before.y, max_key_tiles); counts[1] = min(before.z, max_row_tiles); }
 }
 
@@ -727,7 +732,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
     const uint32_t pass = (uint32_t)std::min<uint64_t>(p.kv_heads, std::max<uint64_t>(1, kPassBytes / per_head));
     const size_t head_bytes = align_up((size_t)(pass * key_tiles) * sizeof(TileHead), 256);
     const size_t seg_bytes = align_up((size_t)segments * sizeof(Segment), 256), key_bytes = ragged ? align_up((size_t)key_tiles * 8, 256) : 0;
-    const size_t row_bytes = ragged ? align_up((size_t)row_tiles * 8, 256) : 0, flag_bytes = ragged ? align_up((size_t)p.batch * 4 + 8, 256) : 0;
+    const size_t row_bytes = ragged ? align_up((size_t)row_tiles * 8, 256) : 0, flag_bytes = ragged ? align_up((size_t)p.rows * 4 + 12, 256) : 0;
     l.ws_need = seg_bytes + key_bytes + row_bytes + flag_bytes + head_bytes + (size_t)(pass * per_head);
     if (row_tiles * pass > 0x7fffffffull || key_tiles > 0x7fffffffull || pass > 65535)
         return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
@@ -747,7 +752,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
         plan.key_tiles = kt;
         plan.row_tiles = rt;
         plan.counts = counts;
-        p.tiled = counts + 2;
+        p.left = counts + 2;
         win_plan_kernel<<<1, 256, 0, l.stream>>>(p, kTileFrom, (uint32_t)segments, segs, kt, rt, counts, plan.max_key_tiles,
                                                  plan.max_row_tiles, counts + 2);
         count_launch();
@@ -759,7 +764,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
     for (uint32_t h = 0; h < p.kv_heads && row_tiles; h += pass) {
         const uint32_t now = std::min(pass, p.kv_heads - h);
         if (key_tiles) {
-            win_pack_kernel<T, DP><<<dim3((uint32_t)key_tiles, now, 2), 256, 0, l.stream>>>(p, plan, tiles, heads, h);
+            win_pack_kernel<T, DP><<<dim3((uint32_t)key_tiles, now, 2), kPackThreads, 0, l.stream>>>(p, plan, tiles, heads, h);
             count_launch();
             rc = check_cuda(cudaGetLastError(), name);
             if (rc) return rc;
