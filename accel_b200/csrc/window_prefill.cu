@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(kPackThreads, 2) win_pack_kernel(const WinPara
                                                        uint32_t kvh0)
 {
     __shared__ uint32_t rows[kKeys], amax_bits, bad_any;
+    pdl_trigger();                                       // the tile kernel may set itself up meanwhile
     Segment s = plan.one;
     uint32_t tile = blockIdx.x;
     if (plan.segments) {
@@ -157,20 +158,27 @@ __global__ void __launch_bounds__(kPackThreads, 2) win_pack_kernel(const WinPara
     float x[kEach];
     float big = 0.f;
     bool bad = false;
-    // K: a thread holds a quarter of the dimensions of a position; V: eight positions of a dimension at a time, neighbouring threads
-    // neighbouring dimensions
-    const uint32_t key = t & (kKeys - 1), d0 = (t >> 7) * kEach, dim = t & (DP - 1), group0 = t / DP;
+    // K: eight dimensions of a position at a time; a warp takes eight positions x 32 dimensions, whole lines to read and to
+    // write.  V: eight positions of a dimension at a time, neighbouring threads neighbouring dimensions.
+    const uint32_t lane = t & 31, dim = t & (DP - 1), group0 = t / DP;
+    const auto k_task = [&](int i, uint32_t &key, uint32_t &d) {
+        const uint32_t task = (i / 8) * (kPackThreads / 32) + (t >> 5);            // of 16 x DP / 32
+        key = task / (DP / 32) * 8 + (lane & 7);
+        d = task % (DP / 32) * 32 + (lane >> 3) * 8;
+    };
     if (blockIdx.z == 0) {
-        const T *src = static_cast<const T *>(p.k) + ((uint64_t)(rows[key] == 0xffffffffu ? 0 : rows[key]) * p.kv_heads + kvh) * D;
-        const bool on = rows[key] != 0xffffffffu;
 #pragma unroll
         for (int i = 0; i < kEach; i += 8) {
+            uint32_t key, d;
+            k_task(i, key, d);
+            const uint32_t r = rows[key];
 #pragma unroll
             for (int e = 0; e < 8; e++) x[i + e] = 0.f;
-            if (on && d0 + i < D) {
+            if (r != 0xffffffffu && d < D) {
+                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.k) + ((uint64_t)r * p.kv_heads + kvh) * D + d);
                 uint4 raw[sizeof(T) / 2];
 #pragma unroll
-                for (int r = 0; r < (int)sizeof(T) / 2; r++) raw[r] = __ldg(reinterpret_cast<const uint4 *>(src + d0 + i) + r);
+                for (int n = 0; n < (int)sizeof(T) / 2; n++) raw[n] = __ldg(src + n);
 #pragma unroll
                 for (int e = 0; e < 8; e++) x[i + e] = to_f32(reinterpret_cast<const T *>(raw)[e]);
             }
@@ -211,7 +219,12 @@ __global__ void __launch_bounds__(kPackThreads, 2) win_pack_kernel(const WinPara
         for (int n = 0; n < 8; n++) y[n] = x[i + n] * f;
         uint4 hi, lo;
         split8(y, hi, lo);
-        const uint32_t to = blockIdx.z ? (i / 8 * kTogether + group0) * (DP * 16) + dim * 16 : (d0 + i) / 8 * (kKeys * 16) + key * 16;
+        uint32_t to = (i / 8 * kTogether + group0) * (DP * 16) + dim * 16;
+        if (blockIdx.z == 0) {
+            uint32_t key, d;
+            k_task(i, key, d);
+            to = d / 8 * (kKeys * 16) + key * 16;
+        }
         *reinterpret_cast<uint4 *>(dst + to) = hi;
         if (kParts<T> == 2) *reinterpret_cast<uint4 *>(dst + kSlotBytes<T, DP> + to) = lo;
     }
@@ -373,6 +386,7 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
+    pdl_wait();                                          // the tiles are packed
     // 168 registers a thread at launch; the softmax groups take what the other four warps do not need:
     // 2 x 128 x 224 + 128 x 56 = 384 x 168
     if (warp >= kSoftWarps) {
@@ -769,9 +783,22 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
             rc = check_cuda(cudaGetLastError(), name);
             if (rc) return rc;
         }
-        win_tile_kernel<T, DP><<<(uint32_t)row_tiles * now, kTileThreads, TileSmem<T, DP>::kBytes, l.stream>>>(p, plan, tiles, heads, h);
+        // a programmatic dependent of the pack kernel: its set-up and query rows (which no kernel of this call writes) overlap it.
+        // Beside a plan kernel nothing may be read early, and the launch is an ordinary one
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((uint32_t)row_tiles * now);
+        cfg.blockDim = dim3(kTileThreads);
+        cfg.dynamicSmemBytes = TileSmem<T, DP>::kBytes;
+        cfg.stream = l.stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = key_tiles && !ragged ? 1 : 0;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, win_tile_kernel<T, DP>, p, plan, static_cast<const unsigned char *>(tiles),
+                                                 static_cast<const TileHead *>(heads), h);
         count_launch();
-        rc = check_cuda(cudaGetLastError(), name);
+        rc = check_cuda(e, name);
         if (rc) return rc;
     }
     note_selection("%s: tcgen05 tiles, up to %u tiles of 128 positions and %u of 128 rows, %u pass(es)", name, plan.max_key_tiles,
