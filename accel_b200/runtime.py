@@ -152,6 +152,8 @@ def launch(name: str, bindings: Sequence[torch.Tensor], uniform: Optional[bytes]
 
 
 _arrays: dict = {}      # ctypes array types by (element type, length): making one costs more than filling it
+# the current stream's handle without the Stream object around it, where torch offers that
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _array(kind, values):
@@ -162,64 +164,61 @@ def _array(kind, values):
     return t(*values)
 
 
-def _on_stream(dev: torch.device, call) -> int:
-    """call(stream) with `dev` current, on its current stream."""
-    if dev.index == torch.cuda.current_device():
-        return call(torch.cuda.current_stream(dev).cuda_stream)
-    with torch.cuda.device(dev):
-        return call(torch.cuda.current_stream(dev).cuda_stream)
-
-
 def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: bytes, scratch: bool = False):
     """`launch` for the operators whose scratch memory (scratch: they may need some) is the call's own:
     it comes from torch's allocator, so a call captured into a CUDA graph keeps it in that graph's pool
     and two graphs, or two streams, never share it.  A binding of None is empty; one of more elements
     than 32 bits count is passed as 0xffffffff, which those kernels read as that many or more."""
-    L = _lib.lib()
     dev = bindings[0].device
     if dev.type != "cuda":
         raise _lib.AccelError(_lib.AB_ERR_NO_DEVICE, f"{name}: bindings live on {dev}; this backend "
                               "runs on a CUDA device and has no CPU path")
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return launch_own(name, bindings, uniform, scratch)
     ptrs, lens = [], []
     for t in bindings:
-        if t is None:
+        n = 0 if t is None else t.numel()
+        if n == 0:
             ptrs.append(None)
             lens.append(0)
             continue
         if t.device != dev or not t.is_contiguous():
             raise ValueError(f"{name}: every binding is a contiguous tensor on {dev}")
-        n = t.numel()
-        ptrs.append(t.data_ptr() if n else None)
+        ptrs.append(t.data_ptr())
         lens.append(n if n < 0xffffffff else 0xffffffff)
-    ws = None
+    ws, ws_bytes = None, 0
     if scratch:
-        need = workspace_bytes(name, lens, uniform)
-        if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _lib.check(_on_stream(dev, lambda stream: L.ab_launch(
-        name.encode(), stream, _array(C.c_void_p, ptrs), _array(C.c_uint32, lens), len(ptrs), uniform, len(uniform),
-        ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0)))
+        ws_bytes = workspace_bytes(name, lens, uniform)
+        if ws_bytes:
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    rc = _lib.lib().ab_launch(name.encode(), _raw_stream(dev.index), _array(C.c_void_p, ptrs), _array(C.c_uint32, lens),
+                              len(ptrs), uniform, len(uniform), ws.data_ptr() if ws is not None else None, ws_bytes)
+    if rc:
+        _lib.check(rc)
 
 
 def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], block: int):
     """ab_cache_copy_pages on the current stream of the caches' device."""
-    L = _lib.lib()
-    dev, n = caches[0].device, len(src)
+    t, n = caches[0], len(src)
+    dev = t.device
     if dev.type != "cuda":
         raise _lib.AccelError(_lib.AB_ERR_NO_DEVICE, f"copy_pages: the caches live on {dev}; this backend runs on a CUDA "
                               "device and has no CPU path")
-    if any(not 0 <= p < 0xffffffff for p in (*src, *dst)):
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return copy_pages(caches, src, dst, block)
+    if n and (min(src) < 0 or min(dst) < 0 or max(src) > 0xffffffff or max(dst) > 0xffffffff):
         raise _lib.AccelError(_lib.AB_ERR_INVALID, "copy_pages: a page id is u32")
-    t = caches[0]
-    page_bytes = t.stride(0) * t.element_size() * block if t.numel() else 0
+    page_bytes = t.numel() // t.shape[0] * t.element_size() * block if t.numel() else 0
     if page_bytes == 0:
         if n:
             raise _lib.AccelError(_lib.AB_ERR_INVALID, "copy_pages: the caches are empty")
         return
-    ptrs = _array(C.c_void_p, [c.data_ptr() for c in caches])
-    s, d = (C.c_uint32 * n)(*src), (C.c_uint32 * n)(*dst)
-    _lib.check(_on_stream(dev, lambda stream: L.ab_cache_copy_pages(stream, ptrs, len(caches), page_bytes,
-                                                                    t.shape[0] // block, s, d, n)))
+    rc = _lib.lib().ab_cache_copy_pages(_raw_stream(dev.index), _array(C.c_void_p, [c.data_ptr() for c in caches]), len(caches),
+                                        page_bytes, t.shape[0] // block, (C.c_uint32 * n)(*src), (C.c_uint32 * n)(*dst), n)
+    if rc:
+        _lib.check(rc)
 
 
 def attention_error():

@@ -38,7 +38,8 @@ def _is_u32(t: torch.Tensor) -> bool:
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """A contiguous tensor on a 16-byte boundary, which every binding is: a row of a larger tensor may
     start anywhere."""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -259,9 +260,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
     if opts.lengths.numel() != batch:
         raise Refused(op, f"Lengths holds {opts.lengths.numel()} entries and this step has {batch} "
                       "sequence(s); it is one length per sequence")
-    for name, n in (("Window", opts.window), ("Sinks", opts.sinks)):
-        if not isinstance(n, int) or isinstance(n, bool) or not 0 <= n < 1 << 32:
-            raise Refused(op, f"{name} is {n!r}; it is a number of positions")
+    if opts.window != 0 or opts.sinks != 0:
+        for name, n in (("Window", opts.window), ("Sinks", opts.sinks)):
+            if type(n) is not int or not 0 <= n < 1 << 32:
+                raise Refused(op, f"{name} is {n!r}; it is a number of positions")
     if opts.sinks and not opts.window:
         raise Refused(op, f"Sinks is {opts.sinks} and Window is 0; without a window every position is visible")
     k, v = k.contiguous(), v.contiguous()
@@ -269,7 +271,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
 
     def windowed(form, rows, max_pages=0, base=0, pages=None, offsets=None):
         """The windowed kernel of a form whose arguments have been checked."""
-        out = torch.empty((rows, q_heads, head_dim), dtype=torch.float32, device=q.device)
+        out = q.new_empty((rows, q_heads, head_dim))
         if rows and q_heads and head_dim:
             b = [q, k, v] + [_aligned(t) for t in (pages, opts.lengths, offsets) if t is not None] + [out]
             rt.launch_own("AttentionWindow" + form + ("F16" if f16 else ""), b,
@@ -575,7 +577,6 @@ def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
     numbers; a page that is written twice, or both written and read, is refused.  No reference
     counterpart."""
     op = "CopyPages"
-    caches = list(caches)
     if len(src) != len(dst):
         raise Refused(op, f"{len(src)} source pages and {len(dst)} destination pages")
     if not isinstance(block, int) or block <= 0:
@@ -583,9 +584,10 @@ def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
     if not caches:
         return
     first = caches[0]
+    shape, dtype, device = first.shape, first.dtype, first.device
     seen = set()
     for c in caches:
-        if c.dim() < 1 or c.shape != first.shape or c.dtype != first.dtype or c.device != first.device:
+        if c.dim() < 1 or c.shape != shape or c.dtype != dtype or c.device != device:
             raise Refused(op, f"the caches are {tuple(first.shape)} {first.dtype} on {first.device} and {tuple(c.shape)} "
                           f"{c.dtype} on {c.device}; one call copies in caches of one form")
         if not c.is_contiguous():
@@ -618,7 +620,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     if logits.dtype not in (torch.float32, torch.float16) or logits.dim() != 2 or logits.shape[1] == 0:
         raise Refused(op, f"logits are {logits.dtype} {tuple(logits.shape)}; they are f32 or f16 [rows, vocab]")
     rows, vocab = logits.shape
-    if not isinstance(top, int) or isinstance(top, bool) or not 0 <= top <= min(32, vocab):
+    if type(top) is not int or not 0 <= top <= min(32, vocab):
         raise Refused(op, f"{top!r} alternatives of a vocabulary of {vocab}; at most 32")
     dev = logits.device
     n = 0
@@ -628,9 +630,12 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         if targets.dim() not in (1, 2) or targets.shape[0] != rows:
             raise Refused(op, f"targets are {tuple(targets.shape)} and the logits hold {rows} rows; they are [rows] or [rows, n]")
         n = 1 if targets.dim() == 1 else targets.shape[1]
-    new = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)
-    lp = None if targets is None else torch.empty(targets.shape, dtype=torch.float32, device=dev)
-    out = TokenLogprobs(lp, new(rows), torch.empty((rows, top), dtype=U32, device=dev), new(rows, top))
+    # one allocation for what is f32: the top alternatives' rows first, which start on a 16-byte boundary of their own
+    at = (rows * top + 3) & ~3
+    end = (at + rows + 3) & ~3
+    flat = torch.empty(end + rows * n, dtype=torch.float32, device=dev)
+    lp = None if targets is None else flat[end:].view(targets.shape)
+    out = TokenLogprobs(lp, flat[at:at + rows], torch.empty((rows, top), dtype=U32, device=dev), flat[:rows * top].view(rows, top))
     if rows:
         rt.launch_own("TokenLogprobsF16" if logits.dtype == torch.float16 else "TokenLogprobs",
                       [_aligned(logits), None if targets is None else _aligned(targets), lp, out.entropy,
