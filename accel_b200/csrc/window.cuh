@@ -16,7 +16,8 @@ struct WinParams {
     uint32_t reach;                                // positions the page table (or the cache) addresses
     uint32_t capacity;                             // rows of the cache
     uint32_t base;
-    const uint32_t *left;                          // a ragged step some of whose rows went on tiles: how many did not, and which; or NULL
+    const uint4 *left;                             // a ragged step some of whose rows went on tiles: {how many did not}, then their
+                                                   // {row, sequence (0xffffffff: zeros), position + 1, length}; or NULL
     float scale_log2;                              // Scale * log2(e)
     int form;
 };
@@ -31,6 +32,17 @@ __device__ __forceinline__ uint32_t win_cache_row(const WinParams &p, const uint
         r = (uint64_t)pages[pg] * p.block + (j - pg * p.block);
     }
     return r < p.capacity ? (uint32_t)r : 0xffffffffu;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t smem, uint32_t rank)
+{
+    float v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}"
+                 : "=f"(v) : "r"(smem), "r"(rank) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 #endif
 

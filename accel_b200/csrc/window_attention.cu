@@ -38,12 +38,19 @@ struct WinView {
     bool zero;                                     // a ragged padding row: written as zeros
 };
 
-__device__ __forceinline__ WinView win_view(const WinParams &p, uint32_t row)
+__device__ __forceinline__ WinView win_view(const WinParams &p, uint32_t &row)
 {
     WinView w{p.pages, 0, 0, 0, false};
     uint64_t pos1;                                 // the row's position + 1
     uint32_t len;
-    if (p.form == kRaggedStep) {
+    if (p.left) {
+        const uint4 e = p.left[1 + row];           // row, sequence, position + 1, length
+        row = e.x;
+        if (e.y == 0xffffffffu) { w.zero = true; return w; }
+        pos1 = e.z;
+        len = min(e.w, p.reach);
+        w.pages = p.pages + (size_t)e.y * p.max_pages;
+    } else if (p.form == kRaggedStep) {
         // the sequence whose [offsets[s], offsets[s + 1]) holds the row; empty sequences hold none
         uint32_t a = 0, b = p.batch;
         while (a < b) {
@@ -75,8 +82,7 @@ __device__ __forceinline__ WinView win_view(const WinParams &p, uint32_t row)
 }
 
 // The rows of a launch: all of the call's, or those that are left beside tiles.
-__device__ __forceinline__ uint32_t win_rows(const WinParams &p) { return p.left ? p.left[0] : p.rows; }
-__device__ __forceinline__ uint32_t win_row_of(const WinParams &p, uint32_t turn) { return p.left ? p.left[1 + turn] : turn; }
+__device__ __forceinline__ uint32_t win_rows(const WinParams &p) { return p.left ? p.left[0].x : p.rows; }
 
 // The list's entry i: its position; the page that holds it (loaded now, looked at later: a page's number is asked for
 // two tiles ahead of its rows, so that nothing waits for the table); its cache row, 0xffffffff where that page lies outside
@@ -340,18 +346,6 @@ template <int DP> struct RowMath<__half, DP> {
     static __device__ __forceinline__ int dim(int m, int i, int g) { return 16 * m + g + 8 * (i >> 1); }
 };
 
-__device__ __forceinline__ float ld_cluster(uint32_t smem, uint32_t rank)
-{
-    float v;
-    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}"
-                 : "=f"(v) : "r"(smem), "r"(rank) : "memory");
-    return v;
-}
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // The parts of a row's heads, one per warp (or group of lanes), then one per CTA of the cluster, joined in their order:
 // [part][maxima of C columns, sums of C columns] and [part][C][DP] in shared memory, the CTA's own result behind them.
 template <int N, int C, int DP>
@@ -411,7 +405,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
     const uint32_t tile_k = (uint32_t)__cvta_generic_to_shared(smem) + warp * Tile::kWarpBytes, tile_v = tile_k + Tile::kBytesK;
 
     for (uint32_t turn = blockIdx.x / parts; turn < win_rows(p); turn += gridDim.x / parts) {
-    const uint32_t row = win_row_of(p, turn);
+    uint32_t row = turn;
     const WinView w = win_view(p, row);
     const uint32_t n_tiles = (w.n + kTile - 1) / kTile, step = parts * kRowWarps;
     uint32_t tile = part * kRowWarps + warp;
@@ -557,7 +551,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) win_lanes_kernel(const WinP
     const uint32_t part = blockIdx.x % parts, kvh = blockIdx.y, h0 = kvh * G, D = p.head_dim;
     const bool on = (uint32_t)ll * 4 < D;
     for (uint32_t turn = blockIdx.x / parts; turn < win_rows(p); turn += gridDim.x / parts) {
-    const uint32_t row = win_row_of(p, turn);
+    uint32_t row = turn;
     const WinView w = win_view(p, row);
     const uint32_t n_batches = (w.n + 7) / 8, step = parts * kPart;
     // lanes 0..7 of a group: its eight positions (past the last batch there is nothing to see)
@@ -696,7 +690,7 @@ int launch_split(Launch &l, const WinParams &p, void (*kernel)(const WinParams, 
         const uint64_t cost = rounds * (8 * (steps + 3) + n);
         if (cost < least) { least = cost; parts = n; }
     }
-    const uint64_t turns = p.left ? std::min<uint64_t>(p.rows, std::max<uint64_t>(rows, 2 * places / ((uint64_t)groups * parts) + 1)) : rows;
+    const uint64_t turns = p.left ? std::min<uint64_t>(p.rows, std::max<uint64_t>(rows, places / ((uint64_t)groups * parts) + 1)) : rows;
     if (turns * parts > 0x7fffffffull || groups > 65535)
         return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
     cudaLaunchConfig_t cfg = {};

@@ -302,7 +302,8 @@ __device__ __forceinline__ Range win_range(const WinParams &p, const Segment &k,
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTileThreads, 1)
-win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *tiles, const TileHead *heads, uint32_t kvh0)
+win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *tiles, const TileHead *heads, uint32_t kvh0,
+                uint32_t split)
 {
     using Smem = TileSmem<T, DP>;
     constexpr uint32_t kSlot = kSlotBytes<T, DP>;
@@ -316,9 +317,9 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
 
     // the rows: tokens x heads of the group; the last tokens, which see most, first
     const uint32_t group = p.q_heads / p.kv_heads, per_tile = kRows / group, D = p.head_dim;
-    const uint32_t kv = blockIdx.x / plan.max_row_tiles;
+    const uint32_t index = blockIdx.x / split, part = blockIdx.x % split, kv = index / plan.max_row_tiles;
     Segment keys = plan.one;
-    uint32_t rt = plan.max_row_tiles - 1 - blockIdx.x % plan.max_row_tiles;
+    uint32_t rt = plan.max_row_tiles - 1 - index % plan.max_row_tiles;
     if (plan.segments) {
         if (rt >= plan.counts[1]) return;
         const uint2 e = plan.row_tiles[rt];
@@ -329,8 +330,10 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
     const uint32_t first = rt * per_tile, tok0 = keys.row0 + first, tokens = min(per_tile, keys.rows - first);
     const uint64_t pa = (uint64_t)keys.base + first;
     const Range range = win_range(p, keys, pa, pa + tokens - 1);
-    const uint32_t n = range.sinks_end + (range.end - range.begin);
-    const auto tile_of = [&](uint32_t i) { return i < range.sinks_end ? i : range.begin + (i - range.sinks_end); };
+    // of the tiles that they see, this CTA of the cluster takes n, from the i0-th on
+    const uint32_t all = range.sinks_end + (range.end - range.begin), share = (all + split - 1) / split, i0 = min(part * share, all);
+    const uint32_t n = min(share, all - i0);
+    const auto tile_of = [&](uint32_t i) { return i0 + i < range.sinks_end ? i0 + i : range.begin + (i0 + i - range.sinks_end); };
     tiles += ((size_t)kv * plan.max_key_tiles + keys.tile0) * kTileBytes<T, DP>;
     heads += (size_t)kv * plan.max_key_tiles + keys.tile0;
 
@@ -598,7 +601,7 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
         asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
         const float m0 = ml[0], m1 = ml[3 * kRows], M = fmaxf(m0, m1);
         const float f0 = m0 == -CUDART_INF_F ? 0.f : ab_ex2(m0 - M), f1 = m1 == -CUDART_INF_F ? 0.f : ab_ex2(m1 - M);
-        const float sum = fmaf(ml[kRows], f0, ml[4 * kRows] * f1), fm = (wg ? f1 : f0) / sum, fo = (wg ? f0 : f1) / sum;
+        const float fm = wg ? f1 : f0, fo = wg ? f0 : f1;
 #pragma unroll
         for (int i = 0; i < DP / 2; i += 4) {
             float4 x = *reinterpret_cast<float4 *>(mine + i);
@@ -628,20 +631,46 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
                 }
             }
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
-        // a warp writes a row (two, of a head of 64) at a time
-        constexpr int kLanes = DP / 4, kTogether = 32 / kLanes;
-#pragma unroll 4
-        for (int i = 0; i < kRows / kSoftWarps; i += kTogether) {
-            const uint32_t row = warp * (kRows / kSoftWarps) + i + lane / kLanes, d = lane % kLanes * 4;
-            if (row < tokens * group && d < D)
-                *reinterpret_cast<float4 *>(p.out + ((uint64_t)(tok0 + row / group) * p.q_heads + (kvh0 + kv) * group + row % group) * D + d) =
-                    *reinterpret_cast<const float4 *>(rows + row * kPitch + d);
+        if (wg == 0) {
+            float *total = rows + kRows * kPitch + 6 * kRows + r;      // [m, l][row]
+            total[0] = M;
+            total[kRows] = fmaf(ml[kRows], f0, ml[4 * kRows] * f1);
         }
     }
+    // ---- the CTAs' parts of a row, in their order; a warp writes a row (two, of a head of 64) at a time
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == kSoftWarps) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (split > 1) cluster_sync();
+    if (warp < kSoftWarps) {
+        constexpr int kLanes = DP / 4, kTogether = 32 / kLanes;
+        constexpr uint32_t kPitch = DP + 4;
+        const float *rows = reinterpret_cast<const float *>(smem), *total = rows + kRows * kPitch + 6 * kRows;
+        for (uint32_t i = (part * kSoftWarps + warp) * kTogether; i < kRows; i += split * kSoftWarps * kTogether) {
+            const uint32_t row = i + lane / kLanes, d = lane % kLanes * 4;
+            float4 x = *reinterpret_cast<const float4 *>(rows + row * kPitch + d);
+            float sum = total[kRows + row];
+            if (split > 1) {
+                float M = -CUDART_INF_F;
+                for (uint32_t c = 0; c < split; c++) M = fmaxf(M, ld_cluster(sx_smem(total + row), c));
+                x = make_float4(0.f, 0.f, 0.f, 0.f);
+                sum = 0.f;
+                for (uint32_t c = 0; c < split; c++) {
+                    const float m = ld_cluster(sx_smem(total + row), c), f = m == -CUDART_INF_F ? 0.f : ab_ex2(m - M);
+                    const uint32_t at = sx_smem(rows + row * kPitch + d);
+                    sum = fmaf(ld_cluster(sx_smem(total + kRows + row), c), f, sum);
+                    x.x = fmaf(ld_cluster(at, c), f, x.x);
+                    x.y = fmaf(ld_cluster(at + 4, c), f, x.y);
+                    x.z = fmaf(ld_cluster(at + 8, c), f, x.z);
+                    x.w = fmaf(ld_cluster(at + 12, c), f, x.w);
+                }
+            }
+            if (row < tokens * group && d < D)
+                *reinterpret_cast<float4 *>(p.out + ((uint64_t)(tok0 + row / group) * p.q_heads + (kvh0 + kv) * group + row % group) * D + d) =
+                    make_float4(x.x / sum, x.y / sum, x.z / sum, x.w / sum);
+        }
+    }
+    if (split > 1) cluster_sync();                       // nobody leaves while its parts are being read
 }
 
 template <typename T, int DP> int tile_prepare(const char *name)
@@ -660,10 +689,10 @@ template <typename T, int DP> int tile_prepare(const char *name)
 
 // ------------------------------------------------------------------------------------------------
 // A ragged step: the sequences with at least `from` rows (tokens x heads of a group) become segments, the rows of the
-// others, and those behind the last sequence, are left to the row kernel: left[0] of them, listed behind.  One block.
+// others, and those behind the last sequence, are left to the row kernel (WinParams::left).  One block.
 __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32_t from, uint32_t max_segments, Segment *segments,
                                                        uint2 *key_tiles, uint2 *row_tiles, uint32_t *counts, uint32_t max_key_tiles,
-                                                       uint32_t max_row_tiles, uint32_t *left)
+                                                       uint32_t max_row_tiles, uint4 *left)
 {
     __shared__ uint4 part[8];
     const uint32_t t = threadIdx.x, lane = t & 31, group = p.q_heads / p.kv_heads, per_tile = kRows / group;
@@ -672,10 +701,12 @@ __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32
         const uint32_t s = s0 + t;
         Segment g{};
         uint4 mine = make_uint4(0, 0, 0, 0);
-        uint32_t first = 0;
+        uint32_t first = 0, len = 0, count = 0;
         if (s < p.batch) {
-            const uint32_t a = min(p.offsets[s], p.rows), b = min(p.offsets[s + 1], p.rows), len = p.lengths[s];
+            const uint32_t a = min(p.offsets[s], p.rows), b = min(p.offsets[s + 1], p.rows);
+            len = p.lengths[s];
             first = a;
+            count = p.offsets[s + 1] - p.offsets[s];
             mine.w = b > a ? b - a : 0;
             // (a sequence with more tokens than positions has rows of zeros: the row kernel knows)
             if (b > a && b == p.offsets[s + 1] && (uint64_t)(b - a) * group >= from && len >= b - a) {
@@ -710,12 +741,16 @@ __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32
             for (uint32_t i = at.y; i < max_key_tiles && i - at.y < mine.y; i++) key_tiles[i] = make_uint2(0xffffffffu, 0);
             for (uint32_t i = at.z; i < max_row_tiles && i - at.z < mine.z; i++) row_tiles[i] = make_uint2(0xffffffffu, 0);
         }
-        for (uint32_t i = 0; i < mine.w && at.w + i < p.rows; i++) left[1 + at.w + i] = first + i;
+        for (uint32_t i = 0; i < mine.w && at.w + i < p.rows; i++) {
+            // (the first tokens of a sequence with fewer positions than tokens have none)
+            const uint64_t pos1 = (uint64_t)len + i + 1;
+            left[1 + at.w + i] = make_uint4(first + i, pos1 > count ? s : 0xffffffffu, (uint32_t)(pos1 - count), len);
+        }
         __syncthreads();
     }
     const uint32_t end = min(p.offsets[p.batch], p.rows);
-    for (uint32_t i = end + t; i < p.rows && before.w + (i - end) < p.rows; i += 256) left[1 + before.w + (i - end)] = i;
-    if (t == 0) left[0] = min(before.w + (p.rows - end), p.rows);
+    for (uint32_t i = end + t; i < p.rows && before.w + (i - end) < p.rows; i += 256) left[1 + before.w + (i - end)] = make_uint4(i, 0xffffffffu, 0, 0);
+    if (t == 0) left[0] = make_uint4(min(before.w + (p.rows - end), p.rows), 0, 0, 0);
     if (t == 0) { counts[0] = min(before.y, max_key_tiles); counts[1] = min(before.z, max_row_tiles); }
 }
 
@@ -724,7 +759,7 @@ constexpr uint64_t kPassBytes = 1ull << 30;              // tiles of one pass ov
 template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char *name)
 {
     static_assert(TileSmem<T, DP>::kBytes <= 232448, "shared memory of a CTA");
-    static_assert(kRows * (DP + 4) * 4 + 6 * kRows * 4 <= TileSmem<T, DP>::kBars, "the parts of all groups fit where the operands were");
+    static_assert(kRows * (DP + 4) * 4 + 8 * kRows * 4 <= TileSmem<T, DP>::kBars, "the parts of all groups fit where the operands were");
     const uint32_t group = p.q_heads / p.kv_heads, per_tile = kRows / group;
     const bool ragged = p.form == kRaggedStep;
     TilePlan plan{};
@@ -746,8 +781,8 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
     const uint32_t pass = (uint32_t)std::min<uint64_t>(p.kv_heads, std::max<uint64_t>(1, kPassBytes / per_head));
     const size_t head_bytes = align_up((size_t)(pass * key_tiles) * sizeof(TileHead), 256);
     const size_t seg_bytes = align_up((size_t)segments * sizeof(Segment), 256), key_bytes = ragged ? align_up((size_t)key_tiles * 8, 256) : 0;
-    const size_t row_bytes = ragged ? align_up((size_t)row_tiles * 8, 256) : 0, flag_bytes = ragged ? align_up((size_t)p.rows * 4 + 12, 256) : 0;
-    l.ws_need = seg_bytes + key_bytes + row_bytes + flag_bytes + head_bytes + (size_t)(pass * per_head);
+    const size_t row_bytes = ragged ? align_up((size_t)row_tiles * 8, 256) : 0, left_bytes = ragged ? align_up((size_t)p.rows * 16 + 32, 256) : 0;
+    l.ws_need = seg_bytes + key_bytes + row_bytes + left_bytes + head_bytes + (size_t)(pass * per_head);
     if (row_tiles * pass > 0x7fffffffull || key_tiles > 0x7fffffffull || pass > 65535)
         return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
     if (l.query_ws) return AB_OK;
@@ -766,14 +801,23 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
         plan.key_tiles = kt;
         plan.row_tiles = rt;
         plan.counts = counts;
-        p.left = counts + 2;
+        uint4 *left = reinterpret_cast<uint4 *>(counts + 4);
+        p.left = left;
         win_plan_kernel<<<1, 256, 0, l.stream>>>(p, kTileFrom, (uint32_t)segments, segs, kt, rt, counts, plan.max_key_tiles,
-                                                 plan.max_row_tiles, counts + 2);
+                                                 plan.max_row_tiles, left);
         count_launch();
         rc = check_cuda(cudaGetLastError(), name);
         if (rc) return rc;
     }
-    TileHead *heads = reinterpret_cast<TileHead *>(ws + seg_bytes + key_bytes + row_bytes + flag_bytes);
+    // few row tiles: a cluster shares the positions of each, as long as all CTAs run at once and have four tiles or more
+    uint32_t split = 1;
+    {
+        const uint64_t ctas = (ragged ? p.rows / per_tile + 1 : row_tiles) * pass;
+        const uint64_t seen = std::min<uint64_t>((uint64_t)std::min(p.window, p.reach) + per_tile + p.sinks, ragged ? p.reach : plan.one.end) / kKeys;
+        while (split < 8 && ctas * split * 2 <= (uint64_t)sm_count() && seen >= (uint64_t)split * 2 * 4) split *= 2;
+    }
+    if (row_tiles * pass * split > 0x7fffffffull) return fail(AB_ERR_INVALID, "%s: %u rows of %u heads", name, p.rows, p.q_heads);
+    TileHead *heads = reinterpret_cast<TileHead *>(ws + seg_bytes + key_bytes + row_bytes + left_bytes);
     unsigned char *tiles = reinterpret_cast<unsigned char *>(heads) + head_bytes;
     for (uint32_t h = 0; h < p.kv_heads && row_tiles; h += pass) {
         const uint32_t now = std::min(pass, p.kv_heads - h);
@@ -786,23 +830,30 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
         // a programmatic dependent of the pack kernel: its set-up and query rows (which no kernel of this call writes) overlap it.
         // Beside a plan kernel nothing may be read early, and the launch is an ordinary one
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((uint32_t)row_tiles * now);
+        cfg.gridDim = dim3((uint32_t)row_tiles * now * split);
         cfg.blockDim = dim3(kTileThreads);
         cfg.dynamicSmemBytes = TileSmem<T, DP>::kBytes;
         cfg.stream = l.stream;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchAttribute attr[2];
         cfg.attrs = attr;
-        cfg.numAttrs = key_tiles && !ragged ? 1 : 0;
+        if (key_tiles && !ragged) {
+            attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+        }
+        if (split > 1) {
+            attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+            attr[cfg.numAttrs].val.clusterDim.x = split;
+            attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+            cfg.numAttrs++;
+        }
         const cudaError_t e = cudaLaunchKernelEx(&cfg, win_tile_kernel<T, DP>, p, plan, static_cast<const unsigned char *>(tiles),
-                                                 static_cast<const TileHead *>(heads), h);
+                                                 static_cast<const TileHead *>(heads), h, split);
         count_launch();
         rc = check_cuda(e, name);
         if (rc) return rc;
     }
-    note_selection("%s: tcgen05 tiles, up to %u tiles of 128 positions and %u of 128 rows, %u pass(es)", name, plan.max_key_tiles,
-                   plan.max_row_tiles, (p.kv_heads + pass - 1) / pass);
+    note_selection("%s: tcgen05 tiles, up to %u tiles of 128 positions and %u of 128 rows, split over %u CTA(s), %u pass(es)", name,
+                   plan.max_key_tiles, plan.max_row_tiles, split, (p.kv_heads + pass - 1) / pass);
     return AB_OK;
 }
 

@@ -630,12 +630,9 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         if targets.dim() not in (1, 2) or targets.shape[0] != rows:
             raise Refused(op, f"targets are {tuple(targets.shape)} and the logits hold {rows} rows; they are [rows] or [rows, n]")
         n = 1 if targets.dim() == 1 else targets.shape[1]
-    # one allocation for what is f32: the top alternatives' rows first, which start on a 16-byte boundary of their own
-    at = (rows * top + 3) & ~3
-    end = (at + rows + 3) & ~3
-    flat = torch.empty(end + rows * n, dtype=torch.float32, device=dev)
-    lp = None if targets is None else flat[end:].view(targets.shape)
-    out = TokenLogprobs(lp, flat[at:at + rows], torch.empty((rows, top), dtype=U32, device=dev), flat[:rows * top].view(rows, top))
+    new = lambda shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=dev)
+    lp = None if targets is None else new(targets.shape)
+    out = TokenLogprobs(lp, new((rows,)), new((rows, top), U32), new((rows, top)))
     if rows:
         rt.launch_own("TokenLogprobsF16" if logits.dtype == torch.float16 else "TokenLogprobs",
                       [_aligned(logits), None if targets is None else _aligned(targets), lp, out.entropy,
