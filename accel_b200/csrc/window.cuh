@@ -40,6 +40,13 @@ __device__ __forceinline__ float ld_cluster(uint32_t smem, uint32_t rank)
                  : "=f"(v) : "r"(smem), "r"(rank) : "memory");
     return v;
 }
+__device__ __forceinline__ float4 ld_cluster4(uint32_t smem, uint32_t rank)
+{
+    float4 v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [r];\n\t}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem), "r"(rank) : "memory");
+    return v;
+}
 __device__ __forceinline__ void cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");

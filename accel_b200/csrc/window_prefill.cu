@@ -637,37 +637,53 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
             total[kRows] = fmaf(ml[kRows], f0, ml[4 * kRows] * f1);
         }
     }
-    // ---- the CTAs' parts of a row, in their order; a warp writes a row (two, of a head of 64) at a time
+    // ---- the CTAs' parts of a row, in their order, and out: a warp writes a row (two, of a head of 64) at a time
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == kSoftWarps) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     if (split > 1) cluster_sync();
     if (warp < kSoftWarps) {
-        constexpr int kLanes = DP / 4, kTogether = 32 / kLanes;
-        constexpr uint32_t kPitch = DP + 4;
+        constexpr uint32_t kPitch = DP + 4, kWarpRows = kRows / kSoftWarps, kLanes = DP / 4, kTogether = 32 / kLanes;
         const float *rows = reinterpret_cast<const float *>(smem), *total = rows + kRows * kPitch + 6 * kRows;
-        for (uint32_t i = (part * kSoftWarps + warp) * kTogether; i < kRows; i += split * kSoftWarps * kTogether) {
-            const uint32_t row = i + lane / kLanes, d = lane % kLanes * 4;
-            float4 x = *reinterpret_cast<const float4 *>(rows + row * kPitch + d);
-            float sum = total[kRows + row];
-            if (split > 1) {
-                float M = -CUDART_INF_F;
-                for (uint32_t c = 0; c < split; c++) M = fmaxf(M, ld_cluster(sx_smem(total + row), c));
-                x = make_float4(0.f, 0.f, 0.f, 0.f);
-                sum = 0.f;
-                for (uint32_t c = 0; c < split; c++) {
-                    const float m = ld_cluster(sx_smem(total + row), c), f = m == -CUDART_INF_F ? 0.f : ab_ex2(m - M);
-                    const uint32_t at = sx_smem(rows + row * kPitch + d);
-                    sum = fmaf(ld_cluster(sx_smem(total + kRows + row), c), f, sum);
-                    x.x = fmaf(ld_cluster(at, c), f, x.x);
-                    x.y = fmaf(ld_cluster(at + 4, c), f, x.y);
-                    x.z = fmaf(ld_cluster(at + 8, c), f, x.z);
-                    x.w = fmaf(ld_cluster(at + 12, c), f, x.w);
-                }
+        // a lane knows one of its warp's 16 rows: where it goes, and what each CTA's part is multiplied by
+        const uint32_t mine = warp * kWarpRows + (lane & 15);
+        const uint32_t to = mine < tokens * group ? (mine / group) * p.q_heads + mine % group : 0xffffffffu;
+        float *out = p.out + ((uint64_t)tok0 * p.q_heads + (kvh0 + kv) * group) * D;
+        const uint32_t d = lane % kLanes * 4;
+        if (split == 1) {
+            const float f = 1.f / total[kRows + mine];
+#pragma unroll 4
+            for (uint32_t i = 0; i < kWarpRows; i += kTogether) {
+                const uint32_t row = i + lane / kLanes, at = __shfl_sync(0xffffffffu, to, row);
+                const float g = __shfl_sync(0xffffffffu, f, row);
+                const float4 x = *reinterpret_cast<const float4 *>(rows + (warp * kWarpRows + row) * kPitch + d);
+                if (at != 0xffffffffu && d < D)
+                    *reinterpret_cast<float4 *>(out + (uint64_t)at * D + d) = make_float4(x.x * g, x.y * g, x.z * g, x.w * g);
             }
-            if (row < tokens * group && d < D)
-                *reinterpret_cast<float4 *>(p.out + ((uint64_t)(tok0 + row / group) * p.q_heads + (kvh0 + kv) * group + row % group) * D + d) =
-                    make_float4(x.x / sum, x.y / sum, x.z / sum, x.w / sum);
+        } else {
+            // (the warp's rows are shared out too: every CTA of the cluster writes some of them)
+            float M = -CUDART_INF_F, sum = 0.f;
+            for (uint32_t c = 0; c < split; c++) M = fmaxf(M, ld_cluster(sx_smem(total + mine), c));
+            for (uint32_t c = 0; c < split; c++) {
+                const float m = ld_cluster(sx_smem(total + mine), c), f = m == -CUDART_INF_F ? 0.f : ab_ex2(m - M);
+                sum = fmaf(ld_cluster(sx_smem(total + kRows + mine), c), f, sum);
+            }
+            const float inv = 1.f / sum;
+            const uint32_t some = kWarpRows / split;                // split is 2, 4 or 8
+#pragma unroll 2
+            for (uint32_t i = part * some; i < (part + 1) * some; i += kTogether) {
+                const uint32_t row = i + lane / kLanes, at = __shfl_sync(0xffffffffu, to, row);
+                const float g = __shfl_sync(0xffffffffu, inv, row), top = __shfl_sync(0xffffffffu, M, row);
+                const uint32_t r0 = warp * kWarpRows + row;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (uint32_t c = 0; c < split; c++) {
+                    const float m = ld_cluster(sx_smem(total + r0), c), f = m == -CUDART_INF_F ? 0.f : ab_ex2(m - top);
+                    const float4 y = ld_cluster4(sx_smem(rows + r0 * kPitch + d), c);
+                    x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
+                }
+                if (at != 0xffffffffu && d < D)
+                    *reinterpret_cast<float4 *>(out + (uint64_t)at * D + d) = make_float4(x.x * g, x.y * g, x.z * g, x.w * g);
+            }
         }
     }
     if (split > 1) cluster_sync();                       // nobody leaves while its parts are being read
