@@ -26,6 +26,7 @@
 #include <math_constants.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "sm100.cuh"
@@ -71,7 +72,8 @@ __host__ __device__ inline void segment_list(Segment &s, uint32_t window, uint32
 struct TilePlan {
     Segment one;
     const Segment *segments;                // NULL: one
-    const uint2 *key_tiles, *row_tiles;     // (segment, tile) of each
+    const uint4 *key_tiles;                 // {first position, end of the positions, sequence} of each
+    const uint2 *row_tiles;                 // (segment, tile) of each
     const uint32_t *counts;                 // how many of either
     uint32_t max_key_tiles, max_row_tiles;
 };
@@ -91,6 +93,8 @@ template <typename T, int DP> constexpr uint32_t kTileBytes = 2 * kParts<T> * kS
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float2 two(const float *p) { return __ldg(reinterpret_cast<const float2 *>(p)); }
+__device__ __forceinline__ float2 two(const __half *p) { return __half22float2(__ldg(reinterpret_cast<const __half2 *>(p))); }
 
 // the power of two that brings a largest magnitude into [2^13, 2^14), as an exponent
 __device__ __forceinline__ int fit_exponent(float amax)
@@ -130,14 +134,14 @@ __global__ void __launch_bounds__(kPackThreads, 2) win_pack_kernel(const WinPara
 {
     __shared__ uint32_t rows[kKeys], amax_bits, bad_any;
     pdl_trigger();                                       // the tile kernel may set itself up meanwhile
-    Segment s = plan.one;
-    uint32_t tile = blockIdx.x;
+    uint4 span;                                          // first position, end of the positions, sequence
     if (plan.segments) {
+        span = plan.key_tiles[blockIdx.x];
         if (blockIdx.x >= plan.counts[0]) return;
-        const uint2 e = plan.key_tiles[blockIdx.x];
-        if (e.x == 0xffffffffu) return;
-        s = plan.segments[e.x];
-        tile = e.y;
+    } else {
+        span.x = win_tile_start(plan.one, blockIdx.x);
+        span.y = min(blockIdx.x < plan.one.sink_tiles ? min(plan.one.ns, plan.one.end) : plan.one.end, p.lengths[0]);
+        span.z = 0;
     }
     const uint32_t kvh = kvh0 + blockIdx.y, t = threadIdx.x, D = p.head_dim;
     const size_t at = (size_t)blockIdx.y * plan.max_key_tiles + blockIdx.x;
@@ -145,22 +149,22 @@ __global__ void __launch_bounds__(kPackThreads, 2) win_pack_kernel(const WinPara
     unsigned char *dst = tiles + at * kTileBytes<T, DP> + (blockIdx.z ? kParts<T> * kSlotBytes<T, DP> : 0);
     if (t == 0) { amax_bits = 0; bad_any = 0; }
     if (t < kKeys) {
-        const uint64_t j = (uint64_t)win_tile_start(s, tile) + t;
+        const uint64_t j = (uint64_t)span.x + t;
         uint32_t r = 0xffffffffu;
-        if (j < win_end(p, plan, s) && (tile >= s.sink_tiles || j < s.ns))
-            r = win_cache_row(p, p.pages ? p.pages + (size_t)s.seq * p.max_pages : nullptr, (uint32_t)j);
+        if (j < span.y) r = win_cache_row(p, p.pages ? p.pages + (size_t)span.z * p.max_pages : nullptr, (uint32_t)j);
         rows[t] = r;
         const uint32_t seen = __ballot_sync(0xffffffffu, r != 0xffffffffu);
         if (blockIdx.z == 0 && (t & 31) == 0) head.seen[t >> 5] = seen;
     }
     __syncthreads();
-    constexpr int kEach = kKeys * DP / kPackThreads, kTogether = kPackThreads / DP;              // elements of a thread
+    // elements of a thread; dimensions that it takes of V together (4 bytes of a position); groups of eight positions at a time
+    constexpr int kEach = kKeys * DP / kPackThreads, kWide = sizeof(T) == 2 ? 2 : 1, kTogether = kPackThreads * kWide / DP;
     float x[kEach];
     float big = 0.f;
     bool bad = false;
     // K: eight dimensions of a position at a time; a warp takes eight positions x 32 dimensions, whole lines to read and to
-    // write.  V: eight positions of a dimension at a time, neighbouring threads neighbouring dimensions.
-    const uint32_t lane = t & 31, dim = t & (DP - 1), group0 = t / DP;
+    // write.  V: eight positions of kWide dimensions at a time, neighbouring threads neighbouring dimensions.
+    const uint32_t lane = t & 31, dim = t % (DP / kWide) * kWide, group0 = t / (DP / kWide);
     const auto k_task = [&](int i, uint32_t &key, uint32_t &d) {
         const uint32_t task = (i / 8) * (kPackThreads / 32) + (t >> 5);            // of 16 x DP / 32
         key = task / (DP / 32) * 8 + (lane & 7);
@@ -184,11 +188,19 @@ __global__ void __launch_bounds__(kPackThreads, 2) win_pack_kernel(const WinPara
             }
         }
     } else {
-        const T *v = static_cast<const T *>(p.v);
+        const T *v = static_cast<const T *>(p.v) + (uint64_t)kvh * D + dim;
 #pragma unroll
-        for (int i = 0; i < kEach; i++) {
+        for (int i = 0; i < kEach / kWide; i++) {
             const uint32_t r = rows[(i / 8 * kTogether + group0) * 8 + (i & 7)];
-            x[i] = r != 0xffffffffu && dim < D ? to_f32(v[((uint64_t)r * p.kv_heads + kvh) * D + dim]) : 0.f;
+            const T *src = v + (uint64_t)r * p.kv_heads * D;
+            const bool on = r != 0xffffffffu && dim < D;
+            if (kWide == 2) {
+                const float2 y = on ? two(src) : make_float2(0.f, 0.f);
+                x[i / 8 * 16 + (i & 7)] = y.x;
+                x[i / 8 * 16 + 8 + (i & 7)] = y.y;
+            } else {
+                x[i] = on ? to_f32(*src) : 0.f;
+            }
         }
     }
 #pragma unroll
@@ -219,7 +231,7 @@ __global__ void __launch_bounds__(kPackThreads, 2) win_pack_kernel(const WinPara
         for (int n = 0; n < 8; n++) y[n] = x[i + n] * f;
         uint4 hi, lo;
         split8(y, hi, lo);
-        uint32_t to = (i / 8 * kTogether + group0) * (DP * 16) + dim * 16;
+        uint32_t to = (i / (8 * kWide) * kTogether + group0) * (DP * 16) + (dim + i / 8 % kWide) * 16;
         if (blockIdx.z == 0) {
             uint32_t key, d;
             k_task(i, key, d);
@@ -337,6 +349,16 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
     tiles += ((size_t)kv * plan.max_key_tiles + keys.tile0) * kTileBytes<T, DP>;
     heads += (size_t)kv * plan.max_key_tiles + keys.tile0;
 
+    // The copies: parts of operands, in the order the MMAs take them: K(0) K(1) V(0) K(2) V(1) ... K(n-1) V(n-2) V(n-1)
+    const uint32_t items = 2 * n * kP;
+    const auto copy = [&](uint32_t i) {
+        const uint32_t op = i / kP, part = i % kP, slot = i % kSlots;
+        const bool key = op == 0 || ((op & 1) && op < 2 * n - 1);
+        const uint32_t t = key ? (op + 1) / 2 : (op == 2 * n - 1 ? n - 1 : op / 2 - 1);
+        sx_bar_expect_tx(&full[slot], kSlot);
+        sx_bulk_load(smem + Smem::kRing + slot * kSlot, tiles + (size_t)tile_of(t) * kTileBytes<T, DP> + ((key ? 0 : kP) + part) * kSlot,
+                     kSlot, &full[slot]);
+    };
     if (warp == kSoftWarps) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sx_smem(tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -344,24 +366,32 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
         for (int i = 0; i < kSlots; i++) { sx_bar_init(&full[i], 1); sx_bar_init(&freeb[i], 1); }
         for (int i = 0; i < 2; i++) { sx_bar_init(&s_ready[i], 1); sx_bar_init(&p_ready[i], 4); sx_bar_init(&d_ready[i], 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        // the ring's first fill: nothing to wait for but the pack kernel
+        pdl_wait();
+        for (uint32_t i = 0; i < kSlots && i < items; i++) copy(i);
     }
-    // The query rows, scaled, split, stored as the A operand.  A warp takes 16 rows, eight at a time, four lanes to a row:
-    // 64 bytes of each of eight rows a load, and stores that meet every bank twice
     const uint32_t r = tid & (kRows - 1);
     const bool live = r < tokens * group;
     float *row_scale = reinterpret_cast<float *>(smem + Smem::kScale);
+    // The query rows, scaled, split, stored as the A operand.  A warp takes 16 rows, eight at a time, four lanes to a row:
+    // 64 bytes of each of eight rows a load, and stores that meet every bank twice
     if (warp < kSoftWarps) {
         const uint32_t at = (lane & 3) * 4;
+        float4 both[2][DP / 16];                         // all on their way at once
 #pragma unroll
         for (int g = 0; g < 2; g++) {
             const uint32_t row = warp * 16 + g * 8 + (lane >> 2);
             const bool on = row < tokens * group;
             const float *q = p.q + ((uint64_t)(tok0 + (on ? row / group : 0)) * p.q_heads + (kvh0 + kv) * group + (on ? row % group : 0)) * D;
-            float4 x[DP / 16];
-            float amax = 0.f;
 #pragma unroll
             for (int i = 0; i < DP / 16; i++)
-                x[i] = on && 16 * i + at < D ? __ldg(reinterpret_cast<const float4 *>(q + 16 * i + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                both[g][i] = on && 16 * i + at < D ? __ldg(reinterpret_cast<const float4 *>(q + 16 * i + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const uint32_t row = warp * 16 + g * 8 + (lane >> 2);
+            const float4 (&x)[DP / 16] = both[g];
+            float amax = 0.f;
 #pragma unroll
             for (int i = 0; i < DP / 16; i++)
                 amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
@@ -389,34 +419,23 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
-    pdl_wait();                                          // the tiles are packed
     // 168 registers a thread at launch; the softmax groups take what the other four warps do not need:
     // 2 x 128 x 224 + 128 x 56 = 384 x 168
     if (warp >= kSoftWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == kSoftWarps + 1) {
-            // ---- the copies, in the order the MMAs take them: K(0) K(1) V(0) K(2) V(1) ...
+            // ---- the copies that do not fit at once
             if (lane == 0) {
-                uint32_t slot = 0, use = 0, issued = 0;
                 bool ok = true;
-                const auto load = [&](uint32_t i, uint32_t which) {
-                    for (int part = 0; part < kP && ok; part++) {
-                        if (use) ok = bar_wait(&freeb[slot], (use - 1) & 1);
-                        if (!ok) return;
-                        sx_bar_expect_tx(&full[slot], kSlot);
-                        sx_bulk_load(smem + Smem::kRing + slot * kSlot,
-                                     tiles + (size_t)tile_of(i) * kTileBytes<T, DP> + (which * kP + part) * kSlot, kSlot, &full[slot]);
-                        issued++;
-                        if (++slot == kSlots) { slot = 0; use++; }
-                    }
-                };
-                if (n) load(0, 0);
-                for (uint32_t i = 0; i < n && ok; i++) {
-                    if (i + 1 < n) load(i + 1, 0);
-                    load(i, 1);
+                uint32_t i = kSlots;
+                for (; i < items && ok; i++) {
+                    ok = bar_wait(&freeb[i % kSlots], (i / kSlots - 1) & 1);
+                    if (ok) copy(i);
                 }
                 // nothing may be in flight when the CTA's shared memory goes to another
-                for (uint32_t i = issued > kSlots ? issued - kSlots : 0; i < issued; i++) bar_wait(&full[i % kSlots], (i / kSlots) & 1);
+                const uint32_t issued = ok ? max(i, min(items, (uint32_t)kSlots)) : i - 1;
+                const uint32_t last = min(issued, items);
+                for (uint32_t k = last > kSlots ? last - kSlots : 0; k < last; k++) bar_wait(&full[k % kSlots], (k / kSlots) & 1);
             }
         } else if (warp == kSoftWarps) {
             // ---- the MMAs
@@ -480,6 +499,7 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
         }
     } else {
         // ---- the softmax of every other tile; a thread has a row
+        pdl_wait();                                      // (for what follows of the pack kernel's)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const float q_scale = row_scale[r];
         float m = -CUDART_INF_F, l = 0.f, o[DP];
@@ -662,28 +682,40 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
             }
         } else {
             // (the warp's rows are shared out too: every CTA of the cluster writes some of them)
-            float M = -CUDART_INF_F, sum = 0.f;
-            for (uint32_t c = 0; c < split; c++) M = fmaxf(M, ld_cluster(sx_smem(total + mine), c));
-            for (uint32_t c = 0; c < split; c++) {
-                const float m = ld_cluster(sx_smem(total + mine), c), f = m == -CUDART_INF_F ? 0.f : ab_ex2(m - M);
-                sum = fmaf(ld_cluster(sx_smem(total + kRows + mine), c), f, sum);
-            }
-            const float inv = 1.f / sum;
-            const uint32_t some = kWarpRows / split;                // split is 2, 4 or 8
-#pragma unroll 2
-            for (uint32_t i = part * some; i < (part + 1) * some; i += kTogether) {
-                const uint32_t row = i + lane / kLanes, at = __shfl_sync(0xffffffffu, to, row);
-                const float g = __shfl_sync(0xffffffffu, inv, row), top = __shfl_sync(0xffffffffu, M, row);
-                const uint32_t r0 = warp * kWarpRows + row;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (uint32_t c = 0; c < split; c++) {
-                    const float m = ld_cluster(sx_smem(total + r0), c), f = m == -CUDART_INF_F ? 0.f : ab_ex2(m - top);
-                    const float4 y = ld_cluster4(sx_smem(rows + r0 * kPitch + d), c);
-                    x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
+            const auto join = [&](auto cs) {
+                constexpr uint32_t S = decltype(cs)::value, kSome = kWarpRows / S;
+                float m[S], l[S], M = -CUDART_INF_F, sum = 0.f;
+#pragma unroll
+                for (uint32_t c = 0; c < S; c++) {
+                    m[c] = ld_cluster(sx_smem(total + mine), c);
+                    l[c] = ld_cluster(sx_smem(total + kRows + mine), c);
                 }
-                if (at != 0xffffffffu && d < D)
-                    *reinterpret_cast<float4 *>(out + (uint64_t)at * D + d) = make_float4(x.x * g, x.y * g, x.z * g, x.w * g);
-            }
+#pragma unroll
+                for (uint32_t c = 0; c < S; c++) M = fmaxf(M, m[c]);
+#pragma unroll
+                for (uint32_t c = 0; c < S; c++) {
+                    m[c] = m[c] == -CUDART_INF_F ? 0.f : ab_ex2(m[c] - M);
+                    sum = fmaf(l[c], m[c], sum);
+                }
+#pragma unroll
+                for (uint32_t c = 0; c < S; c++) m[c] /= sum;
+#pragma unroll
+                for (uint32_t i = 0; i < kSome; i += kTogether) {
+                    const uint32_t row = part * kSome + i + lane / kLanes, at = __shfl_sync(0xffffffffu, to, row);
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y[S];
+#pragma unroll
+                    for (uint32_t c = 0; c < S; c++) y[c] = ld_cluster4(sx_smem(rows + (warp * kWarpRows + row) * kPitch + d), c);
+#pragma unroll
+                    for (uint32_t c = 0; c < S; c++) {
+                        const float f = __shfl_sync(0xffffffffu, m[c], row);
+                        x.x = fmaf(y[c].x, f, x.x); x.y = fmaf(y[c].y, f, x.y); x.z = fmaf(y[c].z, f, x.z); x.w = fmaf(y[c].w, f, x.w);
+                    }
+                    if (at != 0xffffffffu && d < D) *reinterpret_cast<float4 *>(out + (uint64_t)at * D + d) = x;
+                }
+            };
+            if (split == 2) join(std::integral_constant<uint32_t, 2>());
+            else if (split == 4) join(std::integral_constant<uint32_t, 4>());
+            else join(std::integral_constant<uint32_t, 8>());
         }
     }
     if (split > 1) cluster_sync();                       // nobody leaves while its parts are being read
@@ -707,7 +739,7 @@ template <typename T, int DP> int tile_prepare(const char *name)
 // A ragged step: the sequences with at least `from` rows (tokens x heads of a group) become segments, the rows of the
 // others, and those behind the last sequence, are left to the row kernel (WinParams::left).  One block.
 __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32_t from, uint32_t max_segments, Segment *segments,
-                                                       uint2 *key_tiles, uint2 *row_tiles, uint32_t *counts, uint32_t max_key_tiles,
+                                                       uint4 *key_tiles, uint2 *row_tiles, uint32_t *counts, uint32_t max_key_tiles,
                                                        uint32_t max_row_tiles, uint4 *left)
 {
     __shared__ uint4 part[8];
@@ -751,10 +783,11 @@ __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32
         if (mine.x && at.x < max_segments && (uint64_t)at.y + mine.y <= max_key_tiles && (uint64_t)at.z + mine.z <= max_row_tiles) {
             g.tile0 = at.y;
             segments[at.x] = g;
-            for (uint32_t i = 0; i < mine.y; i++) key_tiles[at.y + i] = make_uint2(at.x, i);
+            for (uint32_t i = 0; i < mine.y; i++)
+                key_tiles[at.y + i] = make_uint4(win_tile_start(g, i), i < g.sink_tiles ? g.ns : g.end, s, 0);
             for (uint32_t i = 0; i < mine.z; i++) row_tiles[at.z + i] = make_uint2(at.x, i);
         } else if (mine.x) {
-            for (uint32_t i = at.y; i < max_key_tiles && i - at.y < mine.y; i++) key_tiles[i] = make_uint2(0xffffffffu, 0);
+            for (uint32_t i = at.y; i < max_key_tiles && i - at.y < mine.y; i++) key_tiles[i] = make_uint4(0, 0, 0, 0);
             for (uint32_t i = at.z; i < max_row_tiles && i - at.z < mine.z; i++) row_tiles[i] = make_uint2(0xffffffffu, 0);
         }
         for (uint32_t i = 0; i < mine.w && at.w + i < p.rows; i++) {
@@ -796,7 +829,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
     const uint64_t per_head = std::max<uint64_t>(1, key_tiles) * kTileBytes<T, DP>;
     const uint32_t pass = (uint32_t)std::min<uint64_t>(p.kv_heads, std::max<uint64_t>(1, kPassBytes / per_head));
     const size_t head_bytes = align_up((size_t)(pass * key_tiles) * sizeof(TileHead), 256);
-    const size_t seg_bytes = align_up((size_t)segments * sizeof(Segment), 256), key_bytes = ragged ? align_up((size_t)key_tiles * 8, 256) : 0;
+    const size_t seg_bytes = align_up((size_t)segments * sizeof(Segment), 256), key_bytes = ragged ? align_up((size_t)key_tiles * 16, 256) : 0;
     const size_t row_bytes = ragged ? align_up((size_t)row_tiles * 8, 256) : 0, left_bytes = ragged ? align_up((size_t)p.rows * 16 + 32, 256) : 0;
     l.ws_need = seg_bytes + key_bytes + row_bytes + left_bytes + head_bytes + (size_t)(pass * per_head);
     if (row_tiles * pass > 0x7fffffffull || key_tiles > 0x7fffffffull || pass > 65535)
@@ -811,7 +844,8 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
     plan.max_row_tiles = (uint32_t)row_tiles;
     if (ragged) {
         Segment *segs = reinterpret_cast<Segment *>(ws);
-        uint2 *kt = reinterpret_cast<uint2 *>(ws + seg_bytes), *rt = reinterpret_cast<uint2 *>(ws + seg_bytes + key_bytes);
+        uint4 *kt = reinterpret_cast<uint4 *>(ws + seg_bytes);
+        uint2 *rt = reinterpret_cast<uint2 *>(ws + seg_bytes + key_bytes);
         uint32_t *counts = reinterpret_cast<uint32_t *>(ws + seg_bytes + key_bytes + row_bytes);
         plan.segments = segs;
         plan.key_tiles = kt;
