@@ -60,6 +60,14 @@ int run_copy(cudaStream_t stream, void *const *caches, int n_caches, uint64_t pa
     return AB_OK;
 }
 
+// 2 KB of parameters for the few pairs of a fork, 29 KB of the 32 that a launch may have for a compaction's
+template <typename V>
+int run_copy(cudaStream_t stream, void *const *caches, int n_caches, uint64_t page_bytes, const uint32_t *src, const uint32_t *dst, int n_pairs)
+{
+    return n_pairs <= 96 ? run_copy<V, 96>(stream, caches, n_caches, page_bytes, src, dst, n_pairs)
+                         : run_copy<V, 3500>(stream, caches, n_caches, page_bytes, src, dst, n_pairs);
+}
+
 }  // namespace
 }  // namespace ab
 
@@ -78,26 +86,34 @@ extern "C" int ab_cache_copy_pages(void *stream, void *const *caches, int n_cach
         if (!caches[c]) return fail(AB_ERR_INVALID, "ab_cache_copy_pages: cache %d is NULL", c);
         align |= reinterpret_cast<uintptr_t>(caches[c]);
     }
-    // one pass in no particular order is a copy only if no page is written twice or written and read
-    std::vector<uint32_t> d;
-    try {
-        d.assign(dst, dst + n_pairs);
-    } catch (const std::bad_alloc &) {
-        return fail(AB_ERR_OOM, "ab_cache_copy_pages: host allocation failed");
-    }
-    std::sort(d.begin(), d.end());
+    // One pass in no particular order is a copy only if no page is written twice, or both written and read.  A bit per page
+    // says what is written; it is laid out for the pages between the smallest and the largest destination
+    uint32_t low = 0xffffffffu, high = 0;
     for (int i = 0; i < n_pairs; i++) {
         if (src[i] >= pages || dst[i] >= pages)
             return fail(AB_ERR_INVALID, "ab_cache_copy_pages: pair %d copies page %u to page %u of a cache of %u pages", i,
                         src[i], dst[i], pages);
-        if (i && d[(size_t)i] == d[(size_t)i - 1])
-            return fail(AB_ERR_INVALID, "ab_cache_copy_pages: page %u is written twice", d[(size_t)i]);
-        if (std::binary_search(d.begin(), d.end(), src[i]))
-            return fail(AB_ERR_INVALID, "ab_cache_copy_pages: page %u is both read and written", src[i]);
+        low = std::min(low, dst[i]);
+        high = std::max(high, dst[i]);
     }
+    std::vector<uint64_t> written;
+    try {
+        written.assign((size_t)(high - low) / 64 + 1, 0);
+    } catch (const std::bad_alloc &) {
+        return fail(AB_ERR_OOM, "ab_cache_copy_pages: host allocation failed");
+    }
+    for (int i = 0; i < n_pairs; i++) {
+        uint64_t &w = written[(dst[i] - low) / 64];
+        const uint64_t bit = 1ull << ((dst[i] - low) % 64);
+        if (w & bit) return fail(AB_ERR_INVALID, "ab_cache_copy_pages: page %u is written twice", dst[i]);
+        w |= bit;
+    }
+    for (int i = 0; i < n_pairs; i++)
+        if (src[i] >= low && src[i] <= high && (written[(src[i] - low) / 64] >> ((src[i] - low) % 64) & 1))
+            return fail(AB_ERR_INVALID, "ab_cache_copy_pages: page %u is both read and written", src[i]);
     if (n_caches == 0) return AB_OK;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (align % 16 == 0) return run_copy<uint4, 128>(s, caches, n_caches, page_bytes, src, dst, n_pairs);
-    if (align % 4 == 0) return run_copy<uint32_t, 128>(s, caches, n_caches, page_bytes, src, dst, n_pairs);
-    return run_copy<uint8_t, 128>(s, caches, n_caches, page_bytes, src, dst, n_pairs);
+    if (align % 16 == 0) return run_copy<uint4>(s, caches, n_caches, page_bytes, src, dst, n_pairs);
+    if (align % 4 == 0) return run_copy<uint32_t>(s, caches, n_caches, page_bytes, src, dst, n_pairs);
+    return run_copy<uint8_t>(s, caches, n_caches, page_bytes, src, dst, n_pairs);
 }

@@ -151,17 +151,13 @@ def launch(name: str, bindings: Sequence[torch.Tensor], uniform: Optional[bytes]
     _lib.check(rc)
 
 
-_arrays: dict = {}      # ctypes array types by (element type, length): making one costs more than filling it
 # the current stream's handle without the Stream object around it, where torch offers that
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _array(kind, values):
-    n = len(values)
-    t = _arrays.get((kind, n))
-    if t is None:
-        t = _arrays.setdefault((kind, n), kind * n)
-    return t(*values)
+# a call's pointers and lengths as the bytes of C arrays, by how many there are
+_pointers = [struct.Struct(f"{n}Q").pack for n in range(16)]
+_counts = [struct.Struct(f"{n}I").pack for n in range(16)]
 
 
 def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: bytes, scratch: bool = False):
@@ -180,7 +176,7 @@ def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: b
     for t in bindings:
         n = 0 if t is None else t.numel()
         if n == 0:
-            ptrs.append(None)
+            ptrs.append(0)
             lens.append(0)
             continue
         if t.device != dev or not t.is_contiguous():
@@ -192,14 +188,15 @@ def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: b
         ws_bytes = workspace_bytes(name, lens, uniform)
         if ws_bytes:
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    rc = _lib.lib().ab_launch(name.encode(), _raw_stream(dev.index), _array(C.c_void_p, ptrs), _array(C.c_uint32, lens),
-                              len(ptrs), uniform, len(uniform), ws.data_ptr() if ws is not None else None, ws_bytes)
+    count = len(ptrs)
+    rc = _lib.lib().ab_launch(name.encode(), _raw_stream(dev.index), _pointers[count](*ptrs), _counts[count](*lens), count,
+                              uniform, len(uniform), ws.data_ptr() if ws is not None else None, ws_bytes)
     if rc:
         _lib.check(rc)
 
 
-def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int], block: int):
-    """ab_cache_copy_pages on the current stream of the caches' device."""
+def copy_pages(caches: Sequence[torch.Tensor], pointers: Sequence[int], src: Sequence[int], dst: Sequence[int], block: int):
+    """ab_cache_copy_pages on the current stream of the caches' device; pointers: the caches' addresses."""
     t, n = caches[0], len(src)
     dev = t.device
     if dev.type != "cuda":
@@ -207,16 +204,18 @@ def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
                               "device and has no CPU path")
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return copy_pages(caches, src, dst, block)
-    if n and (min(src) < 0 or min(dst) < 0 or max(src) > 0xffffffff or max(dst) > 0xffffffff):
-        raise _lib.AccelError(_lib.AB_ERR_INVALID, "copy_pages: a page id is u32")
+            return copy_pages(caches, pointers, src, dst, block)
     page_bytes = t.numel() // t.shape[0] * t.element_size() * block if t.numel() else 0
     if page_bytes == 0:
         if n:
             raise _lib.AccelError(_lib.AB_ERR_INVALID, "copy_pages: the caches are empty")
         return
-    rc = _lib.lib().ab_cache_copy_pages(_raw_stream(dev.index), _array(C.c_void_p, [c.data_ptr() for c in caches]), len(caches),
-                                        page_bytes, t.shape[0] // block, (C.c_uint32 * n)(*src), (C.c_uint32 * n)(*dst), n)
+    try:
+        s, d = struct.pack(f"{n}I", *src), struct.pack(f"{n}I", *dst)
+    except struct.error as e:
+        raise _lib.AccelError(_lib.AB_ERR_INVALID, f"copy_pages: a page id is u32: {e}") from None
+    rc = _lib.lib().ab_cache_copy_pages(_raw_stream(dev.index), struct.pack(f"{len(pointers)}Q", *pointers), len(pointers),
+                                        page_bytes, t.shape[0] // block, s, d, n)
     if rc:
         _lib.check(rc)
 

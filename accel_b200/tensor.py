@@ -585,17 +585,18 @@ def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
         return
     first = caches[0]
     shape, dtype, device = first.shape, first.dtype, first.device
-    seen = set()
+    if not shape:
+        raise Refused(op, "a cache is a scalar; it is [capacity, ...]")
     for c in caches:
-        if c.dim() < 1 or c.shape != shape or c.dtype != dtype or c.device != device:
-            raise Refused(op, f"the caches are {tuple(first.shape)} {first.dtype} on {first.device} and {tuple(c.shape)} "
-                          f"{c.dtype} on {c.device}; one call copies in caches of one form")
+        if c.shape != shape or c.dtype != dtype or c.device != device:
+            raise Refused(op, f"the caches are {tuple(shape)} {dtype} on {device} and {tuple(c.shape)} {c.dtype} on "
+                          f"{c.device}; one call copies in caches of one form")
         if not c.is_contiguous():
             raise Refused(op, "a cache is a strided view; pages are copied in place, so it is contiguous")
-        seen.add(c.data_ptr())
-    if len(seen) != len(caches) and first.numel():
+    pointers = [c.data_ptr() for c in caches]
+    if len(set(pointers)) != len(caches) and first.numel():
         raise Refused(op, "a cache is named twice")
-    rt.copy_pages(caches, src, dst, block)
+    rt.copy_pages(caches, pointers, src, dst, block)
 
 
 # ------------------------------------------------------------------------------- log probabilities
