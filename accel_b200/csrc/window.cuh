@@ -53,8 +53,25 @@ __device__ __forceinline__ void cluster_sync()
 }
 #endif
 
-// query rows (tokens x heads of a KV head) of one sequence from which 128-row tiles take over
-constexpr uint32_t kTileFrom = 64;
+// Whether `rows` query rows (tokens x heads of a KV head) of one sequence, each of which sees up to `seen` positions, go
+// on 128-row tiles.  A tile call costs its two launches and the packing of the positions, whatever the rows; the row
+// kernel's time grows with rows x seen.  (8 KV heads, head dimension 128; tiles / rows one by one, us:
+//     rows x seen           f32, groups of 4      f16, groups of 4      f16, groups of 8 (4 KV heads)
+//       32 x   512          20.8 /  11.5          17.8 /  11.9          17.7 /  10.3
+//       64 x   512          21.4 /  15.7          17.7 /  13.7          17.7 /  10.5
+//      128 x   512          21.7 /  22.8          17.7 /  18.8          17.6 /  13.6
+//      256 x   512          21.7 /  46.7          18.5 /  25.0          17.7 /  15.7
+//       16 x  4096          35.0 /  24.9          29.0 /  28.8          24.0 /  15.7
+//       32 x  4096          35.3 /  42.7          29.0 /  26.9          23.9 /  17.7
+//       64 x  4096          35.7 /  85.6          29.3 /  44.1          24.2 /  31.1
+//       16 x 32768         185.5 / 147.0         147.7 / 123.2         103.8 /  57.8
+//       32 x 32768         185.4 / 319.5         147.9 / 144.7         103.4 /  67.8
+//       64 x 32768         186.0 / 587.2         148.7 / 278.6         104.3 / 125.3 )
+constexpr uint32_t kTileFrom = 32;
+__host__ __device__ inline bool on_tiles(uint64_t rows, uint64_t seen)
+{
+    return rows >= 256 || (rows >= kTileFrom && rows * seen >= 65536);
+}
 // a prefill, or the sequences of a ragged step that have that many rows (it then sets p.left), on 128-row tiles
 // (window_prefill.cu); p.q_heads / p.kv_heads <= 128
 int run_window_tiles(Launch &l, WinParams &p, bool f16, const char *name);

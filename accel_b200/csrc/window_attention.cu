@@ -739,7 +739,12 @@ template <typename T> int run_window(Launch &l, WinParams &p, const char *name)
     l.ws_need = 0;
     if (p.rows == 0) return AB_OK;
     const uint32_t group = p.q_heads / p.kv_heads;
-    if ((p.form == kPrefillRows || p.form == kRaggedStep) && group <= 128 && (uint64_t)p.rows * group >= kTileFrom) {
+    // (the device alone knows how a ragged step's rows are dealt out; with one or more to each sequence, the most that one
+    // has is what the host assumes, and a step of single tokens needs no plan: 16 of them over 1024 positions take 29.6 us of the
+    // row kernel's time, and took 7.0 us more of kernels without work)
+    const uint64_t most = p.form == kPrefillRows ? p.rows : (p.form == kRaggedStep && p.rows >= p.batch ? p.rows - p.batch + 1 : 0);
+    const uint64_t seen = std::min<uint64_t>((uint64_t)p.window + p.sinks, p.form == kPrefillRows ? std::min<uint64_t>((uint64_t)p.base + p.rows, p.reach) : p.reach);
+    if (group <= 128 && on_tiles(most * group, seen)) {
         const int rc = run_window_tiles(l, p, sizeof(T) == 2, name);
         if (rc || p.form == kPrefillRows) return rc;
     }

@@ -736,28 +736,30 @@ template <typename T, int DP> int tile_prepare(const char *name)
 }
 
 // ------------------------------------------------------------------------------------------------
-// A ragged step: the sequences with at least `from` rows (tokens x heads of a group) become segments, the rows of the
-// others, and those behind the last sequence, are left to the row kernel (WinParams::left).  One block.
-__global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32_t from, uint32_t max_segments, Segment *segments,
+// A ragged step: the sequences whose rows pay for tiles (on_tiles) become segments, as many of the first as there is room
+// for; the rows of the others, and those behind the last sequence, are left to the row kernel (WinParams::left).  One block.
+__global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32_t max_segments, Segment *segments,
                                                        uint4 *key_tiles, uint2 *row_tiles, uint32_t *counts, uint32_t max_key_tiles,
                                                        uint32_t max_row_tiles, uint4 *left)
 {
     __shared__ uint4 part[8];
+    __shared__ uint32_t part_left[8];
     const uint32_t t = threadIdx.x, lane = t & 31, group = p.q_heads / p.kv_heads, per_tile = kRows / group;
     uint4 before = make_uint4(0, 0, 0, 0);               // segments, key tiles, row tiles, rows left of the sequences so far
     for (uint32_t s0 = 0; s0 < p.batch; s0 += 256) {
         const uint32_t s = s0 + t;
         Segment g{};
         uint4 mine = make_uint4(0, 0, 0, 0);
-        uint32_t first = 0, len = 0, count = 0;
+        uint32_t first = 0, len = 0, count = 0, mine_left = 0;
         if (s < p.batch) {
             const uint32_t a = min(p.offsets[s], p.rows), b = min(p.offsets[s + 1], p.rows);
             len = p.lengths[s];
             first = a;
             count = p.offsets[s + 1] - p.offsets[s];
-            mine.w = b > a ? b - a : 0;
+            mine_left = b > a ? b - a : 0;
             // (a sequence with more tokens than positions has rows of zeros: the row kernel knows)
-            if (b > a && b == p.offsets[s + 1] && (uint64_t)(b - a) * group >= from && len >= b - a) {
+            if (b > a && b == p.offsets[s + 1] && len >= b - a &&
+                on_tiles((uint64_t)(b - a) * group, min((uint64_t)p.window + p.sinks, (uint64_t)min(len, p.reach)))) {
                 g.row0 = a; g.rows = b - a; g.base = len - (b - a); g.seq = s;
                 g.end = min(len, p.reach);
                 segment_list(g, p.window, p.sinks);
@@ -768,19 +770,20 @@ __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32
 #pragma unroll
         for (int w = 1; w < 32; w *= 2) {
             const uint32_t x = __shfl_up_sync(0xffffffffu, sum.x, w), y = __shfl_up_sync(0xffffffffu, sum.y, w),
-                           z = __shfl_up_sync(0xffffffffu, sum.z, w), u = __shfl_up_sync(0xffffffffu, sum.w, w);
-            if (lane >= (uint32_t)w) { sum.x += x; sum.y += y; sum.z += z; sum.w += u; }
+                           z = __shfl_up_sync(0xffffffffu, sum.z, w);
+            if (lane >= (uint32_t)w) { sum.x += x; sum.y += y; sum.z += z; }
         }
         if (lane == 31) part[t >> 5] = sum;
         __syncthreads();
         uint4 at = before;
         for (uint32_t w = 0; w < 8; w++) {
-            if (w < t >> 5) { at.x += part[w].x; at.y += part[w].y; at.z += part[w].z; at.w += part[w].w; }
-            before.x += part[w].x; before.y += part[w].y; before.z += part[w].z; before.w += part[w].w;
+            if (w < t >> 5) { at.x += part[w].x; at.y += part[w].y; at.z += part[w].z; }
+            before.x += part[w].x; before.y += part[w].y; before.z += part[w].z;
         }
-        at.x += sum.x - mine.x; at.y += sum.y - mine.y; at.z += sum.z - mine.z; at.w += sum.w - mine.w;
-        // (the host's bounds hold for all offsets that ascend, as a prefix sum's do; with others no tile is given away twice)
+        at.x += sum.x - mine.x; at.y += sum.y - mine.y; at.z += sum.z - mine.z;
+        // (once one does not fit none behind it does: the sums go on)
         if (mine.x && at.x < max_segments && (uint64_t)at.y + mine.y <= max_key_tiles && (uint64_t)at.z + mine.z <= max_row_tiles) {
+            mine_left = 0;
             g.tile0 = at.y;
             segments[at.x] = g;
             for (uint32_t i = 0; i < mine.y; i++)
@@ -790,10 +793,23 @@ __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32
             for (uint32_t i = at.y; i < max_key_tiles && i - at.y < mine.y; i++) key_tiles[i] = make_uint4(0, 0, 0, 0);
             for (uint32_t i = at.z; i < max_row_tiles && i - at.z < mine.z; i++) row_tiles[i] = make_uint2(0xffffffffu, 0);
         }
-        for (uint32_t i = 0; i < mine.w && at.w + i < p.rows; i++) {
+        uint32_t sum_left = mine_left;
+#pragma unroll
+        for (int w = 1; w < 32; w *= 2) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, sum_left, w);
+            if (lane >= (uint32_t)w) sum_left += x;
+        }
+        if (lane == 31) part_left[t >> 5] = sum_left;
+        __syncthreads();
+        uint32_t at_left = before.w + sum_left - mine_left;
+        for (uint32_t w = 0; w < 8; w++) {
+            if (w < t >> 5) at_left += part_left[w];
+            before.w += part_left[w];
+        }
+        for (uint32_t i = 0; i < mine_left && at_left + i < p.rows; i++) {
             // (the first tokens of a sequence with fewer positions than tokens have none)
             const uint64_t pos1 = (uint64_t)len + i + 1;
-            left[1 + at.w + i] = make_uint4(first + i, pos1 > count ? s : 0xffffffffu, (uint32_t)(pos1 - count), len);
+            left[1 + at_left + i] = make_uint4(first + i, pos1 > count ? s : 0xffffffffu, (uint32_t)(pos1 - count), len);
         }
         __syncthreads();
     }
@@ -803,7 +819,7 @@ __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32
     if (t == 0) { counts[0] = min(before.y, max_key_tiles); counts[1] = min(before.z, max_row_tiles); }
 }
 
-constexpr uint64_t kPassBytes = 1ull << 30;              // tiles of one pass over KV heads
+constexpr uint64_t kPassBytes = 1ull << 30;              // tiles of one pass over KV heads; a prefill takes more where one head's list does
 
 template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char *name)
 {
@@ -817,6 +833,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
         // at most: a segment has kTileFrom rows; its list ends in two unfilled tiles, its rows in one
         segments = std::min<uint64_t>(p.batch, (uint64_t)p.rows * group / kTileFrom);
         key_tiles = segments * ((uint64_t)std::min(p.sinks, p.reach) / kKeys + std::min<uint64_t>(p.window, p.reach) / kKeys + 3) + p.rows / kKeys;
+        key_tiles = std::min<uint64_t>(key_tiles, kPassBytes / kTileBytes<T, DP>);      // (long lists: the plan stops where they are full)
         row_tiles = segments + p.rows / per_tile;
     } else {
         plan.one.rows = p.rows;
@@ -853,7 +870,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
         plan.counts = counts;
         uint4 *left = reinterpret_cast<uint4 *>(counts + 4);
         p.left = left;
-        win_plan_kernel<<<1, 256, 0, l.stream>>>(p, kTileFrom, (uint32_t)segments, segs, kt, rt, counts, plan.max_key_tiles,
+        win_plan_kernel<<<1, 256, 0, l.stream>>>(p, (uint32_t)segments, segs, kt, rt, counts, plan.max_key_tiles,
                                                  plan.max_row_tiles, left);
         count_launch();
         rc = check_cuda(cudaGetLastError(), name);

@@ -378,3 +378,56 @@ def test_ragged_chunks_in_graphs_on_two_streams():
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(o.cpu(), w) for o, w in zip(outs, want))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("tokens,n,tiles", [(31, 2112, False), (32, 2111, True), (32, 1900, False), (255, 255, False), (256, 256, True)])
+def test_prefill_on_either_side_of_the_choice_of_kernel(tokens, n, tiles, f16):
+    kv, D, window, sinks = 2, 64, 2044, 4                         # 32 rows x 2048 positions, or 256 rows
+    rng = np.random.default_rng(tokens)
+    k, v = (rng.standard_normal((n, kv, D)).astype(np.float16 if f16 else np.float32) for _ in range(2))
+    q = rng.standard_normal((tokens, kv, D)).astype(np.float32)
+    got = T.attention(dev(q), dev(k), dev(v), T.AttentionOptions(
+        lengths=dev(np.array([n], np.uint32)), scale=attn_scale(D), base=n - tokens, window=window, sinks=sinks)).cpu().numpy()
+    assert ("tcgen05 tiles" in rt.last_selection()) == tiles
+    for i in range(0, tokens, 5):
+        check(got[i], *attend(q[i], k, v, visible(n - tokens + i, n, window, sinks), attn_scale(D), 1), f"row {i}")
+
+
+def test_ragged_steps_of_single_tokens_take_one_launch():
+    qH, kv, D, block, batch = 8, 2, 64, 8, 40
+    rng = np.random.default_rng(1)
+    lengths = rng.integers(1, 100, batch)
+    c = Cache(4, kv, D, block, lengths.tolist(), (lengths - 1).tolist(), 50, 2, False)
+    for counts in (np.ones(batch, np.int64), np.where(np.arange(batch) == 11, 30, np.arange(batch) % 4 == 0)):
+        q = rng.standard_normal((int(counts.sum()), qH, D)).astype(np.float32)
+        lens = np.maximum(lengths, counts)
+        c = Cache(4, kv, D, block, lens.tolist(), (lens - counts).tolist(), 50, 2, False)
+        got = T.attention(dev(q), dev(c.pk), dev(c.pv), T.AttentionOptions(
+            lengths=dev(lens.astype(np.uint32)), pages=dev(c.pages), block=block, scale=attn_scale(D),
+            query_extents=dev(counts.astype(np.uint32)), window=50, sinks=2)).cpu().numpy()
+        r = 0
+        for b, (n, m) in enumerate(zip(lens.tolist(), counts.tolist())):
+            for i in range(m):
+                check(got[r], *attend(q[r], c.k[b], c.v[b], visible(n - m + i, n, 50, 2), attn_scale(D), qH // kv), f"{b} {i}")
+                r += 1
+
+
+def test_ragged_lists_longer_than_the_tiles_there_is_room_for():
+    # twelve sequences over one shared cache: 12 x 100000 positions are more than the 8192 tiles of 128 a pass packs
+    # (f32, head dimension 128), so that the last chunks go row by row
+    qH, D, block, batch, n, m = 8, 128, 16, 12, 100000, 40
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    k, v = (torch.randn((n, 1, D), device=DEV, generator=gen) for _ in range(2))
+    q = torch.randn((batch * m, qH, D), device=DEV, generator=gen)
+    table = torch.arange(n // block, dtype=torch.int32, device=DEV).expand(batch, -1).contiguous()
+    lengths = np.arange(n - batch + 1, n + 1).astype(np.uint32)
+    got = T.attention(q, k, v, T.AttentionOptions(
+        lengths=dev(lengths), pages=table, block=block, scale=attn_scale(D), query_extents=dev(np.full(batch, m, np.uint32)),
+        window=n, sinks=0)).cpu().numpy()
+    hq, hk, hv = q.cpu().numpy(), k.cpu().numpy(), v.cpu().numpy()
+    for b in (0, 5, 9, 10, 11):
+        for i in (0, m - 1):
+            r = b * m + i
+            check(got[r], *attend(hq[r], hk, hv, visible(int(lengths[b]) - m + i, int(lengths[b]), n, 0), attn_scale(D), qH), f"{b} {i}")
+    rt.attention_error()
