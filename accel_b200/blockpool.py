@@ -96,7 +96,12 @@ class BlockPool:
 
     def compact(self, rows: Sequence[Sequence[int]]) -> Tuple[List[List[int]], List[int], List[int]]:
         """Moves the held pages to the lowest numbers.  `rows` are all the page rows in use; returns them
-        rewritten, and (src, dst), the copies to make before anything is read through them."""
+        rewritten, and (src, dst), the copies to make before anything is read through them.  A page that
+        is held and in none of the rows is refused: its row could not be rewritten."""
+        held = {p for row in rows for p in row if p != self.NONE}
+        if len(held) != self._blocks - self.available():
+            raise _lib.AccelError(_lib.AB_ERR_INVALID, f"the rows name {len(held)} pages and {self._blocks - self.available()} "
+                                  "are held; a compaction moves them all, so it needs every row in use")
         src, dst = np.zeros(self._blocks, np.uint32), np.zeros(self._blocks, np.uint32)
         n = _lib.check(_lib.lib().ab_blockpool_compact(self._h, src.ctypes.data, dst.ctypes.data))
         to = {int(s): int(d) for s, d in zip(src[:n], dst[:n])}

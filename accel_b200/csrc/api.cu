@@ -1069,8 +1069,13 @@ int ab_blockpool_new(int blocks, int per, ab_blockpool **out)
     ab_blockpool *p = new (std::nothrow) ab_blockpool();
     if (!p) return fail(AB_ERR_OOM, "ab_blockpool_new: host allocation failed");
     p->block = per; p->total = blocks;
-    p->free_list.resize((size_t)blocks);
-    p->refs.assign((size_t)blocks, 0);
+    try {
+        p->free_list.resize((size_t)blocks);
+        p->refs.assign((size_t)blocks, 0);
+    } catch (const std::bad_alloc &) {
+        delete p;
+        return fail(AB_ERR_OOM, "a pool of %d blocks: host allocation failed", blocks);
+    }
     for (int i = 0; i < blocks; i++) p->free_list[(size_t)i] = (uint32_t)(blocks - 1 - i);
     *out = p;
     return AB_OK;

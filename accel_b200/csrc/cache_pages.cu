@@ -97,8 +97,10 @@ extern "C" int ab_cache_copy_pages(void *stream, void *const *caches, int n_cach
         high = std::max(high, dst[i]);
     }
     std::vector<uint64_t> written;
+    std::vector<uintptr_t> starts;
     try {
         written.assign((size_t)(high - low) / 64 + 1, 0);
+        starts.resize((size_t)n_caches);
     } catch (const std::bad_alloc &) {
         return fail(AB_ERR_OOM, "ab_cache_copy_pages: host allocation failed");
     }
@@ -112,6 +114,11 @@ extern "C" int ab_cache_copy_pages(void *stream, void *const *caches, int n_cach
         if (src[i] >= low && src[i] <= high && (written[(src[i] - low) / 64] >> ((src[i] - low) % 64) & 1))
             return fail(AB_ERR_INVALID, "ab_cache_copy_pages: page %u is both read and written", src[i]);
     if (n_caches == 0) return AB_OK;
+    for (int c = 0; c < n_caches; c++) starts[c] = reinterpret_cast<uintptr_t>(caches[c]);
+    std::sort(starts.begin(), starts.end());
+    for (int c = 1; c < n_caches; c++)
+        if ((starts[c] - starts[c - 1]) / page_bytes < pages)
+            return fail(AB_ERR_INVALID, "ab_cache_copy_pages: two of the caches overlap; each is copied on its own");
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (align % 16 == 0) return run_copy<uint4>(s, caches, n_caches, page_bytes, src, dst, n_pairs);
     if (align % 4 == 0) return run_copy<uint32_t>(s, caches, n_caches, page_bytes, src, dst, n_pairs);

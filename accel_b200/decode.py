@@ -24,6 +24,7 @@ from typing import List, Optional
 import numpy as np
 import torch
 
+from . import _lib
 from . import runtime as rt
 from .blockpool import BlockPool
 from .quant import int4_column_split
@@ -381,20 +382,22 @@ class DecodeEngine:
         """Makes sequence `dst` a copy of sequence `src` as it stands (a beam, another sample of one
         prompt): what dst held is freed, the filled pages are shared, and only a partly filled last
         page is copied, since both go on writing there.  dst gets as many reserved positions as src.
+        With too few free pages nothing changes.
         The next step's inputs are the caller's to set for both (step, or set_inputs)."""
         if src == dst or not 0 <= src < self.batch or not 0 <= dst < self.batch:
             raise ValueError(f"fork of sequence {src} to {dst} in a batch of {self.batch}")
         n, blk = int(self.lengths_host[src]), self.cfg.block
         reserved = len(self.page_rows[src]) * blk
+        new = len(self.page_rows[src]) - n // blk                # the reserved pages, and the copy of a partly filled one
+        room = self.pool.available() + sum(p != self.pool.NONE and self.pool.refs(p) == 1 for p in self.page_rows[dst])
+        if new > room:
+            raise _lib.AccelError(_lib.AB_ERR_OOM, f"a fork needs {new} pages and has {room}; the pool does not evict to make "
+                                  "them for you")
         self.pool.free(self.page_rows[dst])
         self.page_rows[dst], self.lengths_host[dst] = [], 0
         row = self.pool.share(self.page_rows[src][:(n + blk - 1) // blk])
-        try:
-            row, s, d = self.pool.own(row, n, n + 1)
-            row = self.pool.grow(row, reserved)
-        except Exception:
-            self.pool.free(row)
-            raise
+        row, s, d = self.pool.own(row, n, n + 1)
+        row = self.pool.grow(row, reserved)
         self._copy_pages(s, d)
         self.page_rows[dst], self.lengths_host[dst] = row, n
         self.upload_pages()
@@ -410,6 +413,8 @@ class DecodeEngine:
     def fill_context(self, context: int, seed: int = 7):
         """Stands in for a prefill: reserves pages for `context` positions per sequence and fills
         those K/V rows with seeded N(0,1) values (f32 or f16 as the cache is)."""
+        if any(p == self.pool.NONE or self.pool.refs(p) > 1 for row in self.page_rows for p in row):
+            raise ValueError("a sequence has given pages back or shares some: its context cannot be written from the start")
         for s in range(self.batch):
             self.reserve(s, context)
         self.upload_pages()

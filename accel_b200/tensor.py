@@ -271,6 +271,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
 
     def windowed(form, rows, max_pages=0, base=0, pages=None, offsets=None):
         """The windowed kernel of a form whose arguments have been checked."""
+        for name, n in (("a cache's capacity", k.shape[0]), ("Block", opts.block)):
+            if n > 0xffffffff:
+                raise Refused(op, f"{name} is {n}; positions are u32")
         out = q.new_empty((rows, q_heads, head_dim))
         if rows and q_heads and head_dim:
             b = [q, k, v] + [_aligned(t) for t in (pages, opts.lengths, offsets) if t is not None] + [out]

@@ -365,8 +365,8 @@ AB_API int ab_blockpool_own(ab_blockpool *p, uint32_t *pages, int n_pages, uint3
 AB_API int ab_blockpool_compact(ab_blockpool *p, uint32_t *src, uint32_t *dst);
 /* caches[c][dst[i]] = caches[c][src[i]] for every cache (a HOST array of device pointers) and pair (HOST
  * numbers), on `stream`: a page is page_bytes contiguous bytes and a cache `pages` of them.  Refused,
- * with nothing launched, when a page is out of range, written twice, or both written and read.  A
- * stream capture records the pairs and pointers of the call. */
+ * with nothing launched, when a page is out of range, written twice, or both written and read, or when
+ * caches overlap.  A stream capture records the pairs and pointers of the call. */
 AB_API int ab_cache_copy_pages(void *stream, void *const *caches, int n_caches, size_t page_bytes, uint32_t pages,
                                const uint32_t *src, const uint32_t *dst, int n_pairs);
 
@@ -393,7 +393,7 @@ AB_API int ab_int4_prepack(void *stream, const uint32_t *codes, const uint16_t *
  * (synchronous; sticky for the process). */
 AB_API int ab_int4_stream_error(void);
 
-/* The same for the windowed prefill's tile kernel (AttentionWindowPrefill... from 64 query rows of a KV head on). */
+/* The same for the tile kernel of AttentionWindowPrefill... and AttentionWindowRagged..., on the current device. */
 AB_API int ab_attention_error(void);
 
 /* ---- One-shot all-reduce over NVLink peer memory (tensor-parallel decode) -----------------

@@ -133,3 +133,14 @@ def test_a_random_script_against_a_model():
         for n in rows:
             for x, w in zip(rows[n], want[n]):
                 assert x == NONE or mem[x] == w, (step, n)
+
+
+def test_compaction_wants_every_row():
+    p = BlockPool(8, 4)
+    a, b = p.grow(None, 8), p.grow(None, 12)
+    p.free(a[:1])
+    with pytest.raises(_lib.AccelError, match="every row in use"):
+        p.compact([b])
+    assert p.available() == 4
+    rows, src, dst = p.compact([[NONE, a[1]], b])
+    assert len(src) == len(dst) and {x for r in rows for x in r} == {NONE, 0, 1, 2, 3}

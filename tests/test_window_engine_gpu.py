@@ -193,3 +193,44 @@ def test_scored_tokens_are_those_of_the_logits():
     assert torch.equal(r.top_ids[:, 0], e.next_tokens) and torch.equal(r.top_logprobs[:, 0], r.logprobs)
     assert torch.equal(r.top_ids, torch.sort(logits[0], dim=1, descending=True, stable=True).indices[:, :4].int())
     assert ((r.entropy.double() + (lp.exp() * lp).sum(1)).abs() <= 2.0**-24 * 1024 * 20).all()
+
+
+def test_a_fork_without_room_leaves_both_sequences_as_they_were():
+    e = engine(model(config()), 3, context=16)
+    for s, n in ((0, 10), (1, 9)):
+        e.reserve(s, n)
+        e.lengths_host[s] = n
+    e.fork(0, 2)
+    before = [list(r) for r in e.page_rows]
+    extra = e.pool.grow(None, e.pool.available() * BLOCK)
+    e.reserve(1, 9)
+    e.fork(2, 1)                                     # 1 gives back three pages of its own, and one is needed
+    assert e.lengths_host[1] == 10 and e.page_rows[1][:2] == before[2][:2]
+    taken = e.pool.grow(None, e.pool.available() * BLOCK)
+    before = [list(r) for r in e.page_rows]
+    e.pool.free([taken[0]])
+    e.fork(0, 1)                                     # its own last page and the free one: room for one
+    refs = [e.pool.refs(x) for r in e.page_rows for x in r]
+    before = [list(r) for r in e.page_rows]
+    more = e.pool.grow(None, e.pool.available() * BLOCK)
+    e.lengths_host[0] = 1                            # the source now shares one page and wants three new ones
+    with pytest.raises(Exception, match="does not evict"):
+        e.fork(0, 1)
+    assert [list(r) for r in e.page_rows] == before and e.lengths_host[1] == 10
+    assert [e.pool.refs(x) for r in e.page_rows for x in r] == refs and len(extra) and more is not None
+
+
+def test_a_context_is_not_written_over_shared_or_missing_pages():
+    e = engine(model(config()), 2, context=64)
+    for s in range(2):
+        e.reserve(s, 50)
+    e.lengths_host[:] = 50
+    e.trim()
+    with pytest.raises(ValueError, match="given pages back or shares"):
+        e.fill_context(60)
+    f = engine(model(config()), 2, context=64)
+    f.reserve(0, 50)
+    f.lengths_host[0] = 50
+    f.fork(0, 1)
+    with pytest.raises(ValueError, match="given pages back or shares"):
+        f.fill_context(60)

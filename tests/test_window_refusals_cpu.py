@@ -113,3 +113,22 @@ def test_page_copies_refuse():
     with pytest.raises(_lib.AccelError, match="bad argument"):
         call([0], [1], size=0)
     assert call([], []) == 0
+
+
+def test_page_copies_refuse_caches_that_overlap():
+    import ctypes as C
+    L = _lib.lib()
+    for starts in ((1 << 20, (1 << 20) + 8 * 64 - 64), ((1 << 20) + 64, 1 << 20), (1 << 20, 1 << 20)):
+        ptrs = (C.c_void_p * 2)(*starts)
+        with pytest.raises(_lib.AccelError, match="overlap"):
+            _lib.check(L.ab_cache_copy_pages(None, ptrs, 2, 64, 8, (C.c_uint32 * 1)(0), (C.c_uint32 * 1)(1), 1))
+
+
+def test_positions_are_u32():
+    q, lens = torch.zeros(4, 8, device="meta"), torch.ones(1, dtype=torch.int32, device="meta")
+    k = torch.empty(1 << 32, 1, 8, dtype=torch.float16, device="meta")
+    with pytest.raises(T.Refused, match="capacity is 4294967296"):
+        T.attention(q, k, k, T.AttentionOptions(lengths=lens, window=4))
+    with pytest.raises(T.Refused, match="Block is 4294967296"):
+        T.attention(q, k[:64], k[:64], T.AttentionOptions(lengths=lens, window=4, block=1 << 32,
+                                                          pages=torch.zeros(3, dtype=torch.int32, device="meta")))
