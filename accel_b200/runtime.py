@@ -6,6 +6,7 @@ The binding order, the lengths block and the std140 uniform bytes are the refere
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import struct
 from typing import Optional, Sequence
 
@@ -155,6 +156,9 @@ def launch(name: str, bindings: Sequence[torch.Tensor], uniform: Optional[bytes]
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
+_encoded = functools.lru_cache(None)(str.encode)
+
+
 # a call's pointers and lengths as the bytes of C arrays, by how many there are
 _pointers = [struct.Struct(f"{n}Q").pack for n in range(16)]
 _counts = [struct.Struct(f"{n}I").pack for n in range(16)]
@@ -163,13 +167,15 @@ _counts = [struct.Struct(f"{n}I").pack for n in range(16)]
 def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: bytes, scratch: bool = False):
     """`launch` for the operators whose scratch memory (scratch: they may need some) is the call's own:
     it comes from torch's allocator, so a call captured into a CUDA graph keeps it in that graph's pool
-    and two graphs, or two streams, never share it.  A binding of None is empty; one of more elements
+    and two graphs, or two streams, never share it.  The bindings are contiguous: the caller has seen to
+    that, and the first is a tensor on a device.  A binding of None is empty; one of more elements
     than 32 bits count is passed as 0xffffffff, which those kernels read as that many or more."""
     dev = bindings[0].device
     if dev.type != "cuda":
         raise _lib.AccelError(_lib.AB_ERR_NO_DEVICE, f"{name}: bindings live on {dev}; this backend "
                               "runs on a CUDA device and has no CPU path")
-    if dev.index != torch.cuda.current_device():
+    index = dev.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return launch_own(name, bindings, uniform, scratch)
     ptrs, lens = [], []
@@ -179,7 +185,7 @@ def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: b
             ptrs.append(0)
             lens.append(0)
             continue
-        if t.device != dev or not t.is_contiguous():
+        if t.get_device() != index:
             raise ValueError(f"{name}: every binding is a contiguous tensor on {dev}")
         ptrs.append(t.data_ptr())
         lens.append(n if n < 0xffffffff else 0xffffffff)
@@ -189,7 +195,7 @@ def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: b
         if ws_bytes:
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     count = len(ptrs)
-    rc = _lib.lib().ab_launch(name.encode(), _raw_stream(dev.index), _pointers[count](*ptrs), _counts[count](*lens), count,
+    rc = _lib.lib().ab_launch(_encoded(name), _raw_stream(index), _pointers[count](*ptrs), _counts[count](*lens), count,
                               uniform, len(uniform), ws.data_ptr() if ws is not None else None, ws_bytes)
     if rc:
         _lib.check(rc)

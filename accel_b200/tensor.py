@@ -8,6 +8,7 @@ poisons the result rather than running."""
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import partial
 from typing import Optional, Sequence
 
 import torch
@@ -21,6 +22,8 @@ __all__ = ["Refused", "Int4", "int4_matvec", "int4_matmul", "AttentionOptions", 
            "copy_pages", "TokenLogprobs", "token_logprobs"]
 
 U32 = torch.int32       # torch has no general uint32 arithmetic; the bits are what the kernels read
+_U32_TYPES = (torch.int32, torch.uint32)
+_F32, _F16 = torch.float32, torch.float16
 
 
 class Refused(ValueError):
@@ -32,7 +35,7 @@ class Refused(ValueError):
 
 
 def _is_u32(t: torch.Tensor) -> bool:
-    return t.dtype in (torch.int32, torch.uint32)
+    return t.dtype in _U32_TYPES
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -40,7 +43,7 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     start anywhere."""
     if not t.is_contiguous():
         t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 # ------------------------------------------------------------------------------- int4 linear
@@ -202,17 +205,18 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
     positions further back than the window, but for the first opts.sinks of the sequence; page-table
     entries of pages that no query sees are not read (BlockPool.trim frees such pages)."""
     op = "Attention"
-    if q.dtype != torch.float32:
+    dtype, q_shape, k_shape = k.dtype, q.shape, k.shape
+    if q.dtype != _F32:
         raise Refused(op, f"q is {q.dtype} and the registered kernels read an f32 query")
-    if k.dtype != v.dtype:
+    if dtype != v.dtype:
         raise Refused(op, f"the key cache is {k.dtype} and the value cache is {v.dtype}; one kernel "
                       "reads both, so they are the same dtype")
-    if k.dtype not in (torch.float32, torch.float16):
+    if dtype != _F32 and dtype != _F16:
         raise Refused(op, f"the cache is {k.dtype}; the registered kernels read f32 or f16")
-    f16 = k.dtype == torch.float16
+    f16 = dtype == _F16
     if not q.is_contiguous():
         raise Refused(op, "q is a strided view and the registered kernels index it contiguously")
-    rank = q.dim()
+    rank = len(q_shape)
     if rank not in (2, 3, 4):
         raise Refused(op, f"q is {tuple(q.shape)}; it is [qHeads, headDim] for one token, "
                       "[qSeq, qHeads, headDim] for a prefill, or [batch, qSeq, qHeads, headDim] "
@@ -221,7 +225,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
     batched = rank == 4
     ragged = prefill = False
     if rank == 4:
-        batch, q_seq = q.shape[0], q.shape[1]
+        batch, q_seq = q_shape[0], q_shape[1]
     if opts.query_extents is not None:
         if rank != 3:
             raise Refused(op, f"q is {tuple(q.shape)} and QueryExtents is set; a ragged step is "
@@ -235,13 +239,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
             raise Refused(op, "QueryExtents is empty; it is one count per sequence and a step has "
                           "at least one sequence")
     elif rank == 3:
-        prefill, q_seq = True, q.shape[0]
-    if k.dim() != 3 or tuple(k.shape) != tuple(v.shape):
+        prefill, q_seq = True, q_shape[0]
+    if len(k_shape) != 3 or k_shape != v.shape:
         raise Refused(op, f"the key cache is {tuple(k.shape)} and the value cache is "
                       f"{tuple(v.shape)}; both are [capacity, kvHeads, headDim] and equal")
-    q_heads, head_dim = q.shape[-2], q.shape[-1]
-    kv_heads = k.shape[1]
-    if k.shape[2] != head_dim:
+    q_heads, head_dim = q_shape[-2], q_shape[-1]
+    capacity, kv_heads, width = k_shape
+    if width != head_dim:
         raise Refused(op, f"q's head is {head_dim} wide and the cache's is {k.shape[2]}")
     if kv_heads == 0 or q_heads % kv_heads != 0:
         raise Refused(op, f"{q_heads} query heads over {kv_heads} key/value heads; several query "
@@ -260,26 +264,37 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
     if opts.lengths.numel() != batch:
         raise Refused(op, f"Lengths holds {opts.lengths.numel()} entries and this step has {batch} "
                       "sequence(s); it is one length per sequence")
-    if opts.window != 0 or opts.sinks != 0:
-        for name, n in (("Window", opts.window), ("Sinks", opts.sinks)):
-            if type(n) is not int or not 0 <= n < 1 << 32:
-                raise Refused(op, f"{name} is {n!r}; it is a number of positions")
-    if opts.sinks and not opts.window:
-        raise Refused(op, f"Sinks is {opts.sinks} and Window is 0; without a window every position is visible")
-    k, v = k.contiguous(), v.contiguous()
+    window, sinks = opts.window, opts.sinks
+    if type(window) is not int or not 0 <= window <= 0xffffffff:
+        raise Refused(op, f"Window is {window!r}; it is a number of positions")
+    if type(sinks) is not int or not 0 <= sinks <= 0xffffffff:
+        raise Refused(op, f"Sinks is {sinks!r}; it is a number of positions")
+    if sinks and not window:
+        raise Refused(op, f"Sinks is {sinks} and Window is 0; without a window every position is visible")
+    if not k.is_contiguous():
+        k = k.contiguous()
+    if not v.is_contiguous():
+        v = v.contiguous()
     scale = float(opts.scale)
 
     def windowed(form, rows, max_pages=0, base=0, pages=None, offsets=None):
         """The windowed kernel of a form whose arguments have been checked."""
-        for name, n in (("a cache's capacity", k.shape[0]), ("Block", opts.block)):
-            if n > 0xffffffff:
-                raise Refused(op, f"{name} is {n}; positions are u32")
-        out = q.new_empty((rows, q_heads, head_dim))
+        if capacity > 0xffffffff:
+            raise Refused(op, f"a cache's capacity is {capacity}; positions are u32")
+        if opts.block > 0xffffffff:
+            raise Refused(op, f"Block is {opts.block}; positions are u32")
+        out = q.new_empty(rows, q_heads, head_dim)
         if rows and q_heads and head_dim:
-            b = [q, k, v] + [_aligned(t) for t in (pages, opts.lengths, offsets) if t is not None] + [out]
+            b = [q, k, v]
+            if pages is not None:
+                b.append(_aligned(pages))
+            b.append(_aligned(opts.lengths))
+            if offsets is not None:
+                b.append(_aligned(offsets))
+            b.append(out)
             rt.launch_own("AttentionWindow" + form + ("F16" if f16 else ""), b,
-                          rt.window_dims(batch, q_heads, kv_heads, head_dim, opts.block, max_pages, scale, opts.window,
-                                         opts.sinks, k.shape[0], rows, base), scratch=prefill or ragged)
+                          rt.window_dims(batch, q_heads, kv_heads, head_dim, opts.block, max_pages, scale, window, sinks,
+                                         capacity, rows, base), scratch=prefill or ragged)
         return out
 
     if prefill:
@@ -587,16 +602,17 @@ def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
     if not caches:
         return
     first = caches[0]
-    shape, dtype, device = first.shape, first.dtype, first.device
+    shape, dtype, device = first.shape, first.dtype, first.get_device()
     if not shape:
         raise Refused(op, "a cache is a scalar; it is [capacity, ...]")
+    pointers = []
     for c in caches:
-        if c.shape != shape or c.dtype != dtype or c.device != device:
-            raise Refused(op, f"the caches are {tuple(shape)} {dtype} on {device} and {tuple(c.shape)} {c.dtype} on "
+        if c.shape != shape or c.dtype != dtype or c.get_device() != device:
+            raise Refused(op, f"the caches are {tuple(shape)} {dtype} on {first.device} and {tuple(c.shape)} {c.dtype} on "
                           f"{c.device}; one call copies in caches of one form")
         if not c.is_contiguous():
             raise Refused(op, "a cache is a strided view; pages are copied in place, so it is contiguous")
-    pointers = [c.data_ptr() for c in caches]
+        pointers.append(c.data_ptr())
     if len(set(pointers)) != len(caches) and first.numel():
         raise Refused(op, "a cache is named twice")
     rt.copy_pages(caches, pointers, src, dst, block)
@@ -621,24 +637,26 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     row that holds a NaN or +inf, or nothing above -inf, gives NaN throughout.  No reference
     counterpart."""
     op = "TokenLogprobs"
-    if logits.dtype not in (torch.float32, torch.float16) or logits.dim() != 2 or logits.shape[1] == 0:
+    dtype, shape = logits.dtype, logits.shape
+    if (dtype != _F32 and dtype != _F16) or len(shape) != 2 or shape[1] == 0:
         raise Refused(op, f"logits are {logits.dtype} {tuple(logits.shape)}; they are f32 or f16 [rows, vocab]")
-    rows, vocab = logits.shape
+    rows, vocab = shape
     if type(top) is not int or not 0 <= top <= min(32, vocab):
         raise Refused(op, f"{top!r} alternatives of a vocabulary of {vocab}; at most 32")
-    dev = logits.device
-    n = 0
+    f16 = dtype == _F16
+    new = partial(logits.new_empty, dtype=_F32) if f16 else logits.new_empty
+    n, lp = 0, None
     if targets is not None:
         if not _is_u32(targets):
             raise Refused(op, f"targets are {targets.dtype} and a token id is u32")
-        if targets.dim() not in (1, 2) or targets.shape[0] != rows:
+        t_shape = targets.shape
+        if len(t_shape) not in (1, 2) or t_shape[0] != rows:
             raise Refused(op, f"targets are {tuple(targets.shape)} and the logits hold {rows} rows; they are [rows] or [rows, n]")
-        n = 1 if targets.dim() == 1 else targets.shape[1]
-    new = lambda shape, dt=torch.float32: torch.empty(shape, dtype=dt, device=dev)
-    lp = None if targets is None else new(targets.shape)
-    out = TokenLogprobs(lp, new((rows,)), new((rows, top), U32), new((rows, top)))
+        n = 1 if len(t_shape) == 1 else t_shape[1]
+        lp = new(*t_shape)
+    out = TokenLogprobs(lp, new(rows), logits.new_empty(rows, top, dtype=U32), new(rows, top))
     if rows:
-        rt.launch_own("TokenLogprobsF16" if logits.dtype == torch.float16 else "TokenLogprobs",
+        rt.launch_own("TokenLogprobsF16" if f16 else "TokenLogprobs",
                       [_aligned(logits), None if targets is None else _aligned(targets), lp, out.entropy,
                        out.top_ids, out.top_logprobs], rt.logprob_dims(vocab, rows, n, top))
     return out
