@@ -72,9 +72,10 @@ __host__ __device__ inline bool on_tiles(uint64_t rows, uint64_t seen)
 {
     return rows >= 256 || (rows >= kTileFrom && rows * seen >= 65536);
 }
-// a prefill, or the sequences of a ragged step that have that many rows (it then sets p.left), on 128-row tiles
-// (window_prefill.cu); p.q_heads / p.kv_heads <= 128
-int run_window_tiles(Launch &l, WinParams &p, bool f16, const char *name);
+// a prefill, or a ragged step: its sequences with that many rows, on 128-row tiles (window_prefill.cu); p.left says which rows
+// are left, and `rows` launches the kernel for those.  p.q_heads / p.kv_heads <= 128
+using WindowRows = int (*)(Launch &l, const WinParams &p, const char *name);
+int run_window_tiles(Launch &l, WinParams &p, bool f16, WindowRows rows, const char *name);
 int window_error_flag();
 
 }  // namespace ab

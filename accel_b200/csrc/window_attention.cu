@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, sizeof(T) == 4 ? 3 : 4) win_ro
     const uint32_t heads = min(8u, (kvh + 1) * group - h0);
     const uint32_t tile_k = (uint32_t)__cvta_generic_to_shared(smem) + warp * Tile::kWarpBytes, tile_v = tile_k + Tile::kBytesK;
 
+    if (p.left) pdl_trigger();                                      // the packing may run beside this
     for (uint32_t turn = blockIdx.x / parts; turn < win_rows(p); turn += gridDim.x / parts) {
     uint32_t row = turn;
     const WinView w = win_view(p, row);
@@ -550,6 +551,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 3) win_lanes_kernel(const WinP
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LR, ll = lane % LR;
     const uint32_t part = blockIdx.x % parts, kvh = blockIdx.y, h0 = kvh * G, D = p.head_dim;
     const bool on = (uint32_t)ll * 4 < D;
+    if (p.left) pdl_trigger();                                      // the packing may run beside this
     for (uint32_t turn = blockIdx.x / parts; turn < win_rows(p); turn += gridDim.x / parts) {
     uint32_t row = turn;
     const WinView w = win_view(p, row);
@@ -732,6 +734,21 @@ template <int G> int launch_lanes(Launch &l, const WinParams &p, const char *nam
     return p.head_dim > 64 ? launch_lanes<G, 32>(l, p, name) : (p.head_dim > 32 ? launch_lanes<G, 16>(l, p, name) : launch_lanes<G, 8>(l, p, name));
 }
 
+template <typename T> int run_rows(Launch &l, const WinParams &p, const char *name)
+{
+    const uint32_t group = p.q_heads / p.kv_heads;
+    if (sizeof(T) == 4) {
+        switch (group) {
+        case 1: return launch_lanes<1>(l, p, name);
+        case 2: return launch_lanes<2>(l, p, name);
+        case 3: return launch_lanes<3>(l, p, name);
+        case 4: return launch_lanes<4>(l, p, name);
+        default: break;
+        }
+    }
+    return p.head_dim <= 64 ? launch_rows<T, 64>(l, p, name) : launch_rows<T, 128>(l, p, name);
+}
+
 template <typename T> int run_window(Launch &l, WinParams &p, const char *name)
 {
     if ((uint64_t)p.base + p.rows > 0xffffffffull)
@@ -744,21 +761,8 @@ template <typename T> int run_window(Launch &l, WinParams &p, const char *name)
     // row kernel's time, and took 7.0 us more of kernels without work)
     const uint64_t most = p.form == kPrefillRows ? p.rows : (p.form == kRaggedStep && p.rows >= p.batch ? p.rows - p.batch + 1 : 0);
     const uint64_t seen = std::min<uint64_t>((uint64_t)p.window + p.sinks, p.form == kPrefillRows ? std::min<uint64_t>((uint64_t)p.base + p.rows, p.reach) : p.reach);
-    if (group <= 128 && on_tiles(most * group, seen)) {
-        const int rc = run_window_tiles(l, p, sizeof(T) == 2, name);
-        if (rc || p.form == kPrefillRows) return rc;
-    }
-    if (l.query_ws) return AB_OK;
-    if (sizeof(T) == 4) {
-        switch (group) {
-        case 1: return launch_lanes<1>(l, p, name);
-        case 2: return launch_lanes<2>(l, p, name);
-        case 3: return launch_lanes<3>(l, p, name);
-        case 4: return launch_lanes<4>(l, p, name);
-        default: break;
-        }
-    }
-    return p.head_dim <= 64 ? launch_rows<T, 64>(l, p, name) : launch_rows<T, 128>(l, p, name);
+    if (group <= 128 && on_tiles(most * group, seen)) return run_window_tiles(l, p, sizeof(T) == 2, run_rows<T>, name);
+    return l.query_ws ? AB_OK : run_rows<T>(l, p, name);
 }
 
 // WindowDims{Batch,QHeads,KVHeads,HeadDim,Block,MaxPages,Scale f32,Window,Sinks,Capacity,QSeq,Base}, 48 bytes.

@@ -127,119 +127,171 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo
 // grid (tiles, KV heads of this pass, 2): K or V of one tile.  An operand's element (r, c), c along the contraction, lies
 // at (c / 8) * rows * 16 + r * 16 + (c % 8) * 2: 128 rows of positions for K, DP rows of dimensions for V.
 // Every element is read once and written once per part: HBM (or L2) bounds it.
+// Measured: 8192 f32 positions of 32 heads, 537 MB in 112 us (4.8 TB/s); 4096 f16 positions of 8 heads, 33.5 MB in 11.5 us,
+// where the values of an f16 cache stay as they are, a copy in another order (16.3 us through f32 registers).
 constexpr int kPackThreads = 512;
-template <typename T, int DP>
-__global__ void __launch_bounds__(kPackThreads, 2) win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, TileHead *heads,
-                                                       uint32_t kvh0)
+
+// Plan: a ragged step's tiles, which the CTAs take by turns; or one for each.
+template <typename T, int DP, bool Plan>
+__global__ void __launch_bounds__(kPackThreads, sizeof(T) == 2 ? 3 : 2)
+win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, TileHead *heads, uint32_t kvh0)
 {
     __shared__ uint32_t rows[kKeys], amax_bits, bad_any;
     pdl_trigger();                                       // the tile kernel may set itself up meanwhile
-    uint4 span;                                          // first position, end of the positions, sequence
-    if (plan.segments) {
-        span = plan.key_tiles[blockIdx.x];
-        if (blockIdx.x >= plan.counts[0]) return;
-    } else {
-        span.x = win_tile_start(plan.one, blockIdx.x);
-        span.y = min(blockIdx.x < plan.one.sink_tiles ? min(plan.one.ns, plan.one.end) : plan.one.end, p.lengths[0]);
-        span.z = 0;
-    }
-    const uint32_t kvh = kvh0 + blockIdx.y, t = threadIdx.x, D = p.head_dim;
-    const size_t at = (size_t)blockIdx.y * plan.max_key_tiles + blockIdx.x;
-    TileHead &head = heads[at];
-    unsigned char *dst = tiles + at * kTileBytes<T, DP> + (blockIdx.z ? kParts<T> * kSlotBytes<T, DP> : 0);
-    if (t == 0) { amax_bits = 0; bad_any = 0; }
-    if (t < kKeys) {
-        const uint64_t j = (uint64_t)span.x + t;
-        uint32_t r = 0xffffffffu;
-        if (j < span.y) r = win_cache_row(p, p.pages ? p.pages + (size_t)span.z * p.max_pages : nullptr, (uint32_t)j);
-        rows[t] = r;
-        const uint32_t seen = __ballot_sync(0xffffffffu, r != 0xffffffffu);
-        if (blockIdx.z == 0 && (t & 31) == 0) head.seen[t >> 5] = seen;
-    }
-    __syncthreads();
+    const uint32_t kvh = kvh0 + blockIdx.y, t = threadIdx.x, D = p.head_dim, lane = t & 31;
     // elements of a thread; dimensions that it takes of V together (4 bytes of a position); groups of eight positions at a time
     constexpr int kEach = kKeys * DP / kPackThreads, kWide = sizeof(T) == 2 ? 2 : 1, kTogether = kPackThreads * kWide / DP;
-    float x[kEach];
-    float big = 0.f;
-    bool bad = false;
     // K: eight dimensions of a position at a time; a warp takes eight positions x 32 dimensions, whole lines to read and to
     // write.  V: eight positions of kWide dimensions at a time, neighbouring threads neighbouring dimensions.
-    const uint32_t lane = t & 31, dim = t % (DP / kWide) * kWide, group0 = t / (DP / kWide);
+    const uint32_t dim = t % (DP / kWide) * kWide, group0 = t / (DP / kWide);
     const auto k_task = [&](int i, uint32_t &key, uint32_t &d) {
         const uint32_t task = (i / 8) * (kPackThreads / 32) + (t >> 5);            // of 16 x DP / 32
         key = task / (DP / 32) * 8 + (lane & 7);
         d = task % (DP / 32) * 32 + (lane >> 3) * 8;
     };
-    if (blockIdx.z == 0) {
-#pragma unroll
-        for (int i = 0; i < kEach; i += 8) {
-            uint32_t key, d;
-            k_task(i, key, d);
-            const uint32_t r = rows[key];
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[i + e] = 0.f;
-            if (r != 0xffffffffu && d < D) {
-                const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.k) + ((uint64_t)r * p.kv_heads + kvh) * D + d);
-                uint4 raw[sizeof(T) / 2];
-#pragma unroll
-                for (int n = 0; n < (int)sizeof(T) / 2; n++) raw[n] = __ldg(src + n);
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[i + e] = to_f32(reinterpret_cast<const T *>(raw)[e]);
-            }
+    const auto v_to = [&](int i) { return (i / (8 * kWide) * kTogether + group0) * (DP * 16) + (dim + i / 8 % kWide) * 16; };
+    uint32_t tile = blockIdx.x;
+    while (!Plan || tile < plan.counts[0]) {
+        uint4 span;                                      // first position, end of the positions, sequence
+        if (Plan) {
+            span = plan.key_tiles[tile];
+        } else {
+            span.x = win_tile_start(plan.one, tile);
+            span.y = min(tile < plan.one.sink_tiles ? min(plan.one.ns, plan.one.end) : plan.one.end, p.lengths[0]);
+            span.z = 0;
         }
-    } else {
-        const T *v = static_cast<const T *>(p.v) + (uint64_t)kvh * D + dim;
+        const size_t at = (size_t)blockIdx.y * plan.max_key_tiles + tile;
+        TileHead &head = heads[at];
+        unsigned char *dst = tiles + at * kTileBytes<T, DP> + (blockIdx.z ? kParts<T> * kSlotBytes<T, DP> : 0);
+        if (t == 0) { amax_bits = 0; bad_any = 0; }
+        if (t < kKeys) {
+            const uint64_t j = (uint64_t)span.x + t;
+            uint32_t r = 0xffffffffu;
+            if (j < span.y) r = win_cache_row(p, p.pages ? p.pages + (size_t)span.z * p.max_pages : nullptr, (uint32_t)j);
+            rows[t] = r;
+            const uint32_t seen = __ballot_sync(0xffffffffu, r != 0xffffffffu);
+            if (blockIdx.z == 0 && (t & 31) == 0) head.seen[t >> 5] = seen;
+        }
+        __syncthreads();
+        bool bad = false;
+        if constexpr (sizeof(T) == 2) {
+            if (blockIdx.z == 0) {
+                uint4 x[kEach / 8];
 #pragma unroll
-        for (int i = 0; i < kEach / kWide; i++) {
-            const uint32_t r = rows[(i / 8 * kTogether + group0) * 8 + (i & 7)];
-            const T *src = v + (uint64_t)r * p.kv_heads * D;
-            const bool on = r != 0xffffffffu && dim < D;
-            if (kWide == 2) {
-                const float2 y = on ? two(src) : make_float2(0.f, 0.f);
-                x[i / 8 * 16 + (i & 7)] = y.x;
-                x[i / 8 * 16 + 8 + (i & 7)] = y.y;
+                for (int i = 0; i < kEach / 8; i++) {
+                    uint32_t key, d;
+                    k_task(i * 8, key, d);
+                    const uint32_t r = rows[key];
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (r != 0xffffffffu && d < D)
+                        x[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.k) + ((uint64_t)r * p.kv_heads + kvh) * D + d));
+                }
+#pragma unroll
+                for (int i = 0; i < kEach / 8; i++) {
+                    uint32_t key, d;
+                    k_task(i * 8, key, d);
+                    *reinterpret_cast<uint4 *>(dst + d / 8 * (kKeys * 16) + key * 16) = x[i];
+                }
             } else {
-                x[i] = on ? to_f32(*src) : 0.f;
+                const T *v = static_cast<const T *>(p.v) + (uint64_t)kvh * D + dim;
+                uint32_t x[kEach / 2];
+#pragma unroll
+                for (int i = 0; i < kEach / 2; i++) {
+                    const uint32_t r = rows[(i / 8 * kTogether + group0) * 8 + (i & 7)];
+                    x[i] = r != 0xffffffffu && dim < D ? __ldg(reinterpret_cast<const uint32_t *>(v + (uint64_t)r * p.kv_heads * D)) : 0;
+                }
+#pragma unroll
+                for (int i = 0; i < kEach / 2; i++) {    // (values that are not finite are left out: see the other case)
+                    if ((x[i] & 0x7c00u) == 0x7c00u) { x[i] &= 0xffff0000u; bad = true; }
+                    if ((x[i] & 0x7c000000u) == 0x7c000000u) { x[i] &= 0xffffu; bad = true; }
+                }
+#pragma unroll
+                for (int i = 0; i < kEach / 2; i += 8) {
+                    *reinterpret_cast<uint4 *>(dst + v_to(2 * i)) =
+                        make_uint4(__byte_perm(x[i], x[i + 1], 0x5410), __byte_perm(x[i + 2], x[i + 3], 0x5410),
+                                   __byte_perm(x[i + 4], x[i + 5], 0x5410), __byte_perm(x[i + 6], x[i + 7], 0x5410));
+                    *reinterpret_cast<uint4 *>(dst + v_to(2 * i + 8)) =
+                        make_uint4(__byte_perm(x[i], x[i + 1], 0x7632), __byte_perm(x[i + 2], x[i + 3], 0x7632),
+                                   __byte_perm(x[i + 4], x[i + 5], 0x7632), __byte_perm(x[i + 6], x[i + 7], 0x7632));
+                }
+            }
+            if (blockIdx.z && __any_sync(0xffffffffu, bad) && lane == 0) bad_any = 1;
+            __syncthreads();
+            if (t == 0) {
+                if (blockIdx.z) { head.v_scale = 1.f; head.bad = bad_any; }
+                else head.k_scale = 1.f;
+            }
+        } else {
+            float x[kEach];
+            float big = 0.f;
+            if (blockIdx.z == 0) {
+#pragma unroll
+                for (int i = 0; i < kEach; i += 8) {
+                    uint32_t key, d;
+                    k_task(i, key, d);
+                    const uint32_t r = rows[key];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[i + e] = 0.f;
+                    if (r != 0xffffffffu && d < D) {
+                        const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.k) + ((uint64_t)r * p.kv_heads + kvh) * D + d);
+                        uint4 raw[2];
+                        raw[0] = __ldg(src);
+                        raw[1] = __ldg(src + 1);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[i + e] = reinterpret_cast<const float *>(raw)[e];
+                    }
+                }
+            } else {
+                const T *v = static_cast<const T *>(p.v) + (uint64_t)kvh * D + dim;
+#pragma unroll
+                for (int i = 0; i < kEach; i++) {
+                    const uint32_t r = rows[(i / 8 * kTogether + group0) * 8 + (i & 7)];
+                    const T *src = v + (uint64_t)r * p.kv_heads * D;
+                    const bool on = r != 0xffffffffu && dim < D;
+                    x[i] = on ? to_f32(*src) : 0.f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kEach; i++) {
+                const bool finite = fabsf(x[i]) <= 3.402823466e38f;
+                if (finite) big = fmaxf(big, fabsf(x[i]));
+                else bad = true;
+                // a value that is not finite would spoil rows that do not see it (0 * inf): it is left out here and added to the
+                // rows that do by the tile kernel.  A score is masked after its product, so a key may stay
+                if (!finite && blockIdx.z) x[i] = 0.f;
+            }
+            const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+            if (lane == 0) atomicMax(&amax_bits, b);
+            if (blockIdx.z && __any_sync(0xffffffffu, bad) && lane == 0) bad_any = 1;
+            __syncthreads();
+            const int e = fit_exponent(__uint_as_float(amax_bits));
+            if (t == 0) {
+                if (blockIdx.z) { head.v_scale = ab_pow2(-e); head.bad = bad_any; }
+                else head.k_scale = ab_pow2(-e);
+            }
+            const float f = ab_pow2(e);
+#pragma unroll
+            for (int i = 0; i < kEach; i += 8) {
+                float y[8];
+#pragma unroll
+                for (int n = 0; n < 8; n++) y[n] = x[i + n] * f;
+                uint4 hi, lo;
+                split8(y, hi, lo);
+                uint32_t to = v_to(i);
+                if (blockIdx.z == 0) {
+                    uint32_t key, d;
+                    k_task(i, key, d);
+                    to = d / 8 * (kKeys * 16) + key * 16;
+                }
+                *reinterpret_cast<uint4 *>(dst + to) = hi;
+                *reinterpret_cast<uint4 *>(dst + kSlotBytes<T, DP> + to) = lo;
             }
         }
+        if (!Plan) return;
+        tile += gridDim.x;
+        __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < kEach; i++) {
-        const bool finite = fabsf(x[i]) <= 3.402823466e38f;
-        if (finite) big = fmaxf(big, fabsf(x[i]));
-        else bad = true;
-        // a value that is not finite would spoil rows that do not see it (0 * inf): it is left out here and added to the
-        // rows that do by the tile kernel.  A score is masked after its product, so a key may stay
-        if (!finite && blockIdx.z) x[i] = 0.f;
-    }
-    if (sizeof(T) == 4) {
-        const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
-        if ((t & 31) == 0) atomicMax(&amax_bits, b);
-    }
-    if (blockIdx.z && __any_sync(0xffffffffu, bad) && (t & 31) == 0) bad_any = 1;
-    __syncthreads();
-    const int e = sizeof(T) == 4 ? fit_exponent(__uint_as_float(amax_bits)) : 0;
-    if (t == 0) {
-        if (blockIdx.z) { head.v_scale = ab_pow2(-e); head.bad = bad_any; }
-        else head.k_scale = ab_pow2(-e);
-    }
-    const float f = ab_pow2(e);
-#pragma unroll
-    for (int i = 0; i < kEach; i += 8) {
-        float y[8];
-#pragma unroll
-        for (int n = 0; n < 8; n++) y[n] = x[i + n] * f;
-        uint4 hi, lo;
-        split8(y, hi, lo);
-        uint32_t to = (i / (8 * kWide) * kTogether + group0) * (DP * 16) + (dim + i / 8 % kWide) * 16;
-        if (blockIdx.z == 0) {
-            uint32_t key, d;
-            k_task(i, key, d);
-            to = d / 8 * (kKeys * 16) + key * 16;
-        }
-        *reinterpret_cast<uint4 *>(dst + to) = hi;
-        if (kParts<T> == 2) *reinterpret_cast<uint4 *>(dst + kSlotBytes<T, DP> + to) = lo;
-    }
+    pdl_wait();                                          // beside a ragged step's rows (run_tiles): done when those are
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -821,7 +873,7 @@ __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32
 
 constexpr uint64_t kPassBytes = 1ull << 30;              // tiles of one pass over KV heads; a prefill takes more where one head's list does
 
-template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char *name)
+template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, WindowRows rows_kernel, const char *name)
 {
     static_assert(TileSmem<T, DP>::kBytes <= 232448, "shared memory of a CTA");
     static_assert(kRows * (DP + 4) * 4 + 8 * kRows * 4 <= TileSmem<T, DP>::kBars, "the parts of all groups fit where the operands were");
@@ -874,6 +926,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
                                                  plan.max_row_tiles, left);
         count_launch();
         rc = check_cuda(cudaGetLastError(), name);
+        if (rc == AB_OK) rc = rows_kernel(l, p, name);
         if (rc) return rc;
     }
     // few row tiles: a cluster shares the positions of each, as long as all CTAs run at once and have four tiles or more
@@ -888,10 +941,23 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
     unsigned char *tiles = reinterpret_cast<unsigned char *>(heads) + head_bytes;
     for (uint32_t h = 0; h < p.kv_heads && row_tiles; h += pass) {
         const uint32_t now = std::min(pass, p.kv_heads - h);
+        // A ragged step's rows left run beside the packing, which waits for them at its end: it is their programmatic dependent,
+        // and what it reads was there before either.  Its grid is two rounds of CTAs, which take what tiles there are by
+        // turns (the bound on their number is many times that).  8 single tokens and 4 chunks of 64 over windows of 1024, f16:
+        // rows 19 and packing 21 us one after the other, 29 us together
         if (key_tiles) {
-            win_pack_kernel<T, DP><<<dim3((uint32_t)key_tiles, now, 2), kPackThreads, 0, l.stream>>>(p, plan, tiles, heads, h);
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((uint32_t)(ragged ? std::min<uint64_t>(key_tiles, (uint64_t)sm_count() * (sizeof(T) == 2 ? 3 : 2) / now + 1) : key_tiles), now, 2);
+            cfg.blockDim = dim3(kPackThreads);
+            cfg.stream = l.stream;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = ragged && h == 0 ? 1 : 0;
+            const cudaError_t e = cudaLaunchKernelEx(&cfg, ragged ? win_pack_kernel<T, DP, true> : win_pack_kernel<T, DP, false>, p, plan, tiles, heads, h);
             count_launch();
-            rc = check_cuda(cudaGetLastError(), name);
+            rc = check_cuda(e, name);
             if (rc) return rc;
         }
         // a programmatic dependent of the pack kernel: its set-up and query rows (which no kernel of this call writes) overlap it.
@@ -926,10 +992,10 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, const char 
 
 }  // namespace
 
-int run_window_tiles(Launch &l, WinParams &p, bool f16, const char *name)
+int run_window_tiles(Launch &l, WinParams &p, bool f16, WindowRows rows, const char *name)
 {
-    if (f16) return p.head_dim <= 64 ? run_tiles<__half, 64>(l, p, name) : run_tiles<__half, 128>(l, p, name);
-    return p.head_dim <= 64 ? run_tiles<float, 64>(l, p, name) : run_tiles<float, 128>(l, p, name);
+    if (f16) return p.head_dim <= 64 ? run_tiles<__half, 64>(l, p, rows, name) : run_tiles<__half, 128>(l, p, rows, name);
+    return p.head_dim <= 64 ? run_tiles<float, 64>(l, p, rows, name) : run_tiles<float, 128>(l, p, rows, name);
 }
 
 int window_error_flag()
