@@ -17,7 +17,8 @@ namespace {
 
 constexpr int kMaxCaches = 128;       // per launch: 1 KB of the parameters
 constexpr int kThreads = 256;
-constexpr uint32_t kChunk = 16384;    // bytes a CTA copies
+constexpr uint32_t kChunk = 16384;    // bytes a CTA copies (537 MB in 16 caches: 81.6 us, 6.6 TB/s; 81.9 with 8 KB, 86.0 with 64 KB; one
+                                      // page of 64 KB in 8 caches: 2.4, 2.0 and 4.8 us)
 
 template <int P> struct CopyParams {
     void *cache[kMaxCaches];
@@ -60,7 +61,8 @@ int run_copy(cudaStream_t stream, void *const *caches, int n_caches, uint64_t pa
     return AB_OK;
 }
 
-// 2 KB of parameters for the few pairs of a fork, 29 KB of the 32 that a launch may have for a compaction's
+// 2 KB of parameters for the few pairs of a fork, 29 KB of the 32 that a launch may have for a compaction's (one pair in 64
+// caches: 2.6 us on the device with the small block, 2.8 with the large, and 29 KB less to write on the host)
 template <typename V>
 int run_copy(cudaStream_t stream, void *const *caches, int n_caches, uint64_t page_bytes, const uint32_t *src, const uint32_t *dst, int n_pairs)
 {

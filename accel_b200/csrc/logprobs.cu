@@ -413,7 +413,8 @@ template <typename T> int run_logprobs(Launch &l, const char *name)
     p.targets = ptr<const uint32_t>(l, 1);
     p.logprobs = ptr<float>(l, 2); p.entropy = ptr<float>(l, 3);
     p.top_ids = ptr<uint32_t>(l, 4); p.top_logprobs = ptr<float>(l, 5);
-    // few rows: a row over several CTAs, as long as each has a step of every thread to do
+    // few rows: a row over several CTAs, as long as each has a step of every thread to do (16 rows of 128256 logits: 9.0 us
+    // against 19.1 with a CTA a row; 1 of 32000: 7.1 against 7.5; 148 of 32000: 11.1 against 11.4)
     uint32_t parts = 1;
     while (parts < 8 && rows * parts * 2 <= 2ull * sm_count() && p.vocab >= parts * 2 * kThreads * 16 / 2) parts *= 2;
     cudaLaunchConfig_t cfg = {};

@@ -22,6 +22,10 @@
 // exponentials run under the other's MMAs; one lane issues the MMAs in the order QK(0) QK(1) PV(0) QK(2)
 // PV(1) ..., one lane the bulk copies, in the same order, into a ring of slots.  Tensor memory: 128 columns of
 // scores and 128 of output for each group; the weights overwrite their scores.
+//
+// Measured, the tile kernel alone: 4096 tokens of 32 heads over windows of 2048, f16 cache, groups of 4, 228 us, which is
+// 0.90 PFLOP/s of issued products (the MMAs and copies without the softmax: 196 us); 4096 tokens behind 4096 over windows of
+// 4096, f32 cache, 32 heads, 690 us, 1.20 PFLOP/s issued (592 us: there the tiles from L2, 33 bytes a clock and SM).
 #include <algorithm>
 #include <math_constants.h>
 
@@ -929,7 +933,10 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, WindowRows 
         if (rc == AB_OK) rc = rows_kernel(l, p, name);
         if (rc) return rc;
     }
-    // few row tiles: a cluster shares the positions of each, as long as all CTAs run at once and have four tiles or more
+    // few row tiles: a cluster shares the positions of each, as long as all CTAs run at once and have four tiles or more.
+    // (8 KV heads, groups of 4, f32, with its packing: 64 tokens that see 1024 positions 30.6 us split, 40.5 whole, 40.2 split
+    // without the limit of four tiles; 64 tokens that see 300 21.3, 21.5 and 34.5 us; 32 tokens of one KV head that see 16384
+    // 57.3 us split over eight, 304 whole)
     uint32_t split = 1;
     {
         const uint64_t ctas = (ragged ? p.rows / per_tile + 1 : row_tiles) * pass;
