@@ -23,9 +23,9 @@
 // PV(1) ..., one lane the bulk copies, in the same order, into a ring of slots.  Tensor memory: 128 columns of
 // scores and 128 of output for each group; the weights overwrite their scores.
 //
-// Measured, the tile kernel alone: 4096 tokens of 32 heads over windows of 2048, f16 cache, groups of 4, 228 us, which is
-// 0.90 PFLOP/s of issued products (the MMAs and copies without the softmax: 196 us); 4096 tokens behind 4096 over windows of
-// 4096, f32 cache, 32 heads, 690 us, 1.20 PFLOP/s issued (592 us: there the tiles from L2, 33 bytes a clock and SM).
+// Measured, the tile kernel alone: 4096 tokens of 32 heads over windows of 2048, f16 cache, groups of 4, 225 us, which is
+// 0.92 PFLOP/s of issued products (the MMAs and copies without the softmax: 196 us); 4096 tokens behind 4096 over windows of
+// 4096, f32 cache, 32 heads, 685 us, 1.21 PFLOP/s issued (592 us: there the tiles from L2, 33 bytes a clock and SM).
 #include <algorithm>
 #include <math_constants.h>
 
@@ -396,6 +396,24 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
         rt = e.y;
     }
     const uint32_t first = rt * per_tile, tok0 = keys.row0 + first, tokens = min(per_tile, keys.rows - first);
+    // The query rows.  A warp takes 16 of them, eight at a time, four lanes to a row: 64 bytes of each of eight rows a load.
+    // All are on their way before anything else is worked out
+    float4 both[2][DP / 16];
+    if (warp < kSoftWarps) {
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const uint32_t row = warp * 16 + g * 8 + (lane >> 2), at = (lane & 3) * 4;
+            const bool on = row < tokens * group;
+            const float *q = p.q + ((uint64_t)(tok0 + (on ? row / group : 0)) * p.q_heads + (kvh0 + kv) * group + (on ? row % group : 0)) * D;
+#pragma unroll
+            for (int i = 0; i < DP / 16; i++) {
+                both[g][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (on && 16 * i + at < D)
+                    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(both[g][i].x), "=f"(both[g][i].y), "=f"(both[g][i].z), "=f"(both[g][i].w) : "l"(q + 16 * i + at));
+            }
+        }
+    }
     const uint64_t pa = (uint64_t)keys.base + first;
     const Range range = win_range(p, keys, pa, pa + tokens - 1);
     // of the tiles that they see, this CTA of the cluster takes n, from the i0-th on
@@ -429,20 +447,9 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
     const uint32_t r = tid & (kRows - 1);
     const bool live = r < tokens * group;
     float *row_scale = reinterpret_cast<float *>(smem + Smem::kScale);
-    // The query rows, scaled, split, stored as the A operand.  A warp takes 16 rows, eight at a time, four lanes to a row:
-    // 64 bytes of each of eight rows a load, and stores that meet every bank twice
+    // scaled, split, stored as the A operand (the stores meet every bank twice)
     if (warp < kSoftWarps) {
         const uint32_t at = (lane & 3) * 4;
-        float4 both[2][DP / 16];                         // all on their way at once
-#pragma unroll
-        for (int g = 0; g < 2; g++) {
-            const uint32_t row = warp * 16 + g * 8 + (lane >> 2);
-            const bool on = row < tokens * group;
-            const float *q = p.q + ((uint64_t)(tok0 + (on ? row / group : 0)) * p.q_heads + (kvh0 + kv) * group + (on ? row % group : 0)) * D;
-#pragma unroll
-            for (int i = 0; i < DP / 16; i++)
-                both[g][i] = on && 16 * i + at < D ? __ldg(reinterpret_cast<const float4 *>(q + 16 * i + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
 #pragma unroll
         for (int g = 0; g < 2; g++) {
             const uint32_t row = warp * 16 + g * 8 + (lane >> 2);

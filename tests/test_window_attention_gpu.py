@@ -431,3 +431,17 @@ def test_ragged_lists_longer_than_the_tiles_there_is_room_for():
             r = b * m + i
             check(got[r], *attend(hq[r], hk, hv, visible(int(lengths[b]) - m + i, int(lengths[b]), n, 0), attn_scale(D), qH), f"{b} {i}")
     rt.attention_error()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_more_sequences_than_a_grid_has_rows(f16):
+    # every query sees one position: its value is the answer
+    batch, kv, D = 70000, 2, 8
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    k, v = (torch.randn((batch, kv, D), device=DEV, generator=gen).to(torch.float16 if f16 else torch.float32) for _ in range(2))
+    q = torch.randn((batch, 1, kv, D), device=DEV, generator=gen)
+    pages = torch.randperm(batch, device=DEV, generator=gen).to(torch.int32)[:, None]
+    got = T.attention(q, k, v, T.AttentionOptions(lengths=torch.ones(batch, dtype=torch.int32, device=DEV), pages=pages, block=1,
+                                                  scale=0.3, window=3))
+    want = v[pages[:, 0].long()].float()
+    assert ((got - want).abs() <= 2.0**-22 * want.abs()).all()      # a weight of 1: a quotient and two products of one value
