@@ -445,3 +445,18 @@ def test_more_sequences_than_a_grid_has_rows(f16):
                                                   scale=0.3, window=3))
     want = v[pages[:, 0].long()].float()
     assert ((got - want).abs() <= 2.0**-22 * want.abs()).all()      # a weight of 1: a quotient and two products of one value
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("tokens,qH,kv", [(1, 4, 2), (1, 12, 1), (200, 4, 2)])
+def test_scales_of_any_sign_and_size(tokens, qH, kv, f16):
+    D, n = 64, 300
+    rng = np.random.default_rng(9)
+    k, v = (rng.standard_normal((n, kv, D)).astype(np.float16 if f16 else np.float32) for _ in range(2))
+    q = rng.standard_normal((tokens, qH, D)).astype(np.float32)
+    q[0, 0] = 0                                                   # and a query of zeros: every weight the same
+    for scale in (0.0, -0.3, 1e-30, 1e-40):
+        got = T.attention(dev(q), dev(k), dev(v), T.AttentionOptions(
+            lengths=dev(np.array([n], np.uint32)), scale=scale, base=n - tokens, window=100, sinks=2)).cpu().numpy()
+        for i in range(0, tokens, 9):
+            check(got[i], *attend(q[i], k, v, visible(n - tokens + i, n, 100, 2), scale, qH // kv), f"scale {scale} row {i}")

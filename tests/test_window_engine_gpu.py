@@ -234,3 +234,54 @@ def test_a_context_is_not_written_over_shared_or_missing_pages():
     f.fork(0, 1)
     with pytest.raises(ValueError, match="given pages back or shares"):
         f.fill_context(60)
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_chunks_tokens_and_scores_through_the_plan_seam(graphs):
+    # a prefill on tiles, a ragged step of chunks and tokens, and log probabilities of f16 logits as one plan, two submissions of
+    # it in flight: the bits of the calls
+    from accel_b200 import driver as D
+    from accel_b200 import tensor as T
+    qH, kv, Dh, block, window, sinks = 8, 2, 64, 16, 60, 3
+    rng = np.random.default_rng(8)
+    counts, lengths = np.array([70, 1, 90, 2], np.uint32), np.array([200, 33, 90, 400], np.uint32)
+    pages = rng.permutation(4 * 25).astype(np.uint32).reshape(4, 25)
+    k, v = (rng.standard_normal((100 * block, kv, Dh)).astype(np.float16) for _ in range(2))
+    q1, q2 = rng.standard_normal((300, qH, Dh)).astype(np.float32), rng.standard_normal((163, qH, Dh)).astype(np.float32)
+    n1 = np.array([400], np.uint32)
+    x, t = rng.standard_normal((5, 1000)).astype(np.float16), rng.integers(0, 1000, 5).astype(np.uint32)
+    gpu = lambda a: torch.from_numpy(a.view(np.int32) if a.dtype == np.uint32 else a).to(DEV)
+    kd, vd = gpu(k), gpu(v)
+    o = dict(scale=0.2, window=window, sinks=sinks)
+    want1 = T.attention(gpu(q1), kd, vd, T.AttentionOptions(lengths=gpu(n1), pages=gpu(pages[3]), block=block, base=100, **o)).cpu().numpy()
+    want2 = T.attention(gpu(q2), kd, vd, T.AttentionOptions(lengths=gpu(lengths), pages=gpu(pages), block=block,
+                                                            query_extents=gpu(counts), **o)).cpu().numpy()
+    r = T.token_logprobs(gpu(x), gpu(t), top=3)
+    dev = D.Device(0, use_graphs=graphs)
+    op = lambda b, n=None: D.Operand(block=b, offset=0, size=b.size if n is None else n)
+    up = lambda a: dev.upload(np.ascontiguousarray(a))
+    blocks = [up(a) for a in (k, v, q1, n1, pages[3], q2, lengths, pages, np.r_[0, np.cumsum(counts)].astype(np.uint32), x, t)]
+    bk, bv, bq1, bn1, bp3, bq2, bl, bp, boff, bx, bt = blocks
+    outs = [dev.alloc(n) for n in (q1.nbytes, q2.nbytes, 20, 20, 60, 60)]
+    dims = lambda batch, mp, q_seq, base: rt.window_dims(batch, qH, kv, Dh, block, mp, 0.2, window, sinks, 100 * block, q_seq, base)
+    exe = dev.compile([
+        D.Dispatch("AttentionWindowPrefillPagedF16", [op(bq1, q1.nbytes), op(bk, k.nbytes), op(bv, k.nbytes), op(bp3, 100), op(bn1, 4),
+                                                      op(outs[0], q1.nbytes)], dims(1, 25, 300, 100)),
+        D.Dispatch("AttentionWindowRaggedF16", [op(bq2, q2.nbytes), op(bk, k.nbytes), op(bv, k.nbytes), op(bp, 400), op(bl, 16), op(boff, 20),
+                                                op(outs[1], q2.nbytes)], dims(4, 25, 0, 0)),
+        D.Dispatch("TokenLogprobsF16", [op(bx, x.nbytes), op(bt, 20), op(outs[2], 20), op(outs[3], 20), op(outs[4], 60), op(outs[5], 60)],
+                   rt.logprob_dims(1000, 5, 1, 3)),
+    ], max_in_flight=2)
+    for _ in range(2):
+        fences = [exe.submit(), exe.submit()]
+        for f in fences:
+            f.wait()
+        assert np.array_equal(outs[0].read(0, np.zeros_like(q1)), want1) and np.array_equal(outs[1].read(0, np.zeros_like(q2)), want2)
+        for b, w in zip(outs[2:], (r.logprobs, r.entropy, r.top_ids, r.top_logprobs)):
+            w = w.cpu().numpy()
+            assert np.array_equal(b.read(0, np.zeros_like(w)), w)
+    exe.close()
+    for b in blocks + outs:
+        b.free()
+    dev.close()
+    rt.attention_error()
