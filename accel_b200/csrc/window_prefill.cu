@@ -389,9 +389,11 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
     Segment keys = plan.one;
     uint32_t rt = plan.max_row_tiles - 1 - index % plan.max_row_tiles;
     if (plan.segments) {
-        if (rt >= plan.counts[1]) return;
-        const uint2 e = plan.row_tiles[rt];
-        if (e.x == 0xffffffffu) return;
+        const uint2 e = rt < plan.counts[1] ? plan.row_tiles[rt] : make_uint2(0xffffffffu, 0);
+        if (e.x == 0xffffffffu) {
+            pdl_wait();                                  // (this kernel is done when all before it is, whatever it had to do)
+            return;
+        }
         keys = plan.segments[e.x];
         rt = e.y;
     }
@@ -808,6 +810,7 @@ __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32
     __shared__ uint4 part[8];
     __shared__ uint32_t part_left[8];
     const uint32_t t = threadIdx.x, lane = t & 31, group = p.q_heads / p.kv_heads, per_tile = kRows / group;
+    pdl_enter();                                         // (the rows' kernel may come and wait)
     uint4 before = make_uint4(0, 0, 0, 0);               // segments, key tiles, row tiles, rows left of the sequences so far
     for (uint32_t s0 = 0; s0 < p.batch; s0 += 256) {
         const uint32_t s = s0 + t;
@@ -933,10 +936,19 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, WindowRows 
         plan.counts = counts;
         uint4 *left = reinterpret_cast<uint4 *>(counts + 4);
         p.left = left;
-        win_plan_kernel<<<1, 256, 0, l.stream>>>(p, (uint32_t)segments, segs, kt, rt, counts, plan.max_key_tiles,
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(1);
+        cfg.blockDim = dim3(256);
+        cfg.stream = l.stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, win_plan_kernel, p, (uint32_t)segments, segs, kt, rt, counts, plan.max_key_tiles,
                                                  plan.max_row_tiles, left);
         count_launch();
-        rc = check_cuda(cudaGetLastError(), name);
+        rc = check_cuda(e, name);
         if (rc == AB_OK) rc = rows_kernel(l, p, name);
         if (rc) return rc;
     }
@@ -956,7 +968,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, WindowRows 
     for (uint32_t h = 0; h < p.kv_heads && row_tiles; h += pass) {
         const uint32_t now = std::min(pass, p.kv_heads - h);
         // A ragged step's rows left run beside the packing, which waits for them at its end: it is their programmatic dependent,
-        // and what it reads was there before either.  Its grid is two rounds of CTAs, which take what tiles there are by
+        // and they let it start once the plan, which both read, is complete.  Its grid is two rounds of CTAs, which take what tiles there are by
         // turns (the bound on their number is many times that).  8 single tokens and 4 chunks of 64 over windows of 1024, f16:
         // rows 19 and packing 21 us one after the other, 29 us together
         if (key_tiles) {
@@ -974,8 +986,8 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, WindowRows 
             rc = check_cuda(e, name);
             if (rc) return rc;
         }
-        // a programmatic dependent of the pack kernel: its set-up and query rows (which no kernel of this call writes) overlap it.
-        // Beside a plan kernel nothing may be read early, and the launch is an ordinary one
+        // a programmatic dependent of the pack kernel: its set-up and query rows (which no kernel of this call writes) overlap it;
+        // a plan was complete before the packing began
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((uint32_t)row_tiles * now * split);
         cfg.blockDim = dim3(kTileThreads);
@@ -983,7 +995,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, WindowRows 
         cfg.stream = l.stream;
         cudaLaunchAttribute attr[2];
         cfg.attrs = attr;
-        if (key_tiles && !ragged) {
+        if (key_tiles) {
             attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
             attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
         }
