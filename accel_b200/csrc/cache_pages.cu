@@ -29,6 +29,7 @@ template <int P> struct CopyParams {
 
 template <typename V, int P> __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ CopyParams<P> p)
 {
+    pdl_wait();
     const uint32_t chunk = blockIdx.x % p.chunks, pair = blockIdx.x / p.chunks;
     char *cache = static_cast<char *>(p.cache[blockIdx.y]);
     const uint64_t at = (uint64_t)chunk * kChunk;
@@ -45,6 +46,14 @@ int run_copy(cudaStream_t stream, void *const *caches, int n_caches, uint64_t pa
     CopyParams<P> p;
     p.page_bytes = page_bytes;
     p.chunks = (uint32_t)((page_bytes + kChunk - 1) / kChunk);
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     const int per_launch = (int)std::min<uint64_t>(P, std::max<uint64_t>(1, 0x7fffffffull / p.chunks));
     for (int c0 = 0; c0 < n_caches; c0 += kMaxCaches)
         for (int i0 = 0; i0 < n_pairs; i0 += per_launch) {
@@ -53,9 +62,10 @@ int run_copy(cudaStream_t stream, void *const *caches, int n_caches, uint64_t pa
             memcpy(p.cache, caches + c0, p.n_caches * sizeof(void *));
             memcpy(p.src, src + i0, p.n_pairs * 4);
             memcpy(p.dst, dst + i0, p.n_pairs * 4);
-            copy_pages_kernel<V, P><<<dim3(p.chunks * p.n_pairs, p.n_caches), kThreads, 0, stream>>>(p);
+            cfg.gridDim = dim3(p.chunks * p.n_pairs, p.n_caches);
+            const cudaError_t e = cudaLaunchKernelEx(&cfg, copy_pages_kernel<V, P>, p);
             count_launch();
-            const int rc = check_cuda(cudaGetLastError(), "ab_cache_copy_pages");
+            const int rc = check_cuda(e, "ab_cache_copy_pages");
             if (rc) return rc;
         }
     return AB_OK;

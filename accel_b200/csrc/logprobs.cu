@@ -150,6 +150,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 6) logprobs_ke
     __shared__ uint32_t maxima[kWarps * (kMaxTop / kWarps + 2)], at_floor, n_list, n_held;
     __shared__ uint8_t held[kThreads];
     __shared__ u64 list[kList], best[kMaxTop], all[16 * kMaxTop], slow[kWarps];
+    pdl_wait();
     const uint32_t row = blockIdx.x / parts, part = blockIdx.x % parts, V = p.vocab, t = threadIdx.x;
     const int warp = t >> 5, lane = t & 31;
     const T *x = static_cast<const T *>(p.x) + (size_t)row * V;
@@ -421,12 +422,14 @@ template <typename T> int run_logprobs(Launch &l, const char *name)
     cfg.gridDim = dim3(p.rows * parts);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = l.stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = parts;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = parts > 1 ? 1 : 0;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = parts;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = parts > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, p, parts);
     count_launch();
     note_selection("%s: %u CTA(s) per row", name, parts);

@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kPackThreads, sizeof(T) == 2 ? 3 : 2)
 win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, TileHead *heads, uint32_t kvh0)
 {
     __shared__ uint32_t rows[kKeys], amax_bits, bad_any;
+    if (!Plan) pdl_wait();
     pdl_trigger();                                       // the tile kernel may set itself up meanwhile
     const uint32_t kvh = kvh0 + blockIdx.y, t = threadIdx.x, D = p.head_dim, lane = t & 31;
     // elements of a thread; dimensions that it takes of V together (4 bytes of a position); groups of eight positions at a time
@@ -980,7 +981,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, WindowRows 
             attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
             attr[0].val.programmaticStreamSerializationAllowed = 1;
             cfg.attrs = attr;
-            cfg.numAttrs = ragged && h == 0 ? 1 : 0;
+            cfg.numAttrs = !ragged || h == 0 ? 1 : 0;
             const cudaError_t e = cudaLaunchKernelEx(&cfg, ragged ? win_pack_kernel<T, DP, true> : win_pack_kernel<T, DP, false>, p, plan, tiles, heads, h);
             count_launch();
             rc = check_cuda(e, name);
