@@ -802,6 +802,8 @@ int window_form(Launch &l, Form form, bool paged, bool f16, const char *name)
         return fail(AB_ERR_INVALID, "%s: a window of 0 positions; a query sees at least its own (without a window: "
                     "the Attention kernels)", name);
     const uint64_t per = (uint64_t)p.q_heads * p.head_dim, kvper = (uint64_t)p.kv_heads * p.head_dim;
+    if (form == kRaggedStep && l.len[0] == 0xffffffffu)
+        return fail(AB_ERR_INVALID, "%s: q's length, which says how many rows there are, does not fit 32 bits", name);
     if (form == kRaggedStep) p.rows = per ? (uint32_t)(l.len[0] / per) : 0;
     int i = 3;
     const int pages_i = paged ? i++ : -1, len_i = i++, off_i = form == kRaggedStep ? i++ : -1, out_i = i;

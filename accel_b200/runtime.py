@@ -8,7 +8,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import struct
-from typing import Optional, Sequence
+from typing import List, Optional, Sequence
 
 import torch
 
@@ -43,9 +43,12 @@ def paged_prefill_dims(q_heads, kv_heads, head_dim, q_seq, base, block, scale) -
     return struct.pack("<IIIIIIfI", q_heads, kv_heads, head_dim, q_seq, base, block, scale, 0)
 
 
+_window_dims = struct.Struct("<IIIIIIfIIIII").pack
+
+
 def window_dims(batch, q_heads, kv_heads, head_dim, block, max_pages, scale, window, sinks, capacity, q_seq, base) -> bytes:
     # WindowDims: the window forms' own block
-    return struct.pack("<IIIIIIfIIIII", batch, q_heads, kv_heads, head_dim, block, max_pages, scale, window, sinks,
+    return _window_dims(batch, q_heads, kv_heads, head_dim, block, max_pages, scale, window, sinks,
                        capacity, q_seq, base)
 
 
@@ -164,36 +167,40 @@ _pointers = [struct.Struct(f"{n}Q").pack for n in range(16)]
 _counts = [struct.Struct(f"{n}I").pack for n in range(16)]
 
 
-def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: bytes, scratch: bool = False):
+# the current device's number, where torch offers it without a look at whether CUDA is up
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: bytes, scratch: bool = False,
+               lens: Optional[List[int]] = None):
     """`launch` for the operators whose scratch memory (scratch: they may need some) is the call's own:
     it comes from torch's allocator, so a call captured into a CUDA graph keeps it in that graph's pool
     and two graphs, or two streams, never share it.  The bindings are contiguous: the caller has seen to
-    that, and the first is a tensor on a device.  A binding of None is empty; one of more elements
+    that, and the first is a tensor on a device.  A caller that knows how many elements each has says so (lens).  A binding
+    of None is empty; one of more elements
     than 32 bits count is passed as 0xffffffff, which those kernels read as that many or more."""
-    dev = bindings[0].device
-    if dev.type != "cuda":
-        raise _lib.AccelError(_lib.AB_ERR_NO_DEVICE, f"{name}: bindings live on {dev}; this backend "
+    index = bindings[0].get_device()
+    if index < 0:
+        raise _lib.AccelError(_lib.AB_ERR_NO_DEVICE, f"{name}: bindings live on {bindings[0].device}; this backend "
                               "runs on a CUDA device and has no CPU path")
-    index = dev.index
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return launch_own(name, bindings, uniform, scratch)
-    ptrs, lens = [], []
-    for t in bindings:
-        n = 0 if t is None else t.numel()
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return launch_own(name, bindings, uniform, scratch, lens)
+    if lens is None:
+        lens = [0 if t is None else min(t.numel(), 0xffffffff) for t in bindings]
+    ptrs = []
+    for t, n in zip(bindings, lens):
         if n == 0:
             ptrs.append(0)
-            lens.append(0)
             continue
         if t.get_device() != index:
-            raise ValueError(f"{name}: every binding is a contiguous tensor on {dev}")
+            raise ValueError(f"{name}: every binding is a contiguous tensor on {bindings[0].device}")
         ptrs.append(t.data_ptr())
-        lens.append(n if n < 0xffffffff else 0xffffffff)
     ws, ws_bytes = None, 0
     if scratch:
         ws_bytes = workspace_bytes(name, lens, uniform)
         if ws_bytes:
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=bindings[0].device)
     count = len(ptrs)
     rc = _lib.lib().ab_launch(_encoded(name), _raw_stream(index), _pointers[count](*ptrs), _counts[count](*lens), count,
                               uniform, len(uniform), ws.data_ptr() if ws is not None else None, ws_bytes)
@@ -208,7 +215,7 @@ def copy_pages(caches: Sequence[torch.Tensor], pointers: Sequence[int], src: Seq
     if dev.type != "cuda":
         raise _lib.AccelError(_lib.AB_ERR_NO_DEVICE, f"copy_pages: the caches live on {dev}; this backend runs on a CUDA "
                               "device and has no CPU path")
-    if dev.index != torch.cuda.current_device():
+    if dev.index != _current_device():
         with torch.cuda.device(dev):
             return copy_pages(caches, pointers, src, dst, block)
     page_bytes = t.numel() // t.shape[0] * t.element_size() * block if t.numel() else 0

@@ -283,18 +283,23 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, opts: Attention
             raise Refused(op, f"a cache's capacity is {capacity}; positions are u32")
         if opts.block > 0xffffffff:
             raise Refused(op, f"Block is {opts.block}; positions are u32")
+        n = rows * q_heads * head_dim
+        if n > 0xffffffff:
+            raise Refused(op, f"q holds {n} elements; a call counts them in 32 bits, so it takes several calls")
         out = q.new_empty(rows, q_heads, head_dim)
-        if rows and q_heads and head_dim:
-            b = [q, k, v]
+        if n:
+            cached = min(capacity * kv_heads * head_dim, 0xffffffff)
+            lengths = _aligned(opts.lengths)
+            b, lens = [q, k, v, lengths, out], [n, cached, cached, batch, n]
             if pages is not None:
-                b.append(_aligned(pages))
-            b.append(_aligned(opts.lengths))
+                b.insert(3, _aligned(pages))
+                lens.insert(3, pages.numel())
             if offsets is not None:
-                b.append(_aligned(offsets))
-            b.append(out)
+                b.insert(5, _aligned(offsets))
+                lens.insert(5, batch + 1)
             rt.launch_own("AttentionWindow" + form + ("F16" if f16 else ""), b,
                           rt.window_dims(batch, q_heads, kv_heads, head_dim, opts.block, max_pages, scale, window, sinks,
-                                         capacity, rows, base), scratch=prefill or ragged)
+                                         capacity, rows, base), prefill or ragged, lens)
         return out
 
     if prefill:
@@ -658,7 +663,8 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     if rows:
         rt.launch_own("TokenLogprobsF16" if f16 else "TokenLogprobs",
                       [_aligned(logits), None if targets is None else _aligned(targets), lp, out.entropy,
-                       out.top_ids, out.top_logprobs], rt.logprob_dims(vocab, rows, n, top))
+                       out.top_ids, out.top_logprobs], rt.logprob_dims(vocab, rows, n, top), False,
+                      [min(x, 0xffffffff) for x in (rows * vocab, rows * n, rows * n, rows, rows * top, rows * top)])
     return out
 
 

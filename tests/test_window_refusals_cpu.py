@@ -132,3 +132,14 @@ def test_positions_are_u32():
     with pytest.raises(T.Refused, match="Block is 4294967296"):
         T.attention(q, k[:64], k[:64], T.AttentionOptions(lengths=lens, window=4, block=1 << 32,
                                                           pages=torch.zeros(3, dtype=torch.int32, device="meta")))
+
+
+def test_query_rows_are_counted_in_32_bits():
+    q = torch.empty(1 << 24, 32, 8, device="meta")                # 2^32 elements
+    k = torch.empty(64, 32, 8, device="meta")
+    one = torch.ones(1, dtype=torch.int32, device="meta")
+    with pytest.raises(T.Refused, match="counts them in 32 bits"):
+        T.attention(q, k, k, T.AttentionOptions(lengths=one, window=4, base=0))
+    with pytest.raises(_lib.AccelError, match="does not fit 32 bits"):
+        rt.workspace_bytes("AttentionWindowRagged", [0xffffffff, 64 * 256, 64 * 256, 4, 1, 2, 0xffffffff],
+                           window(batch=1, qh=32, kv=32, d=8, block=16, mp=4, cap=64))
