@@ -55,8 +55,9 @@ __device__ __forceinline__ void cluster_sync()
 
 // Whether `rows` query rows (tokens x heads of a KV head) of one sequence, each of which sees up to `seen` positions, go
 // on 128-row tiles.  A tile call costs its two launches and the packing of the positions, whatever the rows; the row
-// kernel's time grows with rows x seen.  (8 KV heads, head dimension 128; tiles / rows one by one, us:
-//     rows x seen           f32, groups of 4      f16, groups of 4      f16, groups of 8 (4 KV heads)
+// kernel's time grows with rows x seen x KV heads.  (Head dimension 128, contiguous; tiles / rows one by one, us:
+//     rows x seen           f32, groups of 4      f16, groups of 4      f16, groups of 8
+//                           8 KV heads            8 KV heads            4 KV heads
 //       32 x   512          20.8 /  11.5          17.8 /  11.9          17.7 /  10.3
 //       64 x   512          21.4 /  15.7          17.7 /  13.7          17.7 /  10.5
 //      128 x   512          21.7 /  22.8          17.7 /  18.8          17.6 /  13.6
@@ -66,11 +67,20 @@ __device__ __forceinline__ void cluster_sync()
 //       64 x  4096          35.7 /  85.6          29.3 /  44.1          24.2 /  31.1
 //       16 x 32768         185.5 / 147.0         147.7 / 123.2         103.8 /  57.8
 //       32 x 32768         185.4 / 319.5         147.9 / 144.7         103.4 /  67.8
-//       64 x 32768         186.0 / 587.2         148.7 / 278.6         104.3 / 125.3 )
+//       64 x 32768         186.0 / 587.2         148.7 / 278.6         104.3 / 125.3
+//  and with 32 KV heads of one query head each
+//       32 x   512          23.9 /  57.8          19.7 /  40.4
+//      128 x   512          24.0 / 143.7          19.7 / 132.5
+//       64 x  2048          51.7 / 279.0          32.4 / 270.7
+//  with one KV head of eight
+//      128 x   512          21.0 /  15.8          16.7 /   9.6
+//      128 x  2048          23.1 /  20.0          18.7 /  14.3
+//       64 x  8192          33.2 /  36.3          26.2 /  21.9
+//      256 x  2048          23.1 /  24.0          18.8 /  23.9 )
 constexpr uint32_t kTileFrom = 32;
-__host__ __device__ inline bool on_tiles(uint64_t rows, uint64_t seen)
+__host__ __device__ inline bool on_tiles(uint64_t rows, uint64_t seen, uint32_t kv_heads)
 {
-    return rows >= 256 || (rows >= kTileFrom && rows * seen >= 65536);
+    return rows >= 256 || (rows >= kTileFrom && rows * seen >= (8u * 65536u + kv_heads - 1) / kv_heads);
 }
 // a prefill, or a ragged step: its sequences with that many rows, on 128-row tiles (window_prefill.cu); p.left says which rows
 // are left, and `rows` launches the kernel for those.  p.q_heads / p.kv_heads <= 128

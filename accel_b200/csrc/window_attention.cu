@@ -773,7 +773,7 @@ template <typename T> int run_window(Launch &l, WinParams &p, const char *name)
     // row kernel's time, and took 7.0 us more of kernels without work)
     const uint64_t most = p.form == kPrefillRows ? p.rows : (p.form == kRaggedStep && p.rows >= p.batch ? p.rows - p.batch + 1 : 0);
     const uint64_t seen = std::min<uint64_t>((uint64_t)p.window + p.sinks, p.form == kPrefillRows ? std::min<uint64_t>((uint64_t)p.base + p.rows, p.reach) : p.reach);
-    if (group <= 128 && on_tiles(most * group, seen)) return run_window_tiles(l, p, sizeof(T) == 2, run_rows<T>, name);
+    if (group <= 128 && on_tiles(most * group, seen, p.kv_heads)) return run_window_tiles(l, p, sizeof(T) == 2, run_rows<T>, name);
     return l.query_ws ? AB_OK : run_rows<T>(l, p, name);
 }
 

@@ -826,7 +826,7 @@ __global__ void __launch_bounds__(256) win_plan_kernel(const WinParams p, uint32
             mine_left = b > a ? b - a : 0;
             // (a sequence with more tokens than positions has rows of zeros: the row kernel knows)
             if (b > a && b == p.offsets[s + 1] && len >= b - a &&
-                on_tiles((uint64_t)(b - a) * group, min((uint64_t)p.window + p.sinks, (uint64_t)min(len, p.reach)))) {
+                on_tiles((uint64_t)(b - a) * group, min((uint64_t)p.window + p.sinks, (uint64_t)min(len, p.reach)), p.kv_heads)) {
                 g.row0 = a; g.rows = b - a; g.base = len - (b - a); g.seq = s;
                 g.end = min(len, p.reach);
                 segment_list(g, p.window, p.sinks);

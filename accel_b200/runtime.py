@@ -176,9 +176,9 @@ def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: b
     """`launch` for the operators whose scratch memory (scratch: they may need some) is the call's own:
     it comes from torch's allocator, so a call captured into a CUDA graph keeps it in that graph's pool
     and two graphs, or two streams, never share it.  The bindings are contiguous: the caller has seen to
-    that, and the first is a tensor on a device.  A caller that knows how many elements each has says so (lens).  A binding
-    of None is empty; one of more elements
-    than 32 bits count is passed as 0xffffffff, which those kernels read as that many or more."""
+    that, and the first is a tensor on a device.  A caller that knows how many elements each has says so (lens).  A binding of
+    None is empty; one of more elements than 32 bits count is passed as 0xffffffff, which those kernels read as that many or
+    more."""
     index = bindings[0].get_device()
     if index < 0:
         raise _lib.AccelError(_lib.AB_ERR_NO_DEVICE, f"{name}: bindings live on {bindings[0].device}; this backend "
@@ -196,14 +196,17 @@ def launch_own(name: str, bindings: Sequence[Optional[torch.Tensor]], uniform: b
         if t.get_device() != index:
             raise ValueError(f"{name}: every binding is a contiguous tensor on {bindings[0].device}")
         ptrs.append(t.data_ptr())
-    ws, ws_bytes = None, 0
+    count, counts, ws, ws_bytes = len(ptrs), _counts[len(ptrs)](*lens), None, 0
     if scratch:
-        ws_bytes = workspace_bytes(name, lens, uniform)
+        need = C.c_size_t(0)
+        rc = _lib.lib().ab_workspace_bytes(_encoded(name), counts, count, uniform, len(uniform), C.byref(need))
+        if rc:
+            _lib.check(rc)
+        ws_bytes = need.value
         if ws_bytes:
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=bindings[0].device)
-    count = len(ptrs)
-    rc = _lib.lib().ab_launch(_encoded(name), _raw_stream(index), _pointers[count](*ptrs), _counts[count](*lens), count,
-                              uniform, len(uniform), ws.data_ptr() if ws is not None else None, ws_bytes)
+            ws = bindings[0].new_empty(ws_bytes, dtype=torch.uint8)
+    rc = _lib.lib().ab_launch(_encoded(name), _raw_stream(index), _pointers[count](*ptrs), counts, count, uniform, len(uniform),
+                              ws.data_ptr() if ws is not None else None, ws_bytes)
     if rc:
         _lib.check(rc)
 

@@ -387,7 +387,7 @@ def segment_offsets(counts: torch.Tensor) -> torch.Tensor:
     """tensor/segment.go: exclusive prefix sum counts[R] -> offsets[R+1], on the device."""
     rows = counts.numel()
     offsets = torch.empty(rows + 1, dtype=counts.dtype, device=counts.device)
-    rt.launch("SegmentOffsets", [counts.contiguous(), offsets], rt.segment_dims(rows))
+    rt.launch_own("SegmentOffsets", [counts.contiguous(), offsets], rt.segment_dims(rows), False, [rows, rows + 1])
     return offsets
 
 

@@ -381,9 +381,9 @@ def test_ragged_chunks_in_graphs_on_two_streams():
 
 
 @pytest.mark.parametrize("f16", [False, True])
-@pytest.mark.parametrize("tokens,n,tiles", [(31, 2112, False), (32, 2111, True), (32, 1900, False), (255, 255, False), (256, 256, True)])
+@pytest.mark.parametrize("tokens,n,tiles", [(31, 4200, False), (127, 2112, False), (128, 2048, True), (128, 2047, False), (255, 255, False), (256, 256, True)])
 def test_prefill_on_either_side_of_the_choice_of_kernel(tokens, n, tiles, f16):
-    kv, D, window, sinks = 2, 64, 2044, 4                         # 32 rows x 2048 positions, or 256 rows
+    kv, D, window, sinks = 2, 64, 2044, 4                         # 128 rows x 2048 positions x 2 KV heads, or 256 rows
     rng = np.random.default_rng(tokens)
     k, v = (rng.standard_normal((n, kv, D)).astype(np.float16 if f16 else np.float32) for _ in range(2))
     q = rng.standard_normal((tokens, kv, D)).astype(np.float32)
