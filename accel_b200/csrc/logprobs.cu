@@ -163,7 +163,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 6) logprobs_ke
     // ---- one pass
     Sums a{kLowest, 0.f, 0.f};
     const auto fetch = [&](uint32_t i) {
-        return i < p1 ? __ldg(reinterpret_cast<const uint4 *>(xp) + i) : make_uint4(Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone);
+        return i < p1 ? reinterpret_cast<const uint4 *>(xp)[i] : make_uint4(Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone, Piece<T>::kNone);
     };
     uint4 next[U];
 #pragma unroll

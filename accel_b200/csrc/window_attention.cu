@@ -92,7 +92,7 @@ __device__ __forceinline__ uint32_t win_page(const WinParams &p, const WinView &
 {
     uint32_t pg = 0xffffffffu;
     if (i < w.n && w.pages)
-        asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(pg) : "l"(w.pages + win_position(w, i) / p.block));
+        asm volatile("ld.global.u32 %0, [%1];" : "=r"(pg) : "l"(w.pages + win_position(w, i) / p.block));
     return pg;
 }
 __device__ __forceinline__ uint32_t win_row(const WinParams &p, const WinView &w, uint32_t i, uint32_t page)

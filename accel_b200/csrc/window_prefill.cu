@@ -97,8 +97,6 @@ template <typename T, int DP> constexpr uint32_t kTileBytes = 2 * kParts<T> * kS
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float2 two(const float *p) { return __ldg(reinterpret_cast<const float2 *>(p)); }
-__device__ __forceinline__ float2 two(const __half *p) { return __half22float2(__ldg(reinterpret_cast<const __half2 *>(p))); }
 
 // the power of two that brings a largest magnitude into [2^13, 2^14), as an exponent
 __device__ __forceinline__ int fit_exponent(float amax)
@@ -189,7 +187,7 @@ win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, Ti
                     const uint32_t r = rows[key];
                     x[i] = make_uint4(0, 0, 0, 0);
                     if (r != 0xffffffffu && d < D)
-                        x[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.k) + ((uint64_t)r * p.kv_heads + kvh) * D + d));
+                        x[i] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.k) + ((uint64_t)r * p.kv_heads + kvh) * D + d);
                 }
 #pragma unroll
                 for (int i = 0; i < kEach / 8; i++) {
@@ -203,7 +201,7 @@ win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, Ti
 #pragma unroll
                 for (int i = 0; i < kEach / 2; i++) {
                     const uint32_t r = rows[(i / 8 * kTogether + group0) * 8 + (i & 7)];
-                    x[i] = r != 0xffffffffu && dim < D ? __ldg(reinterpret_cast<const uint32_t *>(v + (uint64_t)r * p.kv_heads * D)) : 0;
+                    x[i] = r != 0xffffffffu && dim < D ? *reinterpret_cast<const uint32_t *>(v + (uint64_t)r * p.kv_heads * D) : 0;
                 }
 #pragma unroll
                 for (int i = 0; i < kEach / 2; i++) {    // (values that are not finite are left out: see the other case)
@@ -240,8 +238,8 @@ win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, Ti
                     if (r != 0xffffffffu && d < D) {
                         const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const T *>(p.k) + ((uint64_t)r * p.kv_heads + kvh) * D + d);
                         uint4 raw[2];
-                        raw[0] = __ldg(src);
-                        raw[1] = __ldg(src + 1);
+                        raw[0] = src[0];
+                        raw[1] = src[1];
 #pragma unroll
                         for (int e = 0; e < 8; e++) x[i + e] = reinterpret_cast<const float *>(raw)[e];
                     }
@@ -412,7 +410,7 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
             for (int i = 0; i < DP / 16; i++) {
                 both[g][i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (on && 16 * i + at < D)
-                    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];"
+                    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];"
                                  : "=f"(both[g][i].x), "=f"(both[g][i].y), "=f"(both[g][i].z), "=f"(both[g][i].w) : "l"(q + 16 * i + at));
             }
         }
@@ -580,9 +578,9 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
         uint4 next_scale = make_uint4(0, 0, 0, 0), next_seen = next_scale;
         const auto look = [&](uint32_t i) {                         // a tile's header, a tile ahead of its use
             const TileHead *h = heads + tile_of(i);
-            asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+            asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(next_scale.x), "=r"(next_scale.y), "=r"(next_scale.z), "=r"(next_scale.w) : "l"(h));
-            asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4 + 16];"
+            asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4 + 16];"
                          : "=r"(next_seen.x), "=r"(next_seen.y), "=r"(next_seen.z), "=r"(next_seen.w) : "l"(h));
         };
         if ((uint32_t)wg < n) look(wg);
