@@ -221,7 +221,9 @@ template <int DP> struct QFrag<float, DP> {
 };
 template <int DP> struct QFrag<__half, DP> {
     uint32_t hi[DP / 8], lo[DP / 8];
-    // f16 has 5 bits of exponent: a head's q is scaled by a power of two that brings its largest element near one
+    // f16 has 5 bits of exponent: a head's q is scaled by a power of two that brings its largest element into [2^13, 2^14),
+    // so that one of 2^-17 of it still keeps 22 bits in its two parts, and one below that 2^-39 of the largest.  (The sums stay
+    // below 2^38.  Near one instead, the channels of a query at a thousandth of its largest would keep 15 bits)
     __device__ __forceinline__ void load(const float *q, bool on, uint32_t D, int t, float scale, float (&undo)[2])
     {
         float2 x[DP / 8];
@@ -236,7 +238,7 @@ template <int DP> struct QFrag<__half, DP> {
         }
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -126), 126);
+        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127 - 13, -126), 113);
 #pragma unroll
         for (int j = 0; j < DP / 8; j++) round_f16x2(x[j].x * ab_pow2(-e), x[j].y * ab_pow2(-e), hi[j], lo[j]);
         const float back = ab_pow2(e);

@@ -462,8 +462,9 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             amax = fminf(amax * fabsf(p.scale_log2), 3.402823466e38f);
-            // near one: the products with keys of up to 2^14 (or f16's largest) stay far inside f32
-            const int e = max(fit_exponent(amax) - 13, -126);
+            // [2^13, 2^14), as the keys: an element down to 2^-17 of the row's largest keeps all its bits, and the products (2^37 with
+            // f16's largest keys) stay far inside f32.  (Near one, 2^-25 of the largest was all that the small ones were held to)
+            const int e = fit_exponent(amax);
             const float f = ab_pow2(e);
             if ((lane & 3) == 0) row_scale[row] = ab_pow2(-e);
 #pragma unroll
