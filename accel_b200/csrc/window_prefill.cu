@@ -11,7 +11,9 @@
 // Accuracy.  q, K and V have up to 24 bits and f16 holds 11, so an operand is two f16 parts, x = hi + lo,
 // and a product three MMAs, lo.hi + hi.lo + hi.hi (2^-22 is dropped); an f16 cache is exact in one
 // part and its products take two.  Powers of two keep the parts inside f16's range: one per query row
-// and one per tile of an f32 cache; the softmax weights are carried times 2^14 (window_attention.cu).
+// and one per tile of an f32 cache; the softmax weights are carried times 2^14 (window_attention.cu).  Of an f32
+// cache, a tile whose elements lie too far apart for that goes to the CUDA cores (kReach, kSpread).  With an f16 cache an element
+// of a query is off by at most 2^-39 of the row's largest element, and a weight by 2^-39 of the row's largest weight.
 // The accumulators of a tile start from zero, the small products first, and the sums over tiles are
 // f32 additions in registers: an accumulator in the tensor core over thousands of positions would
 // truncate at every step.
@@ -50,10 +52,20 @@ constexpr float kBias = 14.f;               // the softmax weights are carried t
 // What the pack kernel says about a tile.
 struct TileHead {
     float k_scale, v_scale;                 // what the parts have to be multiplied by
-    uint32_t bad;                           // a value is not finite (it is left out of the tile)
-    uint32_t pad;
+    uint32_t flags;                         // kBad: a value is not finite (it is left out of the tile); kApart: see kSpread
+    float k_sum;                            // an f32 cache: at least the sum of the magnitudes of any position's key
     uint32_t seen[4];                       // a bit per position: it exists
 };
+constexpr uint32_t kBad = 1, kApart = 2;
+// An f32 tile's parts share one power of two, so an element below 2^-17 of the tile's largest is held to 2^-39 of that
+// largest and not to 22 bits of its own.  Two conditions say where that is as good as f32; rows for which one fails have that
+// tile's scores and values summed in f32 on the CUDA cores instead (exact_tile).
+// Keys and queries: a score is off by at most 2^-39 (largest key * sum |q| + largest |q| * sum |key|) beside what 22 bits of
+// every operand give; up to kReach of that product the error stays below 2^-23 of one, in the exponent of a weight.
+// Values: no position's and no dimension's largest magnitude (but for those that are all zero) lies more than kSpread binary
+// places below the tile's largest.  What is lost is then at most 2^-24 of the largest element of the position and of the dimension.
+constexpr float kReach = 65536.f;
+constexpr uint32_t kSpread = 14;
 
 // A sequence whose rows go on tiles, and the list of positions packed for it: sinks in front of the first row's window,
 // then all from that on.
@@ -139,6 +151,9 @@ __global__ void __launch_bounds__(kPackThreads, sizeof(T) == 2 ? 3 : 2)
 win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, TileHead *heads, uint32_t kvh0)
 {
     __shared__ uint32_t rows[kKeys], amax_bits, bad_any;
+    // an f32 cache, V: the exponents of the largest magnitudes, by position (a byte for each, of every 32 dimensions) and by
+    // dimension; 0 for zeros (and numbers below 2^-126)
+    __shared__ uint32_t sum_bits, smallest, of_positions[kPackThreads / 32 * 8], of_dims[DP];
     if (!Plan) pdl_wait();
     pdl_trigger();                                       // the tile kernel may set itself up meanwhile
     const uint32_t kvh = kvh0 + blockIdx.y, t = threadIdx.x, D = p.head_dim, lane = t & 31;
@@ -167,6 +182,10 @@ win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, Ti
         TileHead &head = heads[at];
         unsigned char *dst = tiles + at * kTileBytes<T, DP> + (blockIdx.z ? kParts<T> * kSlotBytes<T, DP> : 0);
         if (t == 0) { amax_bits = 0; bad_any = 0; }
+        if constexpr (sizeof(T) == 4) {
+            if (t == 0) { sum_bits = 0; smallest = 0xffffffffu; }
+            if (t < DP) of_dims[t] = 0;
+        }
         if (t < kKeys) {
             const uint64_t j = (uint64_t)span.x + t;
             uint32_t r = 0xffffffffu;
@@ -176,7 +195,6 @@ win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, Ti
             if (blockIdx.z == 0 && (t & 31) == 0) head.seen[t >> 5] = seen;
         }
         __syncthreads();
-        bool bad = false;
         if constexpr (sizeof(T) == 2) {
             if (blockIdx.z == 0) {
                 uint4 x[kEach / 8];
@@ -198,6 +216,7 @@ win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, Ti
             } else {
                 const T *v = static_cast<const T *>(p.v) + (uint64_t)kvh * D + dim;
                 uint32_t x[kEach / 2];
+                bool bad = false;
 #pragma unroll
                 for (int i = 0; i < kEach / 2; i++) {
                     const uint32_t r = rows[(i / 8 * kTogether + group0) * 8 + (i & 7)];
@@ -217,16 +236,15 @@ win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, Ti
                         make_uint4(__byte_perm(x[i], x[i + 1], 0x7632), __byte_perm(x[i + 2], x[i + 3], 0x7632),
                                    __byte_perm(x[i + 4], x[i + 5], 0x7632), __byte_perm(x[i + 6], x[i + 7], 0x7632));
                 }
+                if (__any_sync(0xffffffffu, bad) && lane == 0) bad_any = 1;
             }
-            if (blockIdx.z && __any_sync(0xffffffffu, bad) && lane == 0) bad_any = 1;
             __syncthreads();
             if (t == 0) {
-                if (blockIdx.z) { head.v_scale = 1.f; head.bad = bad_any; }
+                if (blockIdx.z) { head.v_scale = 1.f; head.flags = bad_any ? kBad : 0; }
                 else head.k_scale = 1.f;
             }
         } else {
             float x[kEach];
-            float big = 0.f;
             if (blockIdx.z == 0) {
 #pragma unroll
                 for (int i = 0; i < kEach; i += 8) {
@@ -254,23 +272,110 @@ win_pack_kernel(const WinParams p, const TilePlan plan, unsigned char *tiles, Ti
                     x[i] = on ? to_f32(*src) : 0.f;
                 }
             }
+            // the largest magnitude, and what kReach and kSpread ask about.  Values that are not finite show in the first look (in a
+            // sum; as an exponent of 255), and then a second one leaves them out
+            const auto look = [&](auto finite) {
+                float big = 0.f, all = 0.f;
+                bool lost;
+                if (blockIdx.z == 0) {
+                    float sums = 0.f;
 #pragma unroll
-            for (int i = 0; i < kEach; i++) {
-                const bool finite = fabsf(x[i]) <= 3.402823466e38f;
-                if (finite) big = fmaxf(big, fabsf(x[i]));
-                else bad = true;
-                // a value that is not finite would spoil rows that do not see it (0 * inf): it is left out here and added to the
-                // rows that do by the tile kernel.  A score is masked after its product, so a key may stay
-                if (!finite && blockIdx.z) x[i] = 0.f;
+                    for (int i = 0; i < kEach; i += 8) {
+                        float sum = 0.f;
+#pragma unroll
+                        for (int n = 0; n < 8; n++) {
+                            float y = fabsf(x[i + n]);
+                            if (decltype(finite)::value && !(y <= 3.402823466e38f)) y = 0.f;
+                            sum += y;
+                            big = fmaxf(big, y);
+                        }
+                        all += sum;
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 8);         // (a position's 32 dimensions: lanes 8 and 16 apart
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 16);        // have the rest)
+                        sums = fmaxf(sums, sum);
+                    }
+                    const uint32_t c = __reduce_max_sync(0xffffffffu, __float_as_uint(sums));
+                    if (lane == 0) atomicMax(&sum_bits, c);
+                    lost = !(all <= 3.402823466e38f);
+                } else {
+                    constexpr int kWords = kEach / 4;
+                    uint32_t exponents[kWords];                              // a byte a value
+#pragma unroll
+                    for (int i = 0; i < kEach; i += 4) {
+                        uint32_t u[4];
+#pragma unroll
+                        for (int n = 0; n < 4; n++) {
+                            big = fmaxf(big, fabsf(x[i + n]));
+                            u[n] = __float_as_uint(x[i + n]) << 1;
+                        }
+                        exponents[i / 4] = __byte_perm(__byte_perm(u[0], u[1], 0x73), __byte_perm(u[2], u[3], 0x73), 0x5410);
+                    }
+                    atomicMax(&of_dims[dim], __float_as_uint(big) >> 23);
+                    // the warp's 32 dimensions: lanes give away half of their words until each has one, then whole ones
+                    uint32_t word = 0;                                       // which of them a lane ends with
+#pragma unroll
+                    for (int w = 16, n = kWords; w; w /= 2) {
+                        if (n > 1) {
+                            n /= 2;
+                            const bool upper = (lane & w) != 0;
+                            if (upper) word += n;
+#pragma unroll
+                            for (int j = 0; j < n; j++) {
+                                const uint32_t give = upper ? exponents[j] : exponents[j + n], keep = upper ? exponents[j + n] : exponents[j];
+                                exponents[j] = __vmaxu4(keep, __shfl_xor_sync(0xffffffffu, give, w));
+                            }
+                        } else {
+                            exponents[0] = __vmaxu4(exponents[0], __shfl_xor_sync(0xffffffffu, exponents[0], w));
+                        }
+                    }
+                    of_positions[t / 32 * 8 + word] = exponents[0];          // (the lanes that share a word write the same)
+                    lost = __vcmpeq4(exponents[0], 0xffffffffu) != 0;
+                }
+                const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+                if (lane == 0) atomicMax(&amax_bits, b);
+                if (__any_sync(0xffffffffu, lost) && lane == 0) bad_any = 1;
+                __syncthreads();
+            };
+            look(std::false_type());
+            if (bad_any) {
+                // a value that is not finite would spoil rows that do not see it (0 * inf): it is left out here and added to
+                // the rows that do by the tile kernel.  A score is masked after its product, so a key may stay
+                if (blockIdx.z) {
+#pragma unroll
+                    for (int i = 0; i < kEach; i++)
+                        if (!(fabsf(x[i]) <= 3.402823466e38f)) x[i] = 0.f;
+                }
+                __syncthreads();
+                if (t == 0) amax_bits = sum_bits = 0;
+                if (t < DP) of_dims[t] = 0;
+                __syncthreads();
+                look(std::true_type());
             }
-            const uint32_t b = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
-            if (lane == 0) atomicMax(&amax_bits, b);
-            if (blockIdx.z && __any_sync(0xffffffffu, bad) && lane == 0) bad_any = 1;
-            __syncthreads();
             const int e = fit_exponent(__uint_as_float(amax_bits));
+            if (blockIdx.z) {
+                // (the DP / 32 warps that share a group's positions are neighbours)
+                uint32_t m = 0;
+                if (t < kKeys) {
+                    const uint32_t per = kEach, from = t / per * (DP / 32), i = t % per;
+#pragma unroll
+                    for (int w = 0; w < DP / 32; w++) m = max(m, of_positions[(from + w) * 8 + i / 4] >> (i % 4 * 8) & 255u);
+                } else if (t < kKeys + DP) {
+                    m = of_dims[t - kKeys];
+                }
+                const uint32_t least = __reduce_min_sync(0xffffffffu, m ? m : 0xffffffffu);
+                if (lane == 0 && least != 0xffffffffu) atomicMin(&smallest, least);
+                __syncthreads();
+            }
             if (t == 0) {
-                if (blockIdx.z) { head.v_scale = ab_pow2(-e); head.bad = bad_any; }
-                else head.k_scale = ab_pow2(-e);
+                if (blockIdx.z) {
+                    // (the weights' 2^14 goes with it: the sums of an f32 cache are carried without)
+                    head.v_scale = ab_pow2(-e) * (1.f / 16384.f);
+                    const bool apart = smallest != 0xffffffffu && smallest + kSpread < amax_bits >> 23;
+                    head.flags = (bad_any ? kBad : 0) | (apart ? kApart : 0);
+                } else {
+                    head.k_scale = ab_pow2(-e);
+                    head.k_sum = __uint_as_float(sum_bits) * (DP / 32);
+                }
             }
             const float f = ab_pow2(e);
 #pragma unroll
@@ -302,8 +407,8 @@ template <typename T, int DP> struct TileSmem {
     static constexpr uint32_t kQ = kRows * DP * 2;                  // one part of the query rows
     static constexpr uint32_t kRing = 2 * kQ;
     static constexpr uint32_t kBars = kRing + kSlots * kSlotBytes<T, DP>;
-    static constexpr uint32_t kScale = kBars + 256;                 // a power of two per query row
-    static constexpr uint32_t kBytes = kScale + kRows * 4;
+    static constexpr uint32_t kScale = kBars + 256;                 // of every query row: a power of two; its largest magnitude; the sum of all
+    static constexpr uint32_t kBytes = kScale + 3 * kRows * 4;
 };
 
 // sx_bar_wait without its function call: the softmax threads hold more registers than survive one
@@ -365,6 +470,149 @@ __device__ __forceinline__ Range win_range(const WinParams &p, const Segment &k,
     r.sinks_end = min(r.sinks_end, r.end);
     r.begin = min(max(r.sinks_end, k.sink_tiles + (lo - k.lo) / kKeys), r.end);
     return r;
+}
+
+// A tile whose elements lie too far apart for two f16 parts (kReach, kSpread), in f32 on the CUDA cores: by the softmax warps,
+// once the rows' outputs lie in shared memory.  The tile's keys and values are fetched as they are, behind those; a thread
+// has a row, works out the scores of half of the positions (its partner in the other group the others; they meet in tensor
+// memory), and then sums half of the dimensions.  2 x 128 x 128 multiply-adds a row, operands from shared memory, the same to all
+// lanes.  Measured: 2048 tokens of 32 heads over windows of 2048, 8 f32 KV heads, every tile this way: 3580 us
+// (231 us with ordinary numbers; one by one from global memory 44600).
+template <int DP> struct ExactSmem {
+    static constexpr uint32_t kRowOf = kRows * (DP + 4) * 4 + 8 * kRows * 4;          // the positions' cache rows
+    static constexpr uint32_t kK = kRowOf + kKeys * 4, kV = kK + kKeys * DP * 4, kEnd = kV + kKeys * DP * 4;
+};
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// all softmax threads, and what they wrote to tensor memory
+__device__ __forceinline__ void soft_sync()
+{
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// the same barrier; does any thread say yes?
+__device__ __forceinline__ bool soft_sync_or(bool x)
+{
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any) : "r"((uint32_t)x), "n"(kSoftWarps * 32) : "memory");
+    return any;
+}
+// q_row: the thread's query row; seen, mask: the positions that exist, those that the row sees; ts: tensor memory for its scores;
+// out: its half of its output, m and l: its maximum and its sum of weights
+template <int DP> __device__ __forceinline__ void exact_tile(const WinParams &p, const Segment &keys, uint32_t kvh, uint32_t j0, const uint4 &seen,
+                                                             const uint32_t (&mask)[4], const float *q_row, uint32_t ts, unsigned char *smem,
+                                                             float *out, float &m, float &l)
+{
+    using Smem = ExactSmem<DP>;
+    const uint32_t t = threadIdx.x, wg = t / 128, D = p.head_dim;
+    uint32_t *rows = reinterpret_cast<uint32_t *>(smem + Smem::kRowOf);
+    float4 *ks = reinterpret_cast<float4 *>(smem + Smem::kK), *vs = reinterpret_cast<float4 *>(smem + Smem::kV);
+    const auto word = [](const uint32_t (&w)[4], int i) { return i < 2 ? (i ? w[1] : w[0]) : (i == 2 ? w[2] : w[3]); };
+    const uint32_t there[4] = {seen.x, seen.y, seen.z, seen.w};
+    const auto any = [&](int w) { return (word(there, w / 4) >> (w % 4 * 8)) & 255; };       // of the w-th eight positions
+    soft_sync();                                         // (the tile before this one is done with)
+    if (t < kKeys)
+        rows[t] = (word(there, t / 32) >> (t & 31)) & 1
+                      ? win_cache_row(p, p.pages ? p.pages + (size_t)keys.seq * p.max_pages : nullptr, j0 + t) : 0xffffffffu;
+    soft_sync();
+    for (uint32_t i = t; i < kKeys * DP / 4; i += kSoftWarps * 32) {
+        const uint32_t row = rows[i / (DP / 4)], d = i % (DP / 4) * 4;
+        const uint64_t at = ((uint64_t)row * p.kv_heads + kvh) * D + d;
+        const bool on = row != 0xffffffffu && d < D;
+        ks[i] = on ? *reinterpret_cast<const float4 *>(static_cast<const float *>(p.k) + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+        vs[i] = on ? *reinterpret_cast<const float4 *>(static_cast<const float *>(p.v) + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    soft_sync();
+    {
+        float4 q[DP / 4];
+#pragma unroll
+        for (int i = 0; i < DP / 4; i++) {
+            q[i] = 4u * i < D ? *reinterpret_cast<const float4 *>(q_row + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+            q[i].x *= p.scale_log2; q[i].y *= p.scale_log2; q[i].z *= p.scale_log2; q[i].w *= p.scale_log2;
+        }
+#pragma unroll 1
+        for (int w = wg * 8; w < (int)wg * 8 + 8; w++) {
+            if (!any(w)) continue;
+            uint32_t s[8];
+#pragma unroll 2
+            for (int e = 0; e < 8; e += 4) {
+                float2 x[4] = {}, y[4] = {};
+#pragma unroll
+                for (int i = 0; i < DP / 4; i++)
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        const float4 k = ks[(8 * w + e + n) * (DP / 4) + i];
+                        x[n] = ab_fma2(make_float2(q[i].x, q[i].y), make_float2(k.x, k.y), x[n]);
+                        y[n] = ab_fma2(make_float2(q[i].z, q[i].w), make_float2(k.z, k.w), y[n]);
+                    }
+#pragma unroll
+                for (int n = 0; n < 4; n++) s[e + n] = __float_as_uint((x[n].x + x[n].y) + (y[n].x + y[n].y));
+            }
+            tmem_st8(ts + 8 * w, s);
+        }
+    }
+    soft_sync();
+    const auto eight = [&](int w, uint32_t (&s)[8]) {    // scores, -inf where the row does not look
+        const uint32_t bits = word(mask, w / 4) >> (w % 4 * 8);
+        tmem_ld8(ts + 8 * w, s);
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[e] = (bits >> e) & 1 ? s[e] : 0xff800000u;
+    };
+    float top = -CUDART_INF_F;
+#pragma unroll 1
+    for (int w = 0; w < 16; w++) {
+        if (!any(w)) continue;
+        uint32_t s[8];
+        eight(w, s);
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = fmaxf(top, __uint_as_float(s[e]));
+    }
+    const float m1 = fmaxf(m, top), ms = m1 == -CUDART_INF_F ? 0.f : m1, a = m == m1 ? 1.f : ab_ex2(m - m1);
+    float sum = 0.f;
+    float4 o[DP / 8];
+#pragma unroll
+    for (int i = 0; i < DP / 8; i++) {
+        o[i] = reinterpret_cast<const float4 *>(out)[i];
+        o[i].x *= a; o[i].y *= a; o[i].z *= a; o[i].w *= a;
+    }
+#pragma unroll 1
+    for (int w = 0; w < 16; w++) {
+        if (!any(w)) continue;
+        uint32_t s[8];
+        eight(w, s);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float x = ab_ex2(__uint_as_float(s[e]) - ms);
+            sum += x;
+            if (x != 0.f) {                              // (a value that is not finite stays with the rows that see it)
+                const float4 *v = vs + (8 * w + e) * (DP / 4) + wg * (DP / 8);
+#pragma unroll
+                for (int i = 0; i < DP / 8; i++) {
+                    const float4 y = v[i];
+                    const float2 lo = ab_fma2(make_float2(x, x), make_float2(y.x, y.y), make_float2(o[i].x, o[i].y));
+                    const float2 hi = ab_fma2(make_float2(x, x), make_float2(y.z, y.w), make_float2(o[i].z, o[i].w));
+                    o[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
+                }
+            }
+        }
+        __syncwarp();
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 8; i++) reinterpret_cast<float4 *>(out)[i] = o[i];
+    m = m1;
+    l = fmaf(l, a, sum);
 }
 
 template <typename T, int DP>
@@ -455,10 +703,14 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
         for (int g = 0; g < 2; g++) {
             const uint32_t row = warp * 16 + g * 8 + (lane >> 2);
             const float4 (&x)[DP / 16] = both[g];
-            float amax = 0.f;
+            float amax = 0.f, sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < DP / 16; i++)
+            for (int i = 0; i < DP / 16; i++) {
+                sum += (fabsf(x[i].x) + fabsf(x[i].y)) + (fabsf(x[i].z) + fabsf(x[i].w));
                 amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             amax = fminf(amax * fabsf(p.scale_log2), 3.402823466e38f);
@@ -466,7 +718,11 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
             // f16's largest keys) stay far inside f32.  (Near one, 2^-25 of the largest was all that the small ones were held to)
             const int e = fit_exponent(amax);
             const float f = ab_pow2(e);
-            if ((lane & 3) == 0) row_scale[row] = ab_pow2(-e);
+            if ((lane & 3) == 0) {
+                row_scale[row] = ab_pow2(-e);
+                row_scale[kRows + row] = amax;
+                row_scale[2 * kRows + row] = sum * fabsf(p.scale_log2);
+            }
 #pragma unroll
             for (int i = 0; i < DP / 16; i++) {
                 uint2 hi, lo;
@@ -567,6 +823,12 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
         pdl_wait();                                      // (for what follows of the pack kernel's)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const float q_scale = row_scale[r];
+        float q_max = 0.f, q_sum = 0.f;                  // of the CTA's rows
+        if constexpr (sizeof(T) == 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(row_scale + kRows + 4 * lane), y = *reinterpret_cast<const uint4 *>(row_scale + 2 * kRows + 4 * lane);
+            q_max = __uint_as_float(__reduce_max_sync(0xffffffffu, max(max(x.x, x.y), max(x.z, x.w))));
+            q_sum = __uint_as_float(__reduce_max_sync(0xffffffffu, max(max(y.x, y.y), max(y.z, y.w))));
+        }
         float m = -CUDART_INF_F, l = 0.f, o[DP];
         uint32_t bad = 0;
         const int wg = warp >> 2;
@@ -584,24 +846,36 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
             asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4 + 16];"
                          : "=r"(next_seen.x), "=r"(next_seen.y), "=r"(next_seen.z), "=r"(next_seen.w) : "l"(h));
         };
+        // do the rows take the tile in f32, after the others?
+        const auto exact = [&](const uint4 &head) {
+            return sizeof(T) == 4 && (!(q_sum * 16384.f * __uint_as_float(head.x) + q_max * __uint_as_float(head.w) <= kReach) || (head.z & kApart));
+        };
+        const auto rows_mask = [&](int64_t j0, uint32_t (&mask)[4]) {
+            const int top = (int)min(max(pos - j0 + 1, (int64_t)0), (int64_t)kKeys);
+            const int low = (int)min(max(lo_row - j0, (int64_t)0), (int64_t)kKeys);
+            const int snk = (int)min(max((int64_t)p.sinks - j0, (int64_t)0), (int64_t)kKeys);
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+                mask[w] &= bit_range(0, top - 32 * w) & (bit_range(low - 32 * w, 32) | bit_range(0, snk - 32 * w));
+        };
         if ((uint32_t)wg < n) look(wg);
         for (uint32_t i = wg; i < n; i += 2) {
             const int64_t j0 = win_tile_start(keys, tile_of(i));
-            const float c = fmaxf(q_scale * __uint_as_float(next_scale.x), 1.2e-38f), vs = __uint_as_float(next_scale.y);
-            bad |= next_scale.z;
+            const uint32_t flags = next_scale.z;
+            const float c = fmaxf(q_scale * __uint_as_float(next_scale.x), 1.2e-38f);
+            float vs = __uint_as_float(next_scale.y);
+            const bool later = exact(next_scale);
+            bad |= (flags & kBad) | (later ? kApart : 0);
             const uint4 seen = next_seen;
             if (i + 2 < n) look(i + 2);
             // does every row of the CTA see the whole tile?
-            const bool whole = (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && j0 + kKeys - 1 <= (int64_t)pa &&
+            const bool whole = !later && (seen.x & seen.y & seen.z & seen.w) == 0xffffffffu && j0 + kKeys - 1 <= (int64_t)pa &&
                                j0 + (int64_t)p.window > (int64_t)(pa + tokens - 1);
             uint32_t mask[4] = {seen.x, seen.y, seen.z, seen.w};
-            if (!whole) {
-                const int top = (int)min(max(pos - j0 + 1, (int64_t)0), (int64_t)kKeys);
-                const int low = (int)min(max(lo_row - j0, (int64_t)0), (int64_t)kKeys);
-                const int snk = (int)min(max((int64_t)p.sinks - j0, (int64_t)0), (int64_t)kKeys);
-#pragma unroll
-                for (int w = 0; w < 4; w++)
-                    mask[w] &= bit_range(0, top - 32 * w) & (bit_range(low - 32 * w, 32) | bit_range(0, snk - 32 * w));
+            if (later) {
+                mask[0] = mask[1] = mask[2] = mask[3] = 0;
+            } else if (!whole) {
+                rows_mask(j0, mask);
             }
             const auto word = [&](int w) { return w < 2 ? (w ? mask[1] : mask[0]) : (w == 2 ? mask[2] : mask[3]); };
             ok = __all_sync(0xffffffffu, bar_wait(&s_ready[wg], (i >> 1) & 1));
@@ -620,10 +894,15 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
                 for (int e = 4; e < 32; e++) x[e & 3] = fmaxf(x[e & 3], __uint_as_float(s[e]));
                 top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
             }
-            // (rounded up to a 64th: m1 - 14 is then exact, and so the weights of all tiles are relative to the same maxima)
-            const float m1 = fmaxf(m, ceilf(top * c * 64.f) * 0.015625f), ms = (m1 == -CUDART_INF_F ? 0.f : m1) - kBias;
-            const float a = m == m1 ? 1.f : ab_ex2(m - (ms + kBias));
+            // (rounded up to a whole number: m1 - 14 is then exact, so are the factors between maxima, and the weights of all tiles are
+            // relative to the same ones.)  An f32 cache's weights are relative to their own tile's maximum, and its product is
+            // brought to the row's afterwards: a tile of large values under small weights keeps its bits
+            const float mt = ceilf(top * c), m1 = fmaxf(m, mt), mw = sizeof(T) == 4 ? mt : m1;
+            const float ms = (mw == -CUDART_INF_F ? 0.f : mw) - kBias;
+            const float a = m == m1 ? 1.f : ab_ex2(m - m1);
+            const float down = sizeof(T) == 2 || mw == m1 ? 1.f : ab_ex2(mw - m1);
             m = m1;
+            vs *= down;
             float2 sum = make_float2(0.f, 0.f);
             const float2 c2 = make_float2(c, c), ms2 = make_float2(-ms, -ms);
 #pragma unroll 1
@@ -647,7 +926,7 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
                     sx_tmem_st16(ts + 32 * w + k, out);
                 }
             }
-            l = fmaf(l, a, sum.x + sum.y);
+            l = fmaf(l, a, sizeof(T) == 4 ? (sum.x + sum.y) * (down * (1.f / 16384.f)) : sum.x + sum.y);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -683,8 +962,9 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
         ml[wg * 3 * kRows] = m;
         ml[(wg * 3 + 1) * kRows] = l;
         ml[(wg * 3 + 2) * kRows] = __uint_as_float(bad);
-        asm volatile("bar.sync 1, %0;" ::"n"(kSoftWarps * 32) : "memory");
-        const float m0 = ml[0], m1 = ml[3 * kRows], M = fmaxf(m0, m1);
+        const bool apart = soft_sync_or(bad & kApart);   // (one answer for all: what hangs on it has barriers)
+        const float m0 = ml[0], m1 = ml[3 * kRows];
+        float M = fmaxf(m0, m1);
         const float f0 = m0 == -CUDART_INF_F ? 0.f : ab_ex2(m0 - M), f1 = m1 == -CUDART_INF_F ? 0.f : ab_ex2(m1 - M);
         const float fm = wg ? f1 : f0, fo = wg ? f0 : f1;
 #pragma unroll
@@ -696,13 +976,31 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
             x.w = fmaf(x.w, fo, (wg ? o[DP / 2 + i + 3] : o[i + 3]) * fm);
             *reinterpret_cast<float4 *>(mine + i) = x;
         }
-        if (live && (__float_as_uint(ml[2 * kRows]) | __float_as_uint(ml[5 * kRows]))) {
+        float L = fmaf(ml[kRows], f0, ml[4 * kRows] * f1);
+        bad |= __float_as_uint(ml[(2 + 3 * (wg ^ 1)) * kRows]);
+        if constexpr (sizeof(T) == 4) {
+            if (apart) {
+                const uint32_t row = live ? r : 0;
+                const float *q = p.q + ((uint64_t)(tok0 + row / group) * p.q_heads + (kvh0 + kv) * group + row % group) * D;
+                uint32_t left = 0;                       // of 32 tiles, a lane asking about one each
+                for (uint32_t i = 0; i < n; i++) {
+                    if (i % 32 == 0) left = __ballot_sync(0xffffffffu, i + lane < n && exact(*reinterpret_cast<const uint4 *>(heads + tile_of(i + lane))));
+                    if (!((left >> (i & 31)) & 1)) continue;
+                    look(i);
+                    const uint32_t j0 = win_tile_start(keys, tile_of(i));
+                    uint32_t mask[4] = {next_seen.x, next_seen.y, next_seen.z, next_seen.w};
+                    rows_mask(j0, mask);
+                    exact_tile<DP>(p, keys, kvh0 + kv, j0, next_seen, mask, q, tmem + ((uint32_t)(warp & 3) << 21), smem, mine, M, L);
+                }
+            }
+        }
+        if (live && (bad & kBad)) {
             // values that are not finite were left out of the tiles: a row that sees one gets it added
             const uint64_t end = min((uint64_t)win_end(p, plan, keys), (uint64_t)pos + 1);
             const uint32_t *pages = p.pages ? p.pages + (size_t)keys.seq * p.max_pages : nullptr;
             for (uint32_t i = 0; i < n; i++) {
                 const uint32_t tile = tile_of(i);
-                if (!heads[tile].bad) continue;
+                if (!(heads[tile].flags & kBad)) continue;
                 for (uint32_t x = 0; x < (uint32_t)kKeys; x++) {
                     const uint64_t j = (uint64_t)win_tile_start(keys, tile) + x;
                     if (!((heads[tile].seen[x >> 5] >> (x & 31)) & 1) || j >= end || (pos - (int64_t)j >= (int64_t)p.window && j >= p.sinks))
@@ -719,7 +1017,7 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
         if (wg == 0) {
             float *total = rows + kRows * kPitch + 6 * kRows + r;      // [m, l][row]
             total[0] = M;
-            total[kRows] = fmaf(ml[kRows], f0, ml[4 * kRows] * f1);
+            total[kRows] = L;
         }
     }
     // ---- the CTAs' parts of a row, in their order, and out: a warp writes a row (two, of a head of 64) at a time
@@ -891,6 +1189,7 @@ template <typename T, int DP> int run_tiles(Launch &l, WinParams &p, WindowRows 
 {
     static_assert(TileSmem<T, DP>::kBytes <= 232448, "shared memory of a CTA");
     static_assert(kRows * (DP + 4) * 4 + 8 * kRows * 4 <= TileSmem<T, DP>::kBars, "the parts of all groups fit where the operands were");
+    static_assert(ExactSmem<DP>::kEnd <= TileSmem<T, DP>::kBars, "and a tile in f32 behind them");
     const uint32_t group = p.q_heads / p.kv_heads, per_tile = kRows / group;
     const bool ragged = p.form == kRaggedStep;
     TilePlan plan{};
