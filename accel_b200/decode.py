@@ -404,10 +404,18 @@ class DecodeEngine:
 
     def compact(self) -> int:
         """Moves the pages in use to the pool's lowest numbers and returns how many moved; afterwards the
-        caches hold nothing beyond the first (pages in use) * block positions."""
+        caches hold nothing beyond the first (pages in use) * block positions.  The next step's inputs
+        may have been set already (set_inputs, advance_on_device): their slots move with their pages."""
         self.page_rows, s, d = self.pool.compact(self.page_rows)
         self._copy_pages(s, d)
         self.upload_pages()
+        if s:
+            blk = self.cfg.block
+            to = np.arange(self.capacity // blk)
+            to[s] = d
+            slots = self.slots.long() & 0xffffffff               # u32; past the cache: a row that is not written
+            page = torch.from_numpy(to).to(self.dev)[(slots // blk).clamp(max=len(to) - 1)]
+            self.slots.copy_(torch.where(slots < self.capacity, page * blk + slots % blk, slots))
         return len(s)
 
     def fill_context(self, context: int, seed: int = 7):
