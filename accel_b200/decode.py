@@ -274,8 +274,12 @@ class DecodeEngine:
     captured once as a CUDA graph and replayed."""
 
     def __init__(self, model: DecodeModel, batch: int, max_context: int, ops=rt, group=None,
-                 collective: str = "nccl", use_packed: Optional[bool] = None):
-        """collective: how the row-parallel products are summed over the ranks: "nccl" (the
+                 collective: str = "nccl", use_packed: Optional[bool] = None, pool_pages: Optional[int] = None):
+        """max_context: how many positions a sequence's page table addresses.  pool_pages: how many pages
+        there are for all sequences together (default: max_context positions for each).  With an attention
+        window fewer will do, however long the sequences get: trim() as they go gives back what is
+        behind it, and a long prompt is prefilled in pieces with a trim() after each.
+        collective: how the row-parallel products are summed over the ranks: "nccl" (the
         process group's all-reduce) or "peer" (this library's one-shot kernel over NVLink peer
         memory, peer.PeerAllReduce; GPUs only), or "skip": one rank of a sharded model run on its
         own with the sums over ranks left out (its results are NOT the model's: this is for
@@ -297,7 +301,7 @@ class DecodeEngine:
         B, d, D = batch, cfg.d_model, cfg.head_dim
         self.hq, self.hk = len(sh.heads), len(sh.kv_heads)
         self.max_pages = (max_context + cfg.block - 1) // cfg.block
-        pool_blocks = B * self.max_pages
+        pool_blocks = B * self.max_pages if pool_pages is None else pool_pages
         self.capacity = pool_blocks * cfg.block
         self.pool = BlockPool(pool_blocks, cfg.block)
         self.page_rows: List[List[int]] = [[] for _ in range(B)]
