@@ -19,7 +19,7 @@
 // truncate at every step.
 //
 // Bound: the tensor pipe.  4 (f16 cache) or 6 (f32) MMAs of 128 x 128 x 128 for every 128 x 128 scores where
-// 2 would be the floor.  A CTA of 320 threads per SM: two groups of four warps do the softmax of the even
+// 2 would be the floor.  A CTA of 384 threads per SM: two groups of four warps do the softmax of the even
 // and the odd tiles, each with its own maximum, sum and output in registers, so that one group's
 // exponentials run under the other's MMAs; one lane issues the MMAs in the order QK(0) QK(1) PV(0) QK(2)
 // PV(1) ..., one lane the bulk copies, in the same order, into a ring of slots.  Tensor memory: 128 columns of
