@@ -102,6 +102,9 @@ class BlockPool:
         if len(held) != self._blocks - self.available():
             raise _lib.AccelError(_lib.AB_ERR_INVALID, f"the rows name {len(held)} pages and {self._blocks - self.available()} "
                                   "are held; a compaction moves them all, so it needs every row in use")
+        for page in held:
+            if self.refs(page) == 0:
+                raise _lib.AccelError(_lib.AB_ERR_INVALID, f"a row names block {page}, which is free, and so leaves out one that is held")
         src, dst = np.zeros(self._blocks, np.uint32), np.zeros(self._blocks, np.uint32)
         n = _lib.check(_lib.lib().ab_blockpool_compact(self._h, src.ctypes.data, dst.ctypes.data))
         to = {int(s): int(d) for s, d in zip(src[:n], dst[:n])}

@@ -144,3 +144,17 @@ def test_compaction_wants_every_row():
     assert p.available() == 4
     rows, src, dst = p.compact([[NONE, a[1]], b])
     assert len(src) == len(dst) and {x for r in rows for x in r} == {NONE, 0, 1, 2, 3}
+
+
+def test_compaction_refuses_rows_that_name_pages_nobody_holds():
+    p = BlockPool(8, 4)
+    other = p.grow(None, 8)
+    a = p.grow(None, 8)
+    p.free([other[0]])
+    for rows in ([[*a, other[0]]], [[a[0]], [a[1], 7 if 7 not in a + other else 6]], [[*a, 8]]):
+        free = p.available()
+        with pytest.raises(_lib.AccelError):            # as many as are held, and not those: other[1] would move unseen
+            p.compact(rows)
+        assert p.available() == free and all(p.refs(x) == 1 for x in (*a, other[1]))
+    rows, src, dst = p.compact([a, [other[1], NONE]])
+    assert sorted(x for r in rows for x in r if x != NONE) == [0, 1, 2] and len(src) == len(dst)
