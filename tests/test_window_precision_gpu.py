@@ -192,3 +192,57 @@ def test_values_that_are_not_finite_beside_large_ones():
             else:
                 o, b = attend(q[i, h:h + 1], k[:, kvh:kvh + 1], v[:, kvh:kvh + 1], seen, attn_scale(D), 1)
                 check(got[i, h:h + 1], o, b, f"row {i} head {h}")
+
+
+@pytest.mark.parametrize("qH,kv,D", [(4, 4, 128), (4, 1, 64), (8, 1, 128), (20, 2, 40)])
+def test_single_tokens_over_channels_and_positions_far_apart(qH, kv, D):
+    # the row kernels' parts have f32's exponents: the same inputs without tiles
+    n, window, sinks = 900, 700, 4
+    rng = np.random.default_rng(D)
+    k, v = (rng.standard_normal((n, kv, D)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((3, qH, D)).astype(np.float32)
+    k[..., ::2] *= FAR
+    q[..., ::2] /= FAR
+    v[..., 7] *= np.float32(1e12)
+    v[50], v[190] = 1e9, -1e30                                     # positions that no row sees
+    base = n - 3
+    got = T.attention(dev(q), dev(k), dev(v), T.AttentionOptions(
+        lengths=dev(np.array([n], np.uint32)), scale=attn_scale(D), base=base, window=window, sinks=sinks)).cpu().numpy()
+    assert "tcgen05 tiles" not in rt.last_selection()
+    rest = [d for d in range(D) if d != 7]
+    for i in range(3):
+        want, bound = attend(q[i], k, v, visible(base + i, n, window, sinks), attn_scale(D), qH // kv)
+        for part in ([7], rest):
+            check(got[i][:, part], want[:, part], bound[:, part], f"row {i}")
+
+
+def test_tiles_far_apart_repeat_their_bits_on_any_stream_and_in_graphs():
+    def job(seed):
+        rng = np.random.default_rng(seed)
+        k, v = (rng.standard_normal((400, 2, 128)).astype(np.float32) for _ in range(2))
+        q = rng.standard_normal((300, 8, 128)).astype(np.float32)
+        v[150:160] *= np.float32(1e8)
+        k[300:, :, ::2] *= FAR
+        k, v, q = dev(k), dev(v), dev(q)
+        o = T.AttentionOptions(lengths=dev(np.array([400], np.uint32)), scale=0.09, base=100, window=90, sinks=4)
+        return lambda: T.attention(q, k, v, o)
+
+    jobs = [job(1), job(2)]
+    want = [j().cpu() for j in jobs]
+    graphs, outs = [], []
+    for j in jobs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(j())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in jobs]
+    eager = []
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for g, s, j in zip(graphs, streams, jobs):
+            with torch.cuda.stream(s):
+                g.replay()
+                eager.append(j())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o.cpu(), w) for o, w in zip(outs, want))
+    assert all(torch.equal(e.cpu(), want[i % 2]) for i, e in enumerate(eager))
