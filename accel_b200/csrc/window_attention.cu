@@ -111,11 +111,12 @@ __device__ __forceinline__ uint32_t win_row(const WinParams &p, const WinView &w
 //     S^T[16 positions x 8 heads] = K Q^T,      O^T[dims x 8 heads] += V^T P^T
 // and a running maximum and sum per warp; the warps are joined through shared memory and the CTAs of the
 // cluster through distributed shared memory, in a fixed order, so one launch does it all without a
-// workspace and repeats its bits.  HBM bounds it: the list is read once for all heads of the group.
+// workspace and repeats its bits.  HBM bounds it: the list is read once for up to eight heads of a group.  (An f32 cache with
+// groups above four is bound by splitting its operands instead: see the lane kernel.)
 //
 // The products keep f32 accuracy.  An operand is held as a high and a low part of 11 bits each (tf32 for
 // an f32 cache, f16 for an f16 cache, whose K and V are exact in one part); the product of the two low
-// parts, 2^-22, is dropped.  Every tile's products start from zero and the smaller ones come first; the
+// parts, 2^-22, is dropped.  (f16 has fewer exponents: QFrag, kWeightBias.)  Every tile's products start from zero and the smaller ones come first; the
 // sums over tiles are f32 additions outside the tensor core.
 //
 // Measured: 32 rows over up to 4112 f16 positions of 8 KV heads, groups of 4, 536 MB: 96 to 99 us, 5.5 TB/s.
@@ -123,7 +124,8 @@ __device__ __forceinline__ uint32_t win_row(const WinParams &p, const WinView &w
 constexpr int kRowWarps = 4;
 constexpr int kTile = 16;
 // an f16 cache's weights are carried times 2^14: the low part of a small one would otherwise meet f16's
-// smallest step; they are at most 1, and the quotient by their sum does not change
+// smallest step; they are at most 1, and the quotient by their sum does not change.  One below 2^-17 of the largest so far is off
+// by 2^-39 of that
 constexpr float kWeightBias = 14.f;
 
 // Row strides of the tiles in shared memory, in bytes: f32 K is read as 16 bytes of two neighbouring rows by a quarter
@@ -222,7 +224,7 @@ template <int DP> struct QFrag<float, DP> {
 template <int DP> struct QFrag<__half, DP> {
     uint32_t hi[DP / 8], lo[DP / 8];
     // f16 has 5 bits of exponent: a head's q is scaled by a power of two that brings its largest element into [2^13, 2^14),
-    // so that one of 2^-17 of it still keeps 22 bits in its two parts, and one below that 2^-39 of the largest.  (The sums stay
+    // so that one of 2^-16 of it still keeps 22 bits in its two parts, and one below that 2^-38 of the largest.  (The sums stay
     // below 2^38.  Near one instead, the channels of a query at a thousandth of its largest would keep 15 bits)
     __device__ __forceinline__ void load(const float *q, bool on, uint32_t D, int t, float scale, float (&undo)[2])
     {

@@ -13,7 +13,7 @@
 // part and its products take two.  Powers of two keep the parts inside f16's range: one per query row
 // and one per tile of an f32 cache; the softmax weights are carried times 2^14 (window_attention.cu).  Of an f32
 // cache, a tile whose elements lie too far apart for that goes to the CUDA cores (kReach, kSpread).  With an f16 cache an element
-// of a query is off by at most 2^-39 of the row's largest element, and a weight by 2^-39 of the row's largest weight.
+// of a query is off by at most 2^-38 of the row's largest element, and a weight by 2^-38 of the row's largest weight.
 // The accumulators of a tile start from zero, the small products first, and the sums over tiles are
 // f32 additions in registers: an accumulator in the tensor core over thousands of positions would
 // truncate at every step.
@@ -27,7 +27,7 @@
 //
 // Measured, the tile kernel alone: 4096 tokens of 32 heads over windows of 2048, f16 cache, groups of 4, 225 us, which is
 // 0.92 PFLOP/s of issued products (the MMAs and copies without the softmax: 196 us); 4096 tokens behind 4096 over windows of
-// 4096, f32 cache, 32 heads, 685 us, 1.21 PFLOP/s issued (592 us: there the tiles from L2, 33 bytes a clock and SM).
+// 4096, f32 cache, 32 heads, 695 us, 1.19 PFLOP/s issued (592 us: there the tiles from L2, 33 bytes a clock and SM).
 #include <algorithm>
 #include <math_constants.h>
 
@@ -57,11 +57,11 @@ struct TileHead {
     uint32_t seen[4];                       // a bit per position: it exists
 };
 constexpr uint32_t kBad = 1, kApart = 2;
-// An f32 tile's parts share one power of two, so an element below 2^-17 of the tile's largest is held to 2^-39 of that
+// An f32 tile's parts share one power of two, so an element below 2^-16 of the tile's largest is held to 2^-38 of that
 // largest and not to 22 bits of its own.  Two conditions say where that is as good as f32; rows for which one fails have that
 // tile's scores and values summed in f32 on the CUDA cores instead (exact_tile).
-// Keys and queries: a score is off by at most 2^-39 (largest key * sum |q| + largest |q| * sum |key|) beside what 22 bits of
-// every operand give; up to kReach of that product the error stays below 2^-23 of one, in the exponent of a weight.
+// Keys and queries: a score is off by at most 2^-38 (largest key * sum |q| + largest |q| * sum |key|) beside what 22 bits of
+// every operand give; while that sum of products is below kReach the error is below 2^-22, in the exponent of a weight.
 // Values: no position's and no dimension's largest magnitude (but for those that are all zero) lies more than kSpread binary
 // places below the tile's largest.  What is lost is then at most 2^-24 of the largest element of the position and of the dimension.
 constexpr float kReach = 65536.f;
@@ -141,7 +141,7 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo
 // grid (tiles, KV heads of this pass, 2): K or V of one tile.  An operand's element (r, c), c along the contraction, lies
 // at (c / 8) * rows * 16 + r * 16 + (c % 8) * 2: 128 rows of positions for K, DP rows of dimensions for V.
 // Every element is read once and written once per part: HBM (or L2) bounds it.
-// Measured: 8192 f32 positions of 32 heads, 537 MB in 112 us (4.8 TB/s); 4096 f16 positions of 8 heads, 33.5 MB in 11.5 us,
+// Measured: 8192 f32 positions of 32 heads, 537 MB in 107 us (5.0 TB/s); 4096 f16 positions of 8 heads, 33.5 MB in 11.5 us,
 // where the values of an f16 cache stay as they are, a copy in another order (16.3 us through f32 registers).
 constexpr int kPackThreads = 512;
 
@@ -714,7 +714,7 @@ win_tile_kernel(const WinParams p, const TilePlan plan, const unsigned char *til
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             amax = fminf(amax * fabsf(p.scale_log2), 3.402823466e38f);
-            // [2^13, 2^14), as the keys: an element down to 2^-17 of the row's largest keeps all its bits, and the products (2^37 with
+            // [2^13, 2^14), as the keys: an element down to 2^-16 of the row's largest keeps all its bits, and the products (2^37 with
             // f16's largest keys) stay far inside f32.  (Near one, 2^-25 of the largest was all that the small ones were held to)
             const int e = fit_exponent(amax);
             const float f = ab_pow2(e);

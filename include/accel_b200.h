@@ -250,7 +250,10 @@ AB_API uint64_t ab_launch_count(void);
  *                    read, and a visible position whose page is outside the cache counts as masked.  Capacity is the
  *                    cache's positions: its element count may pass 32 bits, and a length of 0xffffffff in the lengths
  *                    block says that many or more.  A row that sees nothing is NaN, ragged padding is zeros.
- *                    A row that sees a key or a value that is not finite comes out NaN or infinite; other rows do not.
+ *                    A row that sees a value that is not finite comes out NaN or infinite, and so does one that sees such a
+ *                    key, unless that key's score is -inf, which may count as a weight of 0.  Rows that see neither are not
+ *                    touched by them.  An f32 cache is taken at f32 accuracy; a prefill or chunk over one whose keys,
+ *                    queries or values lie far apart in size (from a factor of about 2^15) takes longer.
  *  TokenLogprobs, TokenLogprobsF16   logits f32 | f16 [Rows*Vocab], targets u32[Rows*Targets], logprobs f32[Rows*Targets],
  *                    entropy f32[Rows], top_ids u32[Rows*Top], top_logprobs f32[Rows*Top]   {Vocab,Rows,Targets,Top}@0..12
  *                    (16 B).  No reference kernels: log softmax of the targets, the distribution's entropy in nats, and
